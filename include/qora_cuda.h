@@ -38,6 +38,7 @@ extern "C" {
 typedef struct qora_ctx qora_ctx;             /* per-device context */
 typedef struct qora_w4 qora_w4;               /* device Q4 weight */
 typedef struct qora_kv qora_kv;               /* device KV cache, `streams` slabs */
+typedef struct qora_kv4 qora_kv4;             /* device KV cache in 4 bits, paged */
 typedef struct qora_talker qora_talker;       /* device TalkerWeights */
 typedef struct qora_predictor qora_predictor; /* device CodePredictorWeights */
 typedef struct qora_engine qora_engine;       /* per-GPU frame-loop state */
@@ -231,6 +232,82 @@ int qora_kv_attend_noalloc(qora_kv *kv, int32_t layer, const float *qkv, int32_t
                            const float *rope_sin, int32_t rope_max_pos, const int32_t *positions,
                            int32_t B, int32_t advance, float *out, void *stream);
 
+/* ------------------------------------------------------- 4-bit KV cache */
+/* No counterpart in the reference (its cache is f32).  A paged cache whose keys
+ * (after qk-norm and RoPE) and values are held in 4 bits: per position, kv head
+ * and group of 32 dimensions an f16 scale s = f16(amax / 7) and codes round(x /
+ * s) in [-7, 7] (ties to even), 144 bytes per position and kv head at head_dim
+ * 128 where the f32 cache has 1024.  A group that holds an infinity or NaN
+ * reads back as NaN.  Lengths and block tables live on the device and every
+ * call below but _create, _destroy and _lengths_host is asynchronous on
+ * `stream` and may be captured into a CUDA graph, so a step whose lengths
+ * depend on the step before (drafted tokens that were accepted) needs no
+ * return to the host:
+ *     _reserve -> per layer: _append, _attend -> qora_verify_drafts -> _advance.
+ * max_pos <= 2^20; streams <= 4096; head_dim 64 or 128; num_heads a multiple of
+ * kv_heads; page_positions a power of two >= 32; pool_pages <= 2^20, and
+ * pool_pages * page_positions < 2^31 (slots are int32). */
+int qora_kv4_create(qora_ctx *ctx, int32_t num_layers, int32_t num_heads, int32_t kv_heads,
+                    int32_t head_dim, int32_t max_pos, int32_t streams, int32_t page_positions,
+                    int32_t pool_pages, qora_kv4 **out);
+void qora_kv4_destroy(qora_kv4 *kv);
+/* Empties streams (a HOST array of ids; NULL: all): lengths become 0 and their
+ * pages are free for the next _reserve. */
+int qora_kv4_reset(qora_kv4 *kv, const int32_t *ids_host, int32_t count, void *stream);
+int qora_kv4_lengths_host(qora_kv4 *kv, int32_t *len_host, void *stream);
+/* Device pointers of the block table [streams][pages_per_stream] (-1: never
+ * mapped) and of the lengths [streams]. */
+int qora_kv4_state(qora_kv4 *kv, int32_t **table, int32_t *pages_per_stream, int32_t **lengths);
+/* Maps pages for counts[b] >= 0 new tokens of every stream (device int32
+ * [streams]) behind its length, and lists the tokens in stream order: offsets
+ * [streams + 1] (stream b has tokens offsets[b] .. offsets[b + 1]), positions
+ * and slots [max_tokens] (slot = page * page_positions + position in the page).
+ * From the last token on slots are -1, which _append, _write and _read skip,
+ * and positions 0: a captured step may have fewer tokens than rows.  A page is
+ * free when no stream's table names it below that stream's length.  Lengths do
+ * not change.  All or nothing: when a length would pass max_pos (QORA_ERR_RANGE),
+ * the tokens pass max_tokens (QORA_ERR_RANGE) or the pool has too few free
+ * pages (QORA_ERR_OOM; each at the next qora_ctx_check_device_error), no page
+ * is mapped, offsets are all 0 and slots all -1. */
+int qora_kv4_reserve(qora_kv4 *kv, const int32_t *counts, int32_t max_tokens, int32_t *slots,
+                     int32_t *positions, int32_t *offsets, void *stream);
+/* Adds counts[b] (device; negative: rolls back) to every stream's length.  A
+ * length that would leave [0, max_pos] stops there and is QORA_ERR_RANGE at the
+ * next qora_ctx_check_device_error. */
+int qora_kv4_advance(qora_kv4 *kv, const int32_t *counts, void *stream);
+/* qk-norm, RoPE and the cache append of one layer (talker.rs:285-303) for
+ * `tokens` rows: qkv [tokens][(num_heads + 2 kv_heads) head_dim] raw
+ * projections, as qora_kv_attend takes them; positions and slots per row
+ * (slots distinct).  k and v are stored in 4 bits at the slot; q_out [tokens]
+ * [num_heads head_dim] receives the normed and rotated queries.  A row whose
+ * slot is -1 is skipped (its q_out row is left as it was); one whose slot lies
+ * outside the pool or whose position outside the RoPE table is skipped and
+ * QORA_ERR_RANGE at the next qora_ctx_check_device_error. */
+int qora_kv4_append(qora_kv4 *kv, int32_t layer, const float *qkv, const uint16_t *q_norm,
+                    const uint16_t *k_norm, const float *rope_cos, const float *rope_sin,
+                    int32_t rope_max_pos, const int32_t *positions, const int32_t *slots,
+                    int32_t tokens, float *q_out, void *stream);
+/* Stores rows of keys (normed and rotated) and values [rows][kv_heads head_dim]
+ * f32 in 4 bits at their slots, e.g. those of an f32 cache; _read gives the
+ * values that slots hold.  Slots as in _append.  Writing what was read stores
+ * the same codes and scales. */
+int qora_kv4_write(qora_kv4 *kv, int32_t layer, const int32_t *slots, int32_t rows, const float *k,
+                   const float *v, void *stream);
+int qora_kv4_read(qora_kv4 *kv, int32_t layer, const int32_t *slots, int32_t rows, float *k,
+                  float *v, void *stream);
+/* Attention of one layer for the new tokens of every stream (talker.rs:304-331):
+ * q [tokens][num_heads head_dim] normed and rotated, offsets as _reserve wrote
+ * them; token i of stream b attends to positions 0 .. length[b] + i, its own
+ * included (append before).  out [tokens][num_heads head_dim]; rows behind the
+ * last token are left as they were.  A stream whose rows do not lie in [0, tokens) or
+ * whose tokens would pass max_pos is skipped, and a page outside the pool reads
+ * as some other page; both are QORA_ERR_RANGE at the next
+ * qora_ctx_check_device_error.  max_count: the most tokens that one stream
+ * has in this call as the host knows it (1 in a decode step), by which the
+ * kernel is chosen; any value >= 1 gives right results.  Deterministic. */
+int qora_kv4_attend(qora_kv4 *kv, int32_t layer, const float *q, const int32_t *offsets,
+                    int32_t tokens, int32_t max_count, float *out, void *stream);
+
 /* ------------------------------------------------------------ save.rs */
 /* load_model (save.rs:262-409; records gemv.rs:595-687): maps a .qora-tts
  * checkpoint (Q4 format) read-only and parses its talker and code-predictor
@@ -324,6 +401,34 @@ int qora_predictor_embed_sum(qora_predictor *p, const uint32_t *codes, int32_t B
 int qora_sample(qora_ctx *ctx, const float *logits, int32_t B, int32_t V, const uint32_t *prev,
                 int32_t n_prev, uint64_t *rng, const qora_sample_params *params, uint32_t *out,
                 void *stream);
+
+/* The distribution that sample_token draws from (generate_new.rs:771-851) for B
+ * rows of V logits: probs [B][V], after repetition penalty, temperature,
+ * softmax, top-k and top-p, zero where a token is out.  Same parameters and
+ * limits as qora_sample, with vocabularies up to 327680.  Among equal logits the lower index counts
+ * as larger.  A row with a NaN or +infinite logit, or with no finite one, gives
+ * zeros and QORA_ERR_INVALID at the next qora_ctx_check_device_error. */
+int qora_sample_probs(qora_ctx *ctx, const float *logits, int32_t B, int32_t V,
+                      const uint32_t *prev, int32_t n_prev, const qora_sample_params *params,
+                      float *probs, void *stream);
+/* Speculative verification (no counterpart in the reference): keeps the
+ * target's distribution exactly.  Per stream b: K drafted tokens drafts [B][K]
+ * (the first counts[b] of them; counts NULL: all K), drawn from draft_probs
+ * [B][K][V] (NULL: a deterministic draft), the target's target_probs [B][K + 1][V]
+ * at the same positions and one behind, and given uniforms [B][K + 1] in [0, 1).
+ * Draft i is accepted when uniforms[i] * draft_prob < target_prob; at the first
+ * that is not (place a), a token is drawn from max(target - draft, 0)
+ * normalised (the target without the draft when draft_probs is NULL; the target
+ * when nothing is left), and when all counts[b] = a pass, from target row a: the
+ * first index whose cumulative sum passes uniforms[K] times the sum.  Sums are in
+ * 64 bits.  tokens [B][K + 1] = the a accepted drafts, the drawn token, then
+ * -1; n_out [B] = a + 1.  A draft outside [0, V) is rejected, a count outside
+ * [0, K] clamped, and both are QORA_ERR_RANGE at the next
+ * qora_ctx_check_device_error. */
+int qora_verify_drafts(qora_ctx *ctx, const int32_t *drafts, const float *draft_probs,
+                       const float *target_probs, const int32_t *counts, const float *uniforms,
+                       int32_t B, int32_t K, int32_t V, int32_t *tokens, int32_t *n_out,
+                       void *stream);
 
 /* The frame loop (generate_new.rs:606-665) for B streams on one GPU: sample
  * code0 -> semantic embedding -> predictor (15 codes) -> embedding sum +

@@ -7,6 +7,7 @@ pub const QORA_OK: c_int = 0;
 #[repr(C)] pub struct qora_ctx { _p: [u8; 0] }
 #[repr(C)] pub struct qora_w4 { _p: [u8; 0] }
 #[repr(C)] pub struct qora_kv { _p: [u8; 0] }
+#[repr(C)] pub struct qora_kv4 { _p: [u8; 0] }
 #[repr(C)] pub struct qora_talker { _p: [u8; 0] }
 #[repr(C)] pub struct qora_predictor { _p: [u8; 0] }
 #[repr(C)] pub struct qora_engine { _p: [u8; 0] }
@@ -144,6 +145,32 @@ extern "C" {
                                   rope_max_pos: i32, positions: *const i32, b: i32,
                                   advance: i32, out: *mut f32, stream: *mut c_void) -> c_int;
 
+    pub fn qora_kv4_create(ctx: *mut qora_ctx, num_layers: i32, num_heads: i32, kv_heads: i32,
+                           head_dim: i32, max_pos: i32, streams: i32, page_positions: i32,
+                           pool_pages: i32, out: *mut *mut qora_kv4) -> c_int;
+    pub fn qora_kv4_destroy(kv: *mut qora_kv4);
+    pub fn qora_kv4_reset(kv: *mut qora_kv4, ids_host: *const i32, count: i32,
+                          stream: *mut c_void) -> c_int;
+    pub fn qora_kv4_lengths_host(kv: *mut qora_kv4, len_host: *mut i32,
+                                 stream: *mut c_void) -> c_int;
+    pub fn qora_kv4_state(kv: *mut qora_kv4, table: *mut *mut i32, pages_per_stream: *mut i32,
+                          lengths: *mut *mut i32) -> c_int;
+    pub fn qora_kv4_reserve(kv: *mut qora_kv4, counts: *const i32, max_tokens: i32,
+                            slots: *mut i32, positions: *mut i32, offsets: *mut i32,
+                            stream: *mut c_void) -> c_int;
+    pub fn qora_kv4_advance(kv: *mut qora_kv4, counts: *const i32, stream: *mut c_void) -> c_int;
+    pub fn qora_kv4_append(kv: *mut qora_kv4, layer: i32, qkv: *const f32, q_norm: *const u16,
+                           k_norm: *const u16, rope_cos: *const f32, rope_sin: *const f32,
+                           rope_max_pos: i32, positions: *const i32, slots: *const i32,
+                           tokens: i32, q_out: *mut f32, stream: *mut c_void) -> c_int;
+    pub fn qora_kv4_write(kv: *mut qora_kv4, layer: i32, slots: *const i32, rows: i32,
+                          k: *const f32, v: *const f32, stream: *mut c_void) -> c_int;
+    pub fn qora_kv4_read(kv: *mut qora_kv4, layer: i32, slots: *const i32, rows: i32,
+                         k: *mut f32, v: *mut f32, stream: *mut c_void) -> c_int;
+    pub fn qora_kv4_attend(kv: *mut qora_kv4, layer: i32, q: *const f32, offsets: *const i32,
+                           tokens: i32, max_count: i32, out: *mut f32,
+                           stream: *mut c_void) -> c_int;
+
     pub fn qora_talker_create(ctx: *mut qora_ctx, host: *const qora_talker_host,
                               max_batch: i32, out: *mut *mut qora_talker) -> c_int;
     pub fn qora_talker_destroy(t: *mut qora_talker);
@@ -194,6 +221,14 @@ extern "C" {
                        prev: *const u32, n_prev: i32, rng: *mut u64,
                        params: *const qora_sample_params, out: *mut u32,
                        stream: *mut c_void) -> c_int;
+
+    pub fn qora_sample_probs(ctx: *mut qora_ctx, logits: *const f32, b: i32, v: i32,
+                             prev: *const u32, n_prev: i32, params: *const qora_sample_params,
+                             probs: *mut f32, stream: *mut c_void) -> c_int;
+    pub fn qora_verify_drafts(ctx: *mut qora_ctx, drafts: *const i32, draft_probs: *const f32,
+                              target_probs: *const f32, counts: *const i32,
+                              uniforms: *const f32, b: i32, k: i32, v: i32, tokens: *mut i32,
+                              n_out: *mut i32, stream: *mut c_void) -> c_int;
 
     pub fn qora_engine_create(t: *mut qora_talker, p: *mut qora_predictor, b: i32,
                               max_pos: i32, params: *const qora_sample_params,

@@ -209,6 +209,7 @@ int qora_ctx_check_device_error(qora_ctx *ctx, void *stream) {
     QORA_CUDA(cudaStreamSynchronize(st));
     switch (v) {
         case kDevRange: return set_error(QORA_ERR_RANGE, "device: position past RoPE table or KV capacity");
+        case kDevPool: return set_error(QORA_ERR_OOM, "device: 4-bit KV cache out of pages");
         case kDevNaN: return set_error(QORA_ERR_INVALID, "device: NaN reached argmax/sampler");
         case kDevTimeout: return set_error(QORA_ERR_TIMEOUT, "device: bounded wait expired");
         case kDevF16Range:

@@ -72,6 +72,7 @@ enum DeviceError : int {
     kDevRange = 1,   // position past the RoPE table or KV capacity
     kDevNaN = 2,     // NaN logits reached an argmax / sampler
     kDevTimeout = 3, // bounded wait expired
+    kDevPool = 5,    // the 4-bit cache's page pool is exhausted
     kDevF16Range = 4,// an infinite input row value reached the tensor-core GEMV operands
 };
 

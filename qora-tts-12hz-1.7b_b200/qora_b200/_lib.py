@@ -107,6 +107,17 @@ SIGNATURES = {
                                   _vp, _vp]),
     "qora_kv_attend_noalloc": (C.c_int, [_vp, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _i32, _vp, _i32,
                                           _i32, _vp, _vp]),
+    "qora_kv4_create": (C.c_int, [_vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _PP]),
+    "qora_kv4_destroy": (None, [_vp]),
+    "qora_kv4_reset": (C.c_int, [_vp, _vp, _i32, _vp]),
+    "qora_kv4_lengths_host": (C.c_int, [_vp, _vp, _vp]),
+    "qora_kv4_state": (C.c_int, [_vp, _PP, C.POINTER(C.c_int32), _PP]),
+    "qora_kv4_reserve": (C.c_int, [_vp, _vp, _i32, _vp, _vp, _vp, _vp]),
+    "qora_kv4_advance": (C.c_int, [_vp, _vp, _vp]),
+    "qora_kv4_append": (C.c_int, [_vp, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _i32, _vp, _vp]),
+    "qora_kv4_write": (C.c_int, [_vp, _i32, _vp, _i32, _vp, _vp, _vp]),
+    "qora_kv4_read": (C.c_int, [_vp, _i32, _vp, _i32, _vp, _vp, _vp]),
+    "qora_kv4_attend": (C.c_int, [_vp, _i32, _vp, _vp, _i32, _i32, _vp, _vp]),
     "qora_model_file_open": (C.c_int, [C.c_char_p, _PP]),
     "qora_model_file_talker": (C.c_int, [_vp, _vp]),
     "qora_model_file_predictor": (C.c_int, [_vp, _vp]),
@@ -128,6 +139,8 @@ SIGNATURES = {
     "qora_predictor_frame": (C.c_int, [_vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp]),
     "qora_predictor_embed_sum": (C.c_int, [_vp, _vp, _i32, _vp, _vp]),
     "qora_sample": (C.c_int, [_vp, _vp, _i32, _i32, _vp, _i32, _vp, _vp, _vp, _vp]),
+    "qora_sample_probs": (C.c_int, [_vp, _vp, _i32, _i32, _vp, _i32, _vp, _vp, _vp]),
+    "qora_verify_drafts": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp, _vp]),
     "qora_engine_create": (C.c_int, [_vp, _vp, _i32, _i32, _vp, _PP]),
     "qora_engine_destroy": (None, [_vp]),
     "qora_engine_prefill": (C.c_int, [_vp, _vp, _i32, _vp, _vp]),

@@ -364,6 +364,50 @@ def sample_token(ctx: Context, logits: torch.Tensor, prev: torch.Tensor | None,
     return out
 
 
+def _rows_of(name: str, t: torch.Tensor, dtype, shape) -> int:
+    if t.dtype != dtype or tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name}: expected {tuple(shape)} of {dtype}, got {tuple(t.shape)} of {t.dtype}")
+    return _dp(t)
+
+
+def sample_probs(ctx: Context, logits: torch.Tensor, prev: torch.Tensor | None, params: _lib.SampleParams,
+                 out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+    """The distribution that sample_token draws from (generate_new.rs:771-851)
+    for each row of logits [B][V]: [B][V], zero where top-k or top-p leave a
+    token out.  prev int32 [B][n] (repetition penalty) or None."""
+    B, V = logits.shape
+    out = out if out is not None else torch.empty_like(logits)
+    n_prev = 0 if prev is None else prev.shape[-1]
+    _lib.call("qora_sample_probs", ctx.h, _rows_of("logits", logits, torch.float32, (B, V)), B, V,
+              None if not n_prev else _rows_of("prev", prev, torch.int32, (B, n_prev)), n_prev,
+              C.byref(params), _rows_of("out", out, torch.float32, (B, V)), _stream(stream))
+    return out
+
+
+def verify_drafts(ctx: Context, drafts: torch.Tensor, draft_probs: torch.Tensor | None,
+                  target_probs: torch.Tensor, uniforms: torch.Tensor, counts: torch.Tensor | None = None,
+                  out=None, stream=None):
+    """Speculative verification (qora_verify_drafts): drafts int32 [B][K] drawn
+    from draft_probs [B][K][V] (None: deterministic), the target's probabilities
+    [B][K + 1][V], uniforms [B][K + 1] in [0, 1), counts int32 [B] (None: K
+    drafts each).  Returns tokens int32 [B][K + 1] (the accepted drafts, one
+    drawn token, then -1) and n_out int32 [B] (tokens of each stream)."""
+    B, K = drafts.shape
+    V = target_probs.shape[-1]
+    if out is None:
+        out = (torch.empty(B, K + 1, dtype=torch.int32, device=drafts.device),
+               torch.empty(B, dtype=torch.int32, device=drafts.device))
+    tokens, n_out = out
+    _lib.call("qora_verify_drafts", ctx.h, _rows_of("drafts", drafts, torch.int32, (B, K)),
+              None if draft_probs is None else _rows_of("draft_probs", draft_probs, torch.float32, (B, K, V)),
+              _rows_of("target_probs", target_probs, torch.float32, (B, K + 1, V)),
+              None if counts is None else _rows_of("counts", counts, torch.int32, (B,)),
+              _rows_of("uniforms", uniforms, torch.float32, (B, K + 1)), B, K, V,
+              _rows_of("tokens", tokens, torch.int32, (B, K + 1)), _rows_of("n_out", n_out, torch.int32, (B,)),
+              _stream(stream))
+    return out
+
+
 class Engine:
     """The frame loop (generate_new.rs:606-665) for B streams on one GPU."""
 
@@ -463,5 +507,5 @@ class _CudaArray:
                                          "data": (ptr, False), "version": 3, "strides": None}
 
 
-def _device_view(ptr: int, shape, typestr: str) -> torch.Tensor:
-    return torch.as_tensor(_CudaArray(ptr, shape, typestr), device="cuda")
+def _device_view(ptr: int, shape, typestr: str, device: str = "cuda") -> torch.Tensor:
+    return torch.as_tensor(_CudaArray(ptr, shape, typestr), device=device)
