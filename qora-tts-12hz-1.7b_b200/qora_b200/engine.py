@@ -500,12 +500,14 @@ class Engine:
 
 
 class _CudaArray:
-    """A raw device pointer described by __cuda_array_interface__ (no copy)."""
+    """A raw device pointer described by __cuda_array_interface__ (no copy).
+    A tensor made from it keeps it, and so `owner`, alive."""
 
-    def __init__(self, ptr: int, shape, typestr: str):
+    def __init__(self, ptr: int, shape, typestr: str, owner=None):
+        self.owner = owner
         self.__cuda_array_interface__ = {"shape": tuple(shape), "typestr": typestr,
                                          "data": (ptr, False), "version": 3, "strides": None}
 
 
-def _device_view(ptr: int, shape, typestr: str, device: str = "cuda") -> torch.Tensor:
-    return torch.as_tensor(_CudaArray(ptr, shape, typestr), device=device)
+def _device_view(ptr: int, shape, typestr: str, device: str = "cuda", owner=None) -> torch.Tensor:
+    return torch.as_tensor(_CudaArray(ptr, shape, typestr, owner), device=device)

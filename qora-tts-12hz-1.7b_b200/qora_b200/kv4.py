@@ -71,11 +71,11 @@ class Kv4Cache:
 
     def state(self) -> dict:
         """Views of the device state: table [streams][pages_per_stream] and
-        lengths [streams], int32.  They live as long as the cache."""
+        lengths [streams], int32.  A view keeps the cache alive."""
         table, per, lengths = C.c_void_p(), C.c_int32(), C.c_void_p()
         _lib.call("qora_kv4_state", self.h, C.byref(table), C.byref(per), C.byref(lengths))
-        return {"table": _device_view(table.value, (self.streams, per.value), "<i4", self.device),
-                "lengths": _device_view(lengths.value, (self.streams,), "<i4", self.device)}
+        return {"table": _device_view(table.value, (self.streams, per.value), "<i4", self.device, self),
+                "lengths": _device_view(lengths.value, (self.streams,), "<i4", self.device, self)}
 
     def reserve(self, counts: torch.Tensor, max_tokens: int, out=None, stream=None):
         """Maps pages for counts[b] new tokens per stream (int32 [streams]);

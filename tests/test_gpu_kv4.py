@@ -137,6 +137,23 @@ def test_rolled_back_pages_are_free_again(ctx):
     assert _error(ctx) == 0
 
 
+def test_state_views_keep_the_cache(ctx):
+    import gc
+    import weakref
+    kv = _cache(ctx, 1, 2, 1, 64, 64, 2, 32, 4)
+    alive, table = weakref.ref(kv), kv.state()["table"]
+    del kv
+    gc.collect()
+    assert alive() is not None and bool((table == -1).all())
+    row = table[0]
+    del table
+    gc.collect()
+    assert alive() is not None and bool((row == -1).all())
+    del row
+    gc.collect()
+    assert alive() is None
+
+
 # ------------------------------------------------------------ rows
 def _weights(orc, hd, seed):
     rng = np.random.default_rng(seed)
