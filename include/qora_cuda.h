@@ -278,7 +278,8 @@ int qora_kv4_advance(qora_kv4 *kv, const int32_t *counts, void *stream);
 /* qk-norm, RoPE and the cache append of one layer (talker.rs:285-303) for
  * `tokens` rows: qkv [tokens][(num_heads + 2 kv_heads) head_dim] raw
  * projections, as qora_kv_attend takes them; positions and slots per row
- * (slots distinct).  k and v are stored in 4 bits at the slot; q_out [tokens]
+ * (slots distinct; the float and f16 pointers of this call, _write, _read and
+ * _attend 16-byte aligned).  k and v are stored in 4 bits at the slot; q_out [tokens]
  * [num_heads head_dim] receives the normed and rotated queries.  A row whose
  * slot is -1 is skipped (its q_out row is left as it was); one whose slot lies
  * outside the pool or whose position outside the RoPE table is skipped and

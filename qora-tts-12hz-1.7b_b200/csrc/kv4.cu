@@ -1,9 +1,13 @@
 // The 4-bit paged KV cache: creation, block tables and slot maps built on the
 // GPU (k_kv4_reserve), the append with qk-norm and rotation (k_kv4_append),
 // plain writes and reads of rows, and the length update.
-#include "kv4.cuh"
+#include <cooperative_groups.h>
 
 #include <new>
+
+#include "kv4.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace qora {
 
@@ -17,7 +21,16 @@ namespace {
 // but lengths and table is kept between calls, so pages behind a length that
 // was rolled back are free again, and a call repeated before the lengths move
 // gives the same answer.
+//
+// One cluster does it all (one launch, no workspace).  Every block scans the
+// streams' counts for itself (they are few); the table entries are marked by
+// all warps, 256 entries at a time with eight loads in flight; each block then
+// joins its share of the bit maps through distributed shared memory and hands
+// out the free pages in it; tokens are spread over all threads, which look
+// their stream up in the scanned offsets.
 constexpr int kResThreads = 1024;
+constexpr int kResCluster = 8;
+constexpr int kResChunk = 256;  // table entries that a warp marks at a time
 
 struct ReserveArgs {
     const int *counts, *len;
@@ -25,22 +38,27 @@ struct ReserveArgs {
     int streams, max_pos, page_shift, pages_per_stream, pool_pages, max_tokens;
 };
 
-__device__ __forceinline__ int block_scan_excl(int v, int *wsum, int &total) {
+struct ReserveShared {
+    int64_t wsum[32];
+    int bad, free_pages;
+};
+
+__device__ __forceinline__ int64_t block_scan_excl(int64_t v, int64_t *wsum, int64_t &total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int x = v;
+    int64_t x = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
         if (lane >= o) x += y;
     }
     __syncthreads();
     if (lane == 31) wsum[warp] = x;
     __syncthreads();
     if (warp == 0) {
-        int w = wsum[lane];
+        int64_t w = wsum[lane];
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, w, o);
+            const int64_t y = __shfl_up_sync(0xffffffffu, w, o);
             if (lane >= o) w += y;
         }
         wsum[lane] = w;
@@ -50,126 +68,146 @@ __device__ __forceinline__ int block_scan_excl(int v, int *wsum, int &total) {
     return x - v + (warp ? wsum[warp - 1] : 0);
 }
 
+// The last index i with at[i] <= v (at[0] = 0 <= v).
+__device__ __forceinline__ int last_at_most(const int *at, int n, int v) {
+    int lo = 0, hi = n - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (at[mid] <= v) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
 __global__ void __launch_bounds__(kResThreads) k_kv4_reserve(const ReserveArgs a) {
-    extern __shared__ unsigned bits[];  // one bit per pool page: in use
-    __shared__ int wsum[32];
-    __shared__ int bad;
-    griddep_launch_dependents();
-    griddep_wait();
+    extern __shared__ int res_dyn[];
+    __shared__ ReserveShared sh;
+    cg::cluster_group cl = cg::this_cluster();
+    const int rank = (int)cl.block_rank(), nr = (int)cl.num_blocks();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int words = (a.pool_pages + 31) >> 5;
     const int P = 1 << a.page_shift;
-    if (tid == 0) bad = 0;
+    int *len = res_dyn;                   // [streams], -1 when the stream's request is bad
+    int *first = len + a.streams;         // [streams] ordinal of its first new page
+    int *off = first + a.streams;         // [streams] its first token
+    unsigned *bits = reinterpret_cast<unsigned *>(off + a.streams);  // [words] pages in use
+    griddep_launch_dependents();
+    griddep_wait();
+    if (tid == 0) sh.bad = 0;
     for (int w = tid; w < words; w += kResThreads) bits[w] = 0u;
     __syncthreads();
-    // mark, one warp per stream
-    for (int b = warp; b < a.streams; b += kResThreads / 32) {
-        const int len = a.len[b], n = a.counts[b];
-        if (len < 0 || n < 0 || len > a.max_pos || n > a.max_pos - len) {
-            if (lane == 0) atomicMax(&bad, kDevRange);
-            continue;
+    // ---- streams: tokens and new pages, scanned together (tokens in the high half)
+    int64_t base = 0;
+    for (int b0 = 0; b0 < a.streams; b0 += kResThreads) {
+        const int b = b0 + tid;
+        int64_t v = 0;
+        int l = 0;
+        if (b < a.streams) {
+            l = a.len[b];
+            const int n = a.counts[b];
+            if (l < 0 || n < 0 || l > a.max_pos || n > a.max_pos - l) {
+                sh.bad = kDevRange;
+                l = -1;
+            } else {
+                v = ((int64_t)n << 32) | (((l + n + P - 1) >> a.page_shift) - ((l + P - 1) >> a.page_shift));
+            }
         }
-        const int keep = (len + P - 1) >> a.page_shift;
-        for (int j = lane; j < keep; j += 32) {
-            const int pg = a.table[(int64_t)b * a.pages_per_stream + j];
-            if (pg < 0 || pg >= a.pool_pages) atomicMax(&bad, kDevRange);
-            else atomicOr(&bits[pg >> 5], 1u << (pg & 31));
+        int64_t total;
+        const int64_t at = base + block_scan_excl(v, sh.wsum, total);
+        if (b < a.streams) {
+            len[b] = l;
+            first[b] = (int)(at & 0xffffffff);
+            off[b] = (int)min(at >> 32, (int64_t)0x7fffffff);
         }
+        base += total;
     }
+    const int64_t tokens = base >> 32;
+    const int need = (int)(base & 0xffffffff);
     __syncthreads();
-    // totals: tokens and new pages
-    int64_t tokens = 0;
-    int need = 0, free_total = 0;
-    if (!bad) {
-        for (int b0 = 0; b0 < a.streams; b0 += kResThreads) {
-            const int b = b0 + tid;
-            int n = 0, k = 0;
-            if (b < a.streams) {
-                n = a.counts[b];
-                k = ((a.len[b] + n + P - 1) >> a.page_shift) - ((a.len[b] + P - 1) >> a.page_shift);
-            }
-            int t;
-            block_scan_excl(n, wsum, t);
-            tokens += t;
-            block_scan_excl(k, wsum, t);
-            need += t;
+    // ---- mark the pages in use
+    const int chunks = (a.pages_per_stream + kResChunk - 1) / kResChunk;
+    for (int p = rank * (kResThreads / 32) + warp; p < a.streams * chunks; p += nr * (kResThreads / 32)) {
+        const int b = p / chunks, j0 = (p - b * chunks) * kResChunk;
+        const int keep = (len[b] + P - 1) >> a.page_shift;
+        if (j0 >= keep) continue;
+        const int *t = a.table + (int64_t)b * a.pages_per_stream;
+        int pg[kResChunk / 32];
+#pragma unroll
+        for (int i = 0; i < kResChunk / 32; i++) {
+            const int j = j0 + i * 32 + lane;
+            pg[i] = j < keep ? __ldcg(t + j) : -2;
         }
-        for (int w0 = 0; w0 < words; w0 += kResThreads) {
-            const int w = w0 + tid;
-            int f = 0;
-            if (w < words) {
-                f = __popc(~bits[w]);
-                if (w == words - 1 && (a.pool_pages & 31)) f -= 32 - (a.pool_pages & 31);
-            }
-            int t;
-            block_scan_excl(f, wsum, t);
-            free_total += t;
+#pragma unroll
+        for (int i = 0; i < kResChunk / 32; i++) {
+            if (pg[i] == -2 && j0 + i * 32 + lane >= keep) continue;
+            if ((unsigned)pg[i] >= (unsigned)a.pool_pages) sh.bad = kDevRange;
+            else atomicOr(&bits[pg[i] >> 5], 1u << (pg[i] & 31));
         }
     }
-    const int why = bad ? bad : tokens > a.max_tokens ? kDevRange : need > free_total ? kDevPool : 0;
+    cl.sync();
+    // ---- this block's share of the pool: words [wa, wb)
+    const int share = (words + nr - 1) / nr;
+    const int wa = min(words, rank * share), wb = min(words, wa + share);
+    int mine = 0;
+    for (int w = wa + tid; w < wb; w += kResThreads) {
+        unsigned f = 0u;
+        for (int r = 0; r < nr; r++) f |= cl.map_shared_rank(bits, r)[w];
+        f = ~f;
+        if (w == words - 1 && (a.pool_pages & 31)) f &= (1u << (a.pool_pages & 31)) - 1u;
+        bits[w] = f;  // from here on: free pages (no other block reads these words)
+        mine += __popc(f);
+    }
+    int64_t total;
+    block_scan_excl(mine, sh.wsum, total);
+    if (tid == 0) sh.free_pages = (int)total;
+    cl.sync();
+    int ordinal = 0, free_total = 0, bad = 0;
+    for (int r = 0; r < nr; r++) {
+        const ReserveShared *o = cl.map_shared_rank(&sh, r);
+        if (r == rank) ordinal = free_total;
+        free_total += o->free_pages;
+        bad |= o->bad;
+    }
+    const int all = nr * kResThreads, me = rank * kResThreads + tid;
+    const int why = bad ? kDevRange : tokens > a.max_tokens ? kDevRange : need > free_total ? kDevPool : 0;
     if (why) {  // nothing is mapped, and every listed token is skipped
-        if (tid == 0) raise_error(a.err, why);
-        for (int b = tid; b <= a.streams; b += kResThreads) a.offsets[b] = 0;
-        for (int i = tid; i < a.max_tokens; i += kResThreads) {
+        if (me == 0) raise_error(a.err, why);
+        for (int b = me; b <= a.streams; b += all) a.offsets[b] = 0;
+        for (int i = me; i < a.max_tokens; i += all) {
             a.slots[i] = -1;
             a.positions[i] = 0;
         }
+        cl.sync();  // no block leaves while another reads its counts
         return;
     }
-    // the new pages: the i-th free page goes to the i-th new (stream, page)
-    __syncthreads();
-    int page_base = 0, tok_base = 0;
-    // (a) offsets, and each stream's first new page in ordinal order
-    for (int b0 = 0; b0 < a.streams; b0 += kResThreads) {
-        const int b = b0 + tid;
-        int n = 0;
-        if (b < a.streams) n = a.counts[b];
-        int t;
-        const int at = block_scan_excl(n, wsum, t);
-        if (b < a.streams) a.offsets[b] = tok_base + at;
-        tok_base += t;
-    }
-    if (tid == 0) a.offsets[a.streams] = tok_base;
-    // (b) free pages in ascending order: thread w hands out its word's pages
-    for (int w0 = 0; w0 < words; w0 += kResThreads) {
+    for (int b = me; b <= a.streams; b += all) a.offsets[b] = b < a.streams ? off[b] : (int)tokens;
+    // ---- the i-th free page goes to the i-th new (stream, page)
+    for (int w0 = wa; w0 < wb && ordinal < need; w0 += kResThreads) {
         const int w = w0 + tid;
-        unsigned f = w < words ? ~bits[w] : 0u;
-        if (w == words - 1 && (a.pool_pages & 31)) f &= (1u << (a.pool_pages & 31)) - 1u;
-        int t;
-        int at = page_base + block_scan_excl(__popc(f), wsum, t);
-        page_base += t;
-        while (f && at < need) {
-            const int pg = w * 32 + __ffs(f) - 1;
-            f &= f - 1;
-            // the stream that owns ordinal `at`: a walk over the streams' needs
-            int rest = at;
-            for (int b = 0; b < a.streams; b++) {
-                const int len = a.len[b];
-                const int keep = (len + P - 1) >> a.page_shift;
-                const int k = ((len + a.counts[b] + P - 1) >> a.page_shift) - keep;
-                if (rest < k) {
-                    a.table[(int64_t)b * a.pages_per_stream + keep + rest] = pg;
-                    break;
-                }
-                rest -= k;
+        unsigned f = w < wb ? bits[w] : 0u;
+        int at = ordinal + (int)block_scan_excl(__popc(f), sh.wsum, total);
+        ordinal += (int)total;
+        if (f && at < need) {
+            int b = last_at_most(first, a.streams, at);
+            for (; f && at < need; at++, f &= f - 1) {
+                while (b + 1 < a.streams && first[b + 1] <= at) b++;
+                const int keep = (len[b] + P - 1) >> a.page_shift;
+                __stcg(a.table + (int64_t)b * a.pages_per_stream + keep + (at - first[b]), w * 32 + __ffs(f) - 1);
             }
-            at++;
         }
     }
-    __syncthreads();
-    // (c) the tokens' slots and positions, one warp per stream
-    for (int b = warp; b < a.streams; b += kResThreads / 32) {
-        const int len = a.len[b], n = a.counts[b], off = a.offsets[b];
-        for (int i = lane; i < n; i += 32) {
-            const int pos = len + i;
-            const int pg = a.table[(int64_t)b * a.pages_per_stream + (pos >> a.page_shift)];
-            a.slots[off + i] = (pg << a.page_shift) + (pos & (P - 1));
-            a.positions[off + i] = pos;
+    cl.sync();
+    // ---- the tokens' slots and positions
+    for (int i = me; i < a.max_tokens; i += all) {
+        int slot = -1, pos = 0;
+        if (i < tokens) {
+            const int b = last_at_most(off, a.streams, i);
+            pos = len[b] + i - off[b];
+            const int pg = __ldcg(a.table + (int64_t)b * a.pages_per_stream + (pos >> a.page_shift));
+            slot = (pg << a.page_shift) + (pos & (P - 1));
         }
-    }
-    for (int i = tok_base + tid; i < a.max_tokens; i += kResThreads) {
-        a.slots[i] = -1;
-        a.positions[i] = 0;
+        a.slots[i] = slot;
+        a.positions[i] = pos;
     }
 }
 
@@ -185,119 +223,127 @@ __global__ void k_kv4_advance(int *len, const int *counts, int streams, int max_
 }
 
 // ------------------------------------------------------------ rows
-// A warp holds one head vector: lane l has dimensions E l + e (e < E = D/64)
-// of the first half and the same of the second half, so the rotation's pairs
-// (i, i + D/2) lie in one lane.
+// D/8 lanes hold one head vector (a warp two or four of them): lane l of a head
+// has dimensions 4l .. 4l + 3 of each half, so the rotation's pairs (i, i + D/2)
+// and the four codes of a stored halfword lie in one lane, loads and stores are
+// 16 bytes, and a scale group is eight lanes.
+template <int D>
+struct Angles {
+    float4 c, s;
+    __device__ __forceinline__ void load(const float *cs, const float *sn, int l) {
+        c = __ldg(reinterpret_cast<const float4 *>(cs) + l);
+        s = __ldg(reinterpret_cast<const float4 *>(sn) + l);
+    }
+};
+
 template <int D>
 struct HeadVec {
-    static constexpr int E = D / 64;
-    float x[2][E];
+    static constexpr int kLanes = D / 8;
+    float x[2][4];
 
-    __device__ __forceinline__ void load(const float *p, int lane) {
+    __device__ __forceinline__ void load(const float *p, int l) {
 #pragma unroll
-        for (int h = 0; h < 2; h++)
-#pragma unroll
-            for (int e = 0; e < E; e++) x[h][e] = p[h * (D / 2) + E * lane + e];
+        for (int h = 0; h < 2; h++) {
+            const float4 v = __ldcs(reinterpret_cast<const float4 *>(p + h * (D / 2)) + l);
+            x[h][0] = v.x, x[h][1] = v.y, x[h][2] = v.z, x[h][3] = v.w;
+        }
     }
-    __device__ __forceinline__ void store(float *p, int lane) const {
+    __device__ __forceinline__ void store(float *p, int l) const {
 #pragma unroll
         for (int h = 0; h < 2; h++)
-#pragma unroll
-            for (int e = 0; e < E; e++) p[h * (D / 2) + E * lane + e] = x[h][e];
+            reinterpret_cast<float4 *>(p + h * (D / 2))[l] = make_float4(x[h][0], x[h][1], x[h][2], x[h][3]);
     }
 
-    // RMS norm over the head and rotation by the position's angles.  In 64
-    // bits: a key's 4-bit codes are decided next to borders, where the f32
-    // rounding of these sums would move one code in a million by a whole step.
-    // The result is rounded to f32 once.
-    __device__ __forceinline__ void norm_rope(const __half *gamma, const float *cs, const float *sn, int lane) {
-        double ss = 0.0;
+    // RMS norm over the head and rotation by the position's angles, rounded to
+    // f32 at the end.  Keys take T = double: their 4-bit codes are decided next
+    // to borders, where the f32 rounding of these sums would move one code in a
+    // million by a whole step.  Queries take T = float (f64's conversions are
+    // the slowest part of a key: half the heads are queries).
+    template <class T>
+    __device__ __forceinline__ void norm_rope(const __half *gamma, const Angles<D> &ang, int l) {
+        T ss = 0;
 #pragma unroll
         for (int h = 0; h < 2; h++)
 #pragma unroll
-            for (int e = 0; e < E; e++) ss += (double)x[h][e] * (double)x[h][e];
+            for (int e = 0; e < 4; e++) ss += (T)x[h][e] * (T)x[h][e];
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        const double inv = 1.0 / sqrt(ss / D + 1e-6);
+        for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const T inv = (T)1 / sqrt(ss / (T)D + (T)1e-6);
+        const uint2 g0 = __ldg(reinterpret_cast<const uint2 *>(gamma) + l);
+        const uint2 g1 = __ldg(reinterpret_cast<const uint2 *>(gamma + D / 2) + l);
+        const __half2 ga[4] = {*reinterpret_cast<const __half2 *>(&g0.x), *reinterpret_cast<const __half2 *>(&g0.y),
+                               *reinterpret_cast<const __half2 *>(&g1.x), *reinterpret_cast<const __half2 *>(&g1.y)};
+        const float cs[4] = {ang.c.x, ang.c.y, ang.c.z, ang.c.w}, sn[4] = {ang.s.x, ang.s.y, ang.s.z, ang.s.w};
 #pragma unroll
-        for (int e = 0; e < E; e++) {
-            const int i = E * lane + e;
-            const double a = (double)x[0][e] * inv * (double)__half2float(gamma[i]);
-            const double b = (double)x[1][e] * inv * (double)__half2float(gamma[i + D / 2]);
-            const double c = cs[i], s = sn[i];
+        for (int e = 0; e < 4; e++) {
+            const float f0 = (e & 1) ? __high2float(ga[e >> 1]) : __low2float(ga[e >> 1]);
+            const float f1 = (e & 1) ? __high2float(ga[2 + (e >> 1)]) : __low2float(ga[2 + (e >> 1)]);
+            const T a = (T)x[0][e] * inv * (T)f0, b = (T)x[1][e] * inv * (T)f1;
+            const T c = cs[e], s = sn[e];
             x[0][e] = (float)(a * c - b * s);
             x[1][e] = (float)(b * c + a * s);
         }
     }
 
-    // Quantises and writes the row as position r of the unit.
+    // Quantises and writes the row as position r of the unit (`on`: this lane's
+    // head is there; all lanes take part in the exchange).
     template <bool V>
-    __device__ __forceinline__ void store4(uint8_t *unit, int r, int lane) const {
+    __device__ __forceinline__ void store4(uint8_t *unit, int r, int l, bool on) const {
         using U = Kv4Unit<D>;
-        constexpr int kGroupLanes = 32 / E;  // lanes of one scale group
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            float amax = 0.0f;
-            bool fin = true;
+            unsigned top = 0;  // largest magnitude's bits; infinities and NaN lie above all
 #pragma unroll
-            for (int e = 0; e < E; e++) {
-                amax = fmaxf(amax, fabsf(x[h][e]));
-                fin = fin && isfinite(x[h][e]);
-            }
-            if (!fin) amax = INFINITY;
+            for (int e = 0; e < 4; e++) top = max(top, __float_as_uint(x[h][e]) & 0x7fffffffu);
 #pragma unroll
-            for (int o = kGroupLanes / 2; o > 0; o >>= 1)
-                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-            // f32 division by 7 then f16 rounding equals rounding amax / 7 once:
-            // no f32 neighbour of 7m has a quotient that rounds to the 12-bit m
-            __half sh = __float2half_rn(fminf(__fdiv_rn(amax, 7.0f), 65504.0f));
-            if (!isfinite(amax)) sh = __ushort_as_half((unsigned short)0x7e00);
+            for (int o = 1; o < 8; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const bool fin = top < 0x7f800000u;
+            // amax / 7 correctly rounded: one step from a quotient within an ulp.
+            // Rounding that to f16 equals rounding amax / 7 once: no f32 neighbour
+            // of 7m has a quotient that rounds to the 12-bit m.
+            const float amax = __uint_as_float(top), seventh = 0.14285715f;
+            float d = __fmul_rn(amax, seventh);
+            d = fmaf(fmaf(-7.0f, d, amax), seventh, d);
+            const __half sh = fin ? __float2half_rn(fminf(d, 65504.0f)) : __ushort_as_half((unsigned short)0x7e00);
             const float s = __half2float(sh);
-            const bool live = s > 0.0f && isfinite(amax);
-            const float inv = live ? __fdiv_rn(1.0f, s) : 0.0f;
+            const bool live = fin && s > 0.0f;
+            float inv;
+            asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(live ? s : 1.0f));
             unsigned nib = 0;
 #pragma unroll
-            for (int e = 0; e < E; e++) {
+            for (int e = 0; e < 4; e++) {
                 // nearest integer to x / s: rint of the approximate quotient is off
                 // by one at most; x - q s is exact in f32 and decides
-                float q = 0.0f;
-                if (live) {
-                    const float v = x[h][e];
-                    q = rintf(fminf(fmaxf(v * inv, -8.0f), 8.0f));
-                    const float rest = 2.0f * fmaf(-q, s, v);
-                    if (rest > s || (rest == s && ((int)q & 1))) q += 1.0f;
-                    else if (rest < -s || (rest == -s && ((int)q & 1))) q -= 1.0f;
-                    q = fminf(fmaxf(q, -7.0f), 7.0f);
-                }
+                const float v = live ? x[h][e] : 0.0f;
+                float q = rintf(fminf(fmaxf(v * inv, -8.0f), 8.0f));
+                const float rest = 2.0f * fmaf(-q, s, v);
+                const bool odd = (int)q & 1;
+                if (rest > s || (rest == s && odd)) q += 1.0f;
+                if (rest < -s || (rest == -s && odd)) q -= 1.0f;
+                q = live ? fminf(fmaxf(q, -7.0f), 7.0f) : 0.0f;
                 nib |= (unsigned)((int)q + 8) << (4 * e);
             }
-            const int dim = h * (D / 2) + E * lane;
-            constexpr int kLanes = (V ? 4 : 8) / E;  // lanes of one stored word / halfword
-            nib <<= 4 * E * (lane & (kLanes - 1));
-#pragma unroll
-            for (int o = kLanes / 2; o > 0; o >>= 1) nib |= __shfl_xor_sync(0xffffffffu, nib, o);
-            if ((lane & (kLanes - 1)) == 0) {
-                if (V) *reinterpret_cast<uint16_t *>(unit + U::v_half(r, dim)) = (uint16_t)nib;
-                else *reinterpret_cast<uint32_t *>(unit + U::k_word(r, dim)) = nib;
-            }
-            if ((lane & (kGroupLanes - 1)) == 0)
+            if (!on) continue;
+            const int dim = h * (D / 2) + 4 * l;
+            *reinterpret_cast<uint16_t *>(unit + (V ? U::v_half(r, dim) : U::k_word(r, dim) + ((dim & 4) >> 1))) =
+                (uint16_t)nib;
+            if ((l & 7) == 0)
                 *reinterpret_cast<__half *>(unit + (V ? U::v_scale(r, dim >> 5) : U::k_scale(r, dim >> 5))) = sh;
         }
     }
 
     template <bool V>
-    __device__ __forceinline__ void load4(const uint8_t *unit, int r, int lane) {
+    __device__ __forceinline__ void load4(const uint8_t *unit, int r, int l) {
         using U = Kv4Unit<D>;
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            const int dim = h * (D / 2) + E * lane;
+            const int dim = h * (D / 2) + 4 * l;
             const float s = __half2float(
                 *reinterpret_cast<const __half *>(unit + (V ? U::v_scale(r, dim >> 5) : U::k_scale(r, dim >> 5))));
-            const unsigned w = V ? (unsigned)*reinterpret_cast<const uint16_t *>(unit + U::v_half(r, dim))
-                                 : *reinterpret_cast<const uint32_t *>(unit + U::k_word(r, dim));
+            const unsigned w = *reinterpret_cast<const uint16_t *>(
+                unit + (V ? U::v_half(r, dim) : U::k_word(r, dim) + ((dim & 4) >> 1)));
 #pragma unroll
-            for (int e = 0; e < E; e++)
-                x[h][e] = s * (float)((int)((w >> (4 * ((dim + e) & (V ? 3 : 7)))) & 15u) - 8);
+            for (int e = 0; e < 4; e++) x[h][e] = s * (float)((int)((w >> (4 * e)) & 15u) - 8);
         }
     }
 };
@@ -330,17 +376,27 @@ __device__ __forceinline__ bool row_place(const RowArgs &a, int i, int &page, in
     return true;
 }
 
-// One warp per (row, head): q heads are normed, rotated and stored in f32; k
-// heads normed, rotated and stored in 4 bits; v heads stored in 4 bits.
+// Norm, rotation and append.  A warp takes 256 / D heads of one kind of one
+// row: q heads are normed, rotated and stored in f32; k heads normed, rotated
+// and stored in 4 bits; v heads stored in 4 bits.
 template <int D>
 __global__ void __launch_bounds__(kRowWarps * 32) k_kv4_append(const RowArgs a) {
+    constexpr int HW = 256 / D;  // heads of a warp
     griddep_launch_dependents();
     griddep_wait();
-    const int lane = threadIdx.x & 31;
-    const int per = a.heads + 2 * a.L.kvh;
+    const int lane = threadIdx.x & 31, l = lane % (D / 8), sub = lane / (D / 8);
+    const int qt = (a.heads + HW - 1) / HW, kt = (a.L.kvh + HW - 1) / HW, per = qt + 2 * kt;
     const int64_t task = (int64_t)blockIdx.x * kRowWarps + (threadIdx.x >> 5);
-    const int i = (int)(task / per), h = (int)(task % per);
+    const int i = (int)(task / per);
+    int w = (int)(task - (int64_t)i * per);
     if (i >= a.rows) return;
+    const int kind = w < qt ? 0 : w < qt + kt ? 1 : 2;
+    const int n = kind == 0 ? a.heads : a.L.kvh;
+    const int h = (w - (kind == 0 ? 0 : kind == 1 ? qt : qt + kt)) * HW + sub;  // this lane's head of its kind
+    const bool on = h < n;
+    const int first = kind == 0 ? 0 : kind == 1 ? a.heads : a.heads + a.L.kvh;
+    HeadVec<D> x;
+    x.load(a.qkv + ((int64_t)i * (a.heads + 2 * a.L.kvh) + first + (on ? h : 0)) * D, l);
     int page, unit, r;
     if (!row_place(a, i, page, unit, r)) return;
     const int pos = a.positions[i];
@@ -348,44 +404,50 @@ __global__ void __launch_bounds__(kRowWarps * 32) k_kv4_append(const RowArgs a) 
         raise_error(a.err, kDevRange);
         return;
     }
-    HeadVec<D> x;
-    x.load(a.qkv + ((int64_t)i * per + h) * D, lane);
-    const float *cs = a.cos + (int64_t)pos * (D / 2), *sn = a.sin + (int64_t)pos * (D / 2);
-    if (h < a.heads) {
-        x.norm_rope(a.q_gamma, cs, sn, lane);
-        x.store(a.q_out + ((int64_t)i * a.heads + h) * D, lane);
-    } else if (h < a.heads + a.L.kvh) {
-        x.norm_rope(a.k_gamma, cs, sn, lane);
-        x.template store4<false>(a.L.unit(page, h - a.heads, unit, D), r, lane);
+    if (kind == 2) {
+        x.template store4<true>(a.L.unit(page, on ? h : 0, unit, D), r, l, on);
+        return;
+    }
+    Angles<D> ang;
+    ang.load(a.cos + (int64_t)pos * (D / 2), a.sin + (int64_t)pos * (D / 2), l);
+    if (kind == 0) {
+        x.template norm_rope<float>(a.q_gamma, ang, l);
+        if (on) x.store(a.q_out + ((int64_t)i * a.heads + h) * D, l);
     } else {
-        x.template store4<true>(a.L.unit(page, h - a.heads - a.L.kvh, unit, D), r, lane);
+        x.template norm_rope<double>(a.k_gamma, ang, l);
+        x.template store4<false>(a.L.unit(page, on ? h : 0, unit, D), r, l, on);
     }
 }
 
-// Rows of keys and values as they are (READ: back to f32).
+// Rows of keys and values as they are (READ: back to f32), 256 / D heads a warp.
 template <int D, bool READ>
 __global__ void __launch_bounds__(kRowWarps * 32) k_kv4_rows(const RowArgs a) {
+    constexpr int HW = 256 / D;
     griddep_launch_dependents();
     griddep_wait();
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31, l = lane % (D / 8), sub = lane / (D / 8);
+    const int per = (a.L.kvh + HW - 1) / HW;
     const int64_t task = (int64_t)blockIdx.x * kRowWarps + (threadIdx.x >> 5);
-    const int i = (int)(task / a.L.kvh), h = (int)(task % a.L.kvh);
+    const int i = (int)(task / per), h = (int)(task - (int64_t)i * per) * HW + sub;
     if (i >= a.rows) return;
     int page, unit, r;
     if (!row_place(a, i, page, unit, r)) return;
-    uint8_t *u = a.L.unit(page, h, unit, D);
-    const int64_t at = ((int64_t)i * a.L.kvh + h) * D;
-    HeadVec<D> x;
+    const bool on = h < a.L.kvh;
+    uint8_t *u = a.L.unit(page, on ? h : 0, unit, D);
+    const int64_t at = ((int64_t)i * a.L.kvh + (on ? h : 0)) * D;
+    HeadVec<D> k, v;
     if (READ) {
-        x.template load4<false>(u, r, lane);
-        x.store(a.k_out + at, lane);
-        x.template load4<true>(u, r, lane);
-        x.store(a.v_out + at, lane);
+        k.template load4<false>(u, r, l);
+        v.template load4<true>(u, r, l);
+        if (on) {
+            k.store(a.k_out + at, l);
+            v.store(a.v_out + at, l);
+        }
     } else {
-        x.load(a.k_in + at, lane);
-        x.template store4<false>(u, r, lane);
-        x.load(a.v_in + at, lane);
-        x.template store4<true>(u, r, lane);
+        k.load(a.k_in + at, l);
+        v.load(a.v_in + at, l);
+        k.template store4<false>(u, r, l, on);
+        v.template store4<true>(u, r, l, on);
     }
 }
 
@@ -394,6 +456,11 @@ int row_blocks(const char *who, int64_t warps, dim3 &grid) {
     if (blocks > 0x7fffffff) return set_error(QORA_ERR_UNSUPPORTED, "%s: too many rows", who);
     grid = dim3((unsigned)blocks);
     return QORA_OK;
+}
+
+template <class... T>
+bool aligned16(const T *...p) {
+    return !((reinterpret_cast<uintptr_t>(p) | ...) & 15);
 }
 
 int rows_args(const char *who, qora_kv4 *kv, int32_t layer, const int32_t *slots, int32_t rows, RowArgs &a) {
@@ -528,10 +595,14 @@ int qora_kv4_reserve(qora_kv4 *kv, const int32_t *counts, int32_t max_tokens, in
     a.pages_per_stream = kv->pages_per_stream;
     a.pool_pages = kv->pool_pages;
     a.max_tokens = max_tokens;
-    const size_t smem = (size_t)((kv->pool_pages + 31) / 32) * 4;
+    const size_t smem = ((size_t)((kv->pool_pages + 31) / 32) + 3 * (size_t)kv->streams) * 4;
     if (smem > 40 * 1024)
-        QORA_CUDA(cudaFuncSetAttribute(k_kv4_reserve, cudaFuncAttributeMaxDynamicSharedMemorySize, 1 << 17));
-    return launch_ex(k_kv4_reserve, dim3(1), dim3(kResThreads), smem, as_stream(stream), 1u, a);
+        QORA_CUDA(cudaFuncSetAttribute(k_kv4_reserve, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    // a cluster pays when there are more table entries and tokens than one block
+    // takes in a few rounds
+    const bool wide = (int64_t)kv->streams * kv->pages_per_stream + max_tokens > 16384;
+    const unsigned nr = wide ? kResCluster : 1;
+    return launch_ex(k_kv4_reserve, dim3(1, nr), dim3(kResThreads), smem, as_stream(stream), nr, a);
 }
 
 int qora_kv4_advance(qora_kv4 *kv, const int32_t *counts, void *stream) {
@@ -550,6 +621,8 @@ int qora_kv4_append(qora_kv4 *kv, int32_t layer, const float *qkv, const uint16_
     if (!tokens) return QORA_OK;
     if (!qkv || !q_norm || !k_norm || !rope_cos || !rope_sin || !positions || !q_out || rope_max_pos <= 0)
         return set_error(QORA_ERR_INVALID, "qora_kv4_append: bad arguments");
+    if (!aligned16(qkv, rope_cos, rope_sin, q_out) || !aligned16(q_norm, k_norm))
+        return set_error(QORA_ERR_INVALID, "qora_kv4_append: pointers must be 16-byte aligned");
     DeviceGuard dg;
     QORA_TRY(dg.set(kv->ctx->device));
     a.qkv = qkv;
@@ -560,8 +633,10 @@ int qora_kv4_append(qora_kv4 *kv, int32_t layer, const float *qkv, const uint16_
     a.sin = rope_sin;
     a.rope_max = rope_max_pos;
     a.positions = positions;
+    const int hw = 256 / kv->hd;
+    const int64_t per = (kv->heads + hw - 1) / hw + 2 * ((kv->kvh + hw - 1) / hw);
     dim3 grid;
-    QORA_TRY(row_blocks("qora_kv4_append", (int64_t)tokens * (kv->heads + 2 * kv->kvh), grid));
+    QORA_TRY(row_blocks("qora_kv4_append", tokens * per, grid));
     auto kern = kv->hd == 64 ? k_kv4_append<64> : k_kv4_append<128>;
     return launch_ex(kern, grid, dim3(kRowWarps * 32), 0, as_stream(stream), 1u, a);
 }
@@ -572,12 +647,14 @@ int qora_kv4_write(qora_kv4 *kv, int32_t layer, const int32_t *slots, int32_t ro
     QORA_TRY(rows_args("qora_kv4_write", kv, layer, slots, rows, a));
     if (!rows) return QORA_OK;
     if (!k || !v) return set_error(QORA_ERR_INVALID, "qora_kv4_write: null argument");
+    if (!aligned16(k, v)) return set_error(QORA_ERR_INVALID, "qora_kv4_write: pointers must be 16-byte aligned");
     DeviceGuard dg;
     QORA_TRY(dg.set(kv->ctx->device));
     a.k_in = k;
     a.v_in = v;
     dim3 grid;
-    QORA_TRY(row_blocks("qora_kv4_write", (int64_t)rows * kv->kvh, grid));
+    const int hw = 256 / kv->hd;
+    QORA_TRY(row_blocks("qora_kv4_write", (int64_t)rows * ((kv->kvh + hw - 1) / hw), grid));
     auto kern = kv->hd == 64 ? k_kv4_rows<64, false> : k_kv4_rows<128, false>;
     return launch_ex(kern, grid, dim3(kRowWarps * 32), 0, as_stream(stream), 1u, a);
 }
@@ -588,12 +665,14 @@ int qora_kv4_read(qora_kv4 *kv, int32_t layer, const int32_t *slots, int32_t row
     QORA_TRY(rows_args("qora_kv4_read", kv, layer, slots, rows, a));
     if (!rows) return QORA_OK;
     if (!k || !v) return set_error(QORA_ERR_INVALID, "qora_kv4_read: null argument");
+    if (!aligned16(k, v)) return set_error(QORA_ERR_INVALID, "qora_kv4_read: pointers must be 16-byte aligned");
     DeviceGuard dg;
     QORA_TRY(dg.set(kv->ctx->device));
     a.k_out = k;
     a.v_out = v;
     dim3 grid;
-    QORA_TRY(row_blocks("qora_kv4_read", (int64_t)rows * kv->kvh, grid));
+    const int hw = 256 / kv->hd;
+    QORA_TRY(row_blocks("qora_kv4_read", (int64_t)rows * ((kv->kvh + hw - 1) / hw), grid));
     auto kern = kv->hd == 64 ? k_kv4_rows<64, true> : k_kv4_rows<128, true>;
     return launch_ex(kern, grid, dim3(kRowWarps * 32), 0, as_stream(stream), 1u, a);
 }

@@ -525,6 +525,8 @@ extern "C" int qora_kv4_attend(qora_kv4 *kv, int32_t layer, const float *q, cons
     if (layer < 0 || layer >= kv->layers)
         return set_error(QORA_ERR_INVALID, "qora_kv4_attend: layer %d out of range", layer);
     if (!tokens) return QORA_OK;
+    if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15)
+        return set_error(QORA_ERR_INVALID, "qora_kv4_attend: pointers must be 16-byte aligned");
     DeviceGuard dg;
     QORA_TRY(dg.set(kv->ctx->device));
     AttendArgs a;

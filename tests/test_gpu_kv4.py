@@ -182,8 +182,18 @@ def test_append_matches_definition(ctx, orc, heads, kvh, hd, page, n):
     k, v = kv.read(layer, args[-1])
     assert _error(ctx) == 0
     rq, rk, rv = R.append(qkv, heads, kvh, hd, qn, kn, cos, sin, pos)
-    # one rounding to f32 of a value computed in f64
-    assert np.all(np.abs(q.cpu().numpy() - rq) <= np.abs(rq) * 2.0 ** -24 * 1.001 + 1e-12)
+    # q in f32.  With u = 2^-24: the sum of squares is off by 8 u (8 products and sums
+    # in a lane, 4 exchanges, all terms positive, less than 12 roundings of which the
+    # square root halves the effect: 6 u), the mean, eps, root and quotient by 4 u more
+    # (half of the first two), x inv gamma by 2 u, and the rotation a c - b s by 2 u of
+    # |a c| + |b s|: 14 u of that sum covers it.  (When q was computed in f64 this
+    # was one rounding; the reference's own rows are f32 arithmetic.)
+    a = np.stack([[R.norm_rope(qkv[i, h * hd:(h + 1) * hd], qn, np.ones(hd // 2), np.zeros(hd // 2))
+                   for h in range(heads)] for i in range(n)])
+    c, s = np.abs(cos[pos])[:, None], np.abs(sin[pos])[:, None]
+    one, two = np.abs(a[..., :hd // 2]), np.abs(a[..., hd // 2:])
+    size = np.concatenate([one * c + two * s, two * c + one * s], -1).reshape(n, -1)
+    assert np.all(np.abs(q.cpu().numpy() - rq) <= 14 * 2.0 ** -24 * size + 1e-12)
     assert np.array_equal(k.cpu().numpy(), rk) and np.array_equal(v.cpu().numpy(), rv)
     # the other layers and the other slots were left as they were (zeros)
     rest = _i32(np.setdiff1d(np.arange(pool * page), slots))
@@ -356,6 +366,24 @@ def test_attend_sees_nothing_behind_the_last_position(ctx):
     q[0, 1, 3] = np.inf
     out = kv.attend(1, _dev(q.reshape(6, -1)), offsets, 3).view(6, heads, hd)
     assert bool(torch.isnan(out[0, 1]).all()) and bool(torch.isfinite(out[0, 0]).all())
+    assert _error(ctx) == 0
+
+
+def test_unaligned_pointers_are_refused(ctx, orc):
+    import torch
+    from qora_b200 import _lib
+    heads, kvh, hd = 4, 2, 64
+    qn, kn, cos, sin = (_dev(t) for t in _weights(orc, hd, 1))
+    kv = _cache(ctx, 1, heads, kvh, hd, 64, 1, 32, 2)
+    wide = torch.zeros(1 + 2 * (heads + 2 * kvh) * hd, device="cuda")[1:].view(2, -1)
+    narrow = torch.zeros(1 + 2 * kvh * hd, device="cuda")[1:].view(2, -1)
+    i = _i32([0, 1])
+    for call in (lambda: kv.append(0, wide, qn, kn, cos, sin, i, i), lambda: kv.write(0, i, narrow, narrow),
+                 lambda: kv.read(0, i, out=(narrow, narrow)),
+                 lambda: kv.attend(0, wide.view(-1)[:2 * heads * hd].view(2, -1), i, 1)):
+        with pytest.raises(_lib.QoraError) as e:
+            call()
+        assert e.value.status == INVALID
     assert _error(ctx) == 0
 
 
