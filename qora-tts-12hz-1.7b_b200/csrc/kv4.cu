@@ -516,7 +516,6 @@ int qora_kv4_create(qora_ctx *ctx, int32_t num_layers, int32_t num_heads, int32_
     while ((1 << kv->page_shift) < page_positions) kv->page_shift++;
     kv->pages_per_stream = (int)(((int64_t)max_pos + page_positions - 1) / page_positions);
     kv->pool_pages = pool_pages;
-    kv->attend_blocks = kv4_attend_blocks(ctx);
     const int64_t page_bytes =
         (int64_t)num_layers * kv_heads * (page_positions / kKv4Unit) * kv4_unit_bytes(head_dim);
     int rc = kv->pages.alloc((size_t)(page_bytes * pool_pages));
@@ -524,9 +523,7 @@ int qora_kv4_create(qora_ctx *ctx, int32_t num_layers, int32_t num_heads, int32_
     if (rc == QORA_OK) rc = kv->table.alloc((size_t)streams * kv->pages_per_stream * 4);
     if (rc == QORA_OK) rc = kv->len.alloc((size_t)streams * 4);
     if (rc == QORA_OK) rc = kv->len.zero();
-    if (rc == QORA_OK) rc = kv->part.alloc((size_t)kv->attend_blocks * 2 * kKv4PartRows * (head_dim + 2) * 4);
-    if (rc == QORA_OK) rc = kv->tickets.alloc((size_t)kv->attend_blocks * 4);
-    if (rc == QORA_OK) rc = kv->tickets.zero();
+    if (rc == QORA_OK) rc = kv4_attend_setup(kv);
     if (rc == QORA_OK && cudaMemsetAsync(kv->table.p, 0xff, kv->table.bytes, nullptr) != cudaSuccess)
         rc = set_error(QORA_ERR_CUDA, "qora_kv4_create: memset failed");
     if (rc == QORA_OK && cudaDeviceSynchronize() != cudaSuccess)

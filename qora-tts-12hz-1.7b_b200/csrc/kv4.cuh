@@ -9,14 +9,16 @@
 // Storage is by units of 32 positions of one (layer, kv head): 36 * head_dim
 // contiguous bytes, one bulk copy for the attention kernel:
 //     [K codes 16 D | V codes 16 D | K scales 2 D | V scales 2 D]     (D = head_dim)
-// Codes are laid out as the fragments of the attention's matrix instructions:
-//   K: row r (position in the unit) has D/2 bytes = words [t 0..3][c < D/32];
-//      nibble j of word (t, c) is dimension 32c + 8t + j.
-//   V: 16-position tile r/16, plane (r/8)%2, lane (g 0..7, t = (r%8)/2), word
-//      c < D/32, halfword r%2; nibble j of the halfword is dimension
-//      32c + 4g + j (a word holds two neighbouring positions, so one mask
-//      gives the pair that a matrix fragment register needs).
-//   scales: [r][c] f16.
+// Codes are laid out as the fragments of the attention's matrix instructions, by
+// scale group c < D/32, so that a lane (g 0..7, t 0..3) of a warp takes its words
+// of a group in one 16-byte load and the scales of its positions in one of 8:
+//   K: [c][g][t][i 0..3] words; nibble j of a word is dimension 32c + 8t + j of
+//      position g + 8i;
+//   V: [c][g][t][h 0..3] words of two halfwords e; nibble j of a halfword is
+//      dimension 32c + 4g + j of position 8h + 2t + e (a word holds two
+//      neighbouring positions, so one mask gives the pair that a matrix fragment
+//      register needs);
+//   scales: [c][g][i] f16 of position g + 8i.
 // A page holds page_pos positions of every layer and kv head, in the order
 // [layer][kv head][unit].  Logical page j of stream b is physical page
 // table[b][j]; a slot is page * page_pos + position in the page.
@@ -29,15 +31,13 @@ struct qora_kv4 {
     int layers = 0, heads = 0, kvh = 0, hd = 0, max_pos = 0, streams = 0;
     int page_pos = 0, page_shift = 0, pages_per_stream = 0, pool_pages = 0;
     qora::DevBuf pages, table, len;
-    qora::DevBuf part, tickets;  // attend: split partials, one arrival count per block
-    int attend_blocks = 0;
+    int clusters[2][3] = {};  // attend: clusters that run at once, by kernel and cluster size
 };
 
 namespace qora {
 
 constexpr int kKv4Unit = 32;           // positions per unit
 constexpr int kKv4MaxStreams = 4096;   // the attention's work list lies in shared memory
-constexpr int kKv4PartRows = 16;       // query rows of the widest attention tile
 
 __host__ __device__ constexpr int kv4_unit_bytes(int hd) { return 36 * hd; }
 
@@ -67,24 +67,22 @@ inline Kv4Layer kv4_layer(const qora_kv4 *kv, int layer) {
     return L;
 }
 
+// Asks the device what the attention kernels' launches go by (at creation).
+int kv4_attend_setup(qora_kv4 *kv);
+
 // Byte offsets in a unit of head dimension D.
 template <int D>
 struct Kv4Unit {
     static constexpr int kBytes = kv4_unit_bytes(D);
     static constexpr int kK = 0, kV = 16 * D, kKs = 32 * D, kVs = 34 * D;
-    static constexpr int C = D / 32;  // scale groups
     __host__ __device__ static __forceinline__ int k_word(int r, int dim) {
-        return kK + r * (D / 2) + ((dim & 31) >> 3) * (D / 8) + (dim >> 5) * 4;
+        return kK + (((dim >> 5) * 8 + (r & 7)) * 4 + ((dim & 31) >> 3)) * 16 + (r >> 3) * 4;
     }
     __host__ __device__ static __forceinline__ int v_half(int r, int dim) {
-        return kV + (r >> 4) * (8 * D) + ((r >> 3) & 1) * (4 * D) +
-               (((dim & 31) >> 2) * 4 + ((r & 7) >> 1)) * (D / 8) + (dim >> 5) * 4 + (r & 1) * 2;
+        return kV + (((dim >> 5) * 8 + ((dim & 31) >> 2)) * 4 + ((r & 7) >> 1)) * 16 + (r >> 3) * 4 + (r & 1) * 2;
     }
-    __host__ __device__ static __forceinline__ int k_scale(int r, int c) { return kKs + (r * C + c) * 2; }
-    __host__ __device__ static __forceinline__ int v_scale(int r, int c) { return kVs + (r * C + c) * 2; }
+    __host__ __device__ static __forceinline__ int k_scale(int r, int c) { return kKs + ((c * 8 + (r & 7)) * 4 + (r >> 3)) * 2; }
+    __host__ __device__ static __forceinline__ int v_scale(int r, int c) { return kVs + ((c * 8 + (r & 7)) * 4 + (r >> 3)) * 2; }
 };
-
-// Most blocks of one attention launch (its workspace is sized for them).
-int kv4_attend_blocks(const qora_ctx *ctx);
 
 }  // namespace qora

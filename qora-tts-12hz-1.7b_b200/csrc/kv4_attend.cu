@@ -19,12 +19,18 @@
 // (the matrix unit's own additions do not round to nearest).  The running
 // maximum and sum are f32, in base 2.
 //
-// The work of a launch (all streams, kv heads, row tiles, units) is one line
-// of units that the blocks split evenly, whatever the lengths; lengths and
-// offsets are read on the device.  Where a block's share ends inside an item,
-// partial (max, sum, weighted sum) go to a workspace and the item's last block
-// joins them in block order, so the result does not depend on timing.
+// The work of a launch (all streams, kv heads, row tiles, units) is one line of
+// units; lengths and offsets are read on the device.  Each cluster of blocks
+// takes a run of whole items (stream, kv head, row tile) with as near to an even
+// share of the units as whole items allow, and its blocks split the run evenly,
+// through the middle of items.  Partial (max, sum, weighted sum) of an item that
+// several blocks share meet in distributed shared memory, in block order, so
+// there is no workspace and the result does not depend on timing.
+#include <cooperative_groups.h>
+
 #include "kv4.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace qora {
 
@@ -32,27 +38,36 @@ namespace {
 
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
+constexpr int kMaxCluster = 8;  // blocks of a cluster
 
 struct AttendArgs {
     Kv4Layer L;
     const float *q;
     const int *offsets, *len;
-    float *out, *part;
-    unsigned *tickets;
+    float *out;
     int *err;
     int streams, heads, max_pos, tokens;
     float scale_log2;  // log2(e) / sqrt(D)
 };
 
+// D = A B + C for 16 x 16 x 8, f16 in and f32 out; (not volatile: the compiler may
+// interleave the products of different scale groups)
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// the same with C = 0
+__device__ __forceinline__ void mma16816_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                               uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
     uint32_t r;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
 }
 __device__ __forceinline__ float ex2(float x) {
@@ -63,16 +78,25 @@ __device__ __forceinline__ float ex2(float x) {
 __device__ __forceinline__ uint32_t h2u(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
 __device__ __forceinline__ __half2 u2h(uint32_t u) { return *reinterpret_cast<__half2 *>(&u); }
 
+// (w & Mask) | magic in one instruction.  (Left to the compiler it becomes two,
+// 128 more of them for every unit.)
+template <uint32_t Mask>
+__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t magic) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(w), "n"(Mask), "r"(magic));
+    return r;
+}
 // The four pairs of codes of a word: x[j] = (nibble j, nibble j + 4) - 8 in f16.
-__device__ __forceinline__ void codes(uint32_t w, uint32_t (&x)[4]) {
+// `magic` is 0x64006400 (1024 in both halves) in a register.
+__device__ __forceinline__ void codes(uint32_t w, uint32_t magic, uint32_t (&x)[4]) {
     const __half2 lo = __half2half2(__ushort_as_half(0x6408));    // 1032
     const __half2 s16 = __half2half2(__ushort_as_half(0x2c00));   // 1 / 16
     const __half2 hi = __half2half2(__ushort_as_half(0xd480));    // -72
     const uint32_t v = w >> 8;
-    x[0] = h2u(__hsub2(u2h((w & 0x000f000fu) | 0x64006400u), lo));
-    x[1] = h2u(__hfma2(u2h((w & 0x00f000f0u) | 0x64006400u), s16, hi));
-    x[2] = h2u(__hsub2(u2h((v & 0x000f000fu) | 0x64006400u), lo));
-    x[3] = h2u(__hfma2(u2h((v & 0x00f000f0u) | 0x64006400u), s16, hi));
+    x[0] = h2u(__hsub2(u2h(and_or<0x000f000fu>(w, magic)), lo));
+    x[1] = h2u(__hfma2(u2h(and_or<0x00f000f0u>(w, magic)), s16, hi));
+    x[2] = h2u(__hsub2(u2h(and_or<0x000f000fu>(v, magic)), lo));
+    x[3] = h2u(__hfma2(u2h(and_or<0x00f000f0u>(v, magic)), s16, hi));
 }
 
 // t as f16 hi (low half) + f16 lo (high half): the bits that f16 has, and the rest.
@@ -81,50 +105,11 @@ __device__ __forceinline__ uint32_t split_hi_lo(float t) {
     return h2u(__floats2half2_rn(hi, t - hi));
 }
 
-template <int C>
-struct Words {
-    uint32_t w[C];
-    __device__ __forceinline__ void load(const uint8_t *p) {
-        if constexpr (C == 4) {
-            const uint4 v = *reinterpret_cast<const uint4 *>(p);
-            w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-        } else {
-            const uint2 v = *reinterpret_cast<const uint2 *>(p);
-            w[0] = v.x, w[1] = v.y;
-        }
-    }
-};
-template <int C>
-struct Scales {
-    __half2 s[C / 2];
-    __device__ __forceinline__ void load(const uint8_t *p) {
-        if constexpr (C == 4) {
-            const uint2 v = *reinterpret_cast<const uint2 *>(p);
-            s[0] = u2h(v.x), s[1] = u2h(v.y);
-        } else {
-            s[0] = u2h(*reinterpret_cast<const uint32_t *>(p));
-        }
-    }
-    __device__ __forceinline__ float at(int c) const {
-        return (c & 1) ? __high2float(s[c >> 1]) : __low2float(s[c >> 1]);
-    }
-    __device__ __forceinline__ __half2 most() const {
-        if constexpr (C == 4) return __hmax2(s[0], s[1]);
-        return s[0];
-    }
-};
-
-template <int D, int NT, int ST>
-struct Smem {
-    static constexpr int R = 4 * NT;
-    alignas(128) uint8_t ring[kWarps][ST][kv4_unit_bytes(D)];
-    float wo[kWarps][R][D];
-    float wm[kWarps][R], wl[kWarps][R];
-    uint64_t full[kWarps][ST];
-    int64_t scan[kWarps];
-    int last;
-    int64_t start[1];  // [streams + 1] first unit of each stream in the work line
-};
+// The four f16 scales of 8 bytes: element i.
+__device__ __forceinline__ float scale_of(uint2 v, int i) {
+    const __half2 h = u2h(i < 2 ? v.x : v.y);
+    return (i & 1) ? __high2float(h) : __low2float(h);
+}
 
 // One stream's share of the work line.
 struct Stream {
@@ -133,9 +118,9 @@ struct Stream {
 template <int R>
 __device__ __forceinline__ Stream stream_of(const AttendArgs &a, int G, int b) {
     Stream s;
-    s.len = __ldcg(a.len + b);
-    s.off = __ldcg(a.offsets + b);
-    s.n = __ldcg(a.offsets + b + 1) - s.off;
+    s.len = a.len[b];
+    s.off = a.offsets[b];
+    s.n = a.offsets[b + 1] - s.off;
     if (s.len < 0 || s.n < 0 || s.off < 0 || s.len > a.max_pos || s.n > a.max_pos - s.len ||
         s.n > a.tokens - s.off) {
         raise_error(a.err, kDevRange);
@@ -145,6 +130,68 @@ __device__ __forceinline__ Stream stream_of(const AttendArgs &a, int G, int b) {
     s.ub = (s.len + s.n + kKv4Unit - 1) / kKv4Unit;
     return s;
 }
+
+// n / d, in 32 bits where both fit (the work line hardly ever needs more).
+__device__ __forceinline__ int64_t quotient(int64_t n, int64_t d) {
+    if (((n | d) >> 32) == 0) return (int64_t)((uint32_t)n / (uint32_t)d);
+    return n / d;
+}
+
+// W units split over `blocks` blocks: the first `more` blocks take each + 1
+// units, the others `each`.
+struct Split {
+    int64_t each, more;
+    __device__ __forceinline__ Split(int64_t W, int64_t blocks) {
+        each = quotient(W, blocks);
+        more = W - each * blocks;
+    }
+    __device__ __forceinline__ int64_t first(int64_t i) const { return i * each + min(i, more); }
+    __device__ __forceinline__ int block_of(int64_t w) const {
+        const int64_t big = more * (each + 1);
+        return (int)(w < big ? quotient(w, each + 1) : more + quotient(w - big, each));
+    }
+};
+
+// The item that a block begins and others end.
+struct Shared {
+    int there, h, qt, off, rows;
+    int last;  // rank of the block that ends it
+};
+
+// A block's part of one item (stream, kv head, row tile).
+template <int R>
+struct Piece {
+    Stream s;
+    int h, qt, u0, u1;  // units [u0, u1) of the item's s.ub
+    int rows, tok0, tok1;
+    int mine;           // units of this warp
+    __device__ __forceinline__ void locate(const AttendArgs &a, int G, int b, int64_t rel, int64_t left, int warp) {
+        s = stream_of<R>(a, G, b);
+        const int item = (int)quotient(rel, s.ub);
+        u0 = (int)(rel - (int64_t)item * s.ub);
+        h = item / s.nq, qt = item - h * s.nq;
+        u1 = (int)min((int64_t)s.ub, u0 + left);
+        rows = min(R, s.n * G - qt * R);
+        tok0 = qt * R / G, tok1 = (qt * R + rows - 1) / G;
+        const int stop = min(u1, (s.len + tok1) / kKv4Unit + 1);  // no row sees units from here on
+        mine = stop > u0 + warp ? (stop - u0 - warp + kWarps - 1) / kWarps : 0;
+    }
+};
+
+template <int D, int NT, int ST>
+struct Smem {
+    static constexpr int R = 4 * NT;
+    static constexpr int kRow = D + 8;  // a quarter-warp's 16-byte stores fall on distinct banks
+    alignas(128) uint8_t ring[kWarps][ST][kv4_unit_bytes(D)];
+    float wo[kWarps][R][kRow];
+    float wm[kWarps][R], wl[kWarps][R];
+    float po[2][R][D];       // partials: [0] of the item that a block before began, [1] of the one begun here
+    float pm[2][R], pl[2][R];
+    uint64_t full[kWarps][ST];
+    int64_t scan[kWarps];
+    Shared open;
+    int64_t start[1];  // [streams + 1] first unit of each stream in the work line
+};
 
 template <int D, int NT, int ST>
 __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) k_kv4_attend(const AttendArgs a) {
@@ -163,7 +210,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) k_kv4_attend(const 
     }
     griddep_launch_dependents();
     griddep_wait();
-    // ---- the work line: streams' unit counts, scanned
+    // ---- the work line: the streams' units, scanned
     {
         int64_t base = 0;
         for (int b0 = 0; b0 < a.streams; b0 += kThreads) {
@@ -182,71 +229,96 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) k_kv4_attend(const 
             __syncthreads();
             if (lane == 31) sm.scan[warp] = x;
             __syncthreads();
-            int64_t before = base, all = base;
+            int64_t before = base;
+#pragma unroll
             for (int i = 0; i < kWarps; i++) {
-                if (i < warp) before += sm.scan[i];
-                all += sm.scan[i];
+                const int64_t part = sm.scan[i];
+                if (i < warp) before += part;
+                base += part;
             }
             if (b < a.streams) sm.start[b] = before + x - w;
-            base = all;
         }
-        if (tid == 0) sm.start[a.streams] = base;
+        if (tid == 0) {
+            sm.start[a.streams] = base;
+            sm.open.there = 0;
+        }
     }
     __syncthreads();
-    const int64_t W = sm.start[a.streams];
-    const int64_t blocks = min((int64_t)gridDim.x, (W + kWarps - 1) / kWarps);
-    if ((int64_t)blockIdx.x >= blocks) return;
-    const int64_t w0 = W * blockIdx.x / blocks, w1 = W * (blockIdx.x + 1) / blocks;
+    // ---- the cluster's run of whole items: [c0, c1), and how many there are
+    cg::cluster_group cl = cg::this_cluster();
+    const int rank = (int)cl.block_rank();
     int b = 0;
-    for (int lo = 0, hi = a.streams - 1; lo < hi;) {  // last stream that starts at or before w0
-        const int mid = (lo + hi + 1) >> 1;
-        if (sm.start[mid] <= w0) lo = b = mid;
-        else hi = mid - 1;
+    int64_t c0, c1, c_items = 0;
+    {
+        const Split over(sm.start[a.streams], gridDim.x);
+        // the item border nearest to unit t; and the items of the line before it
+        auto border = [&](int64_t t, int &bt) {
+            bt = 0;
+            for (int lo = 0, hi = a.streams - 1; lo < hi;) {  // last stream that starts at or before t
+                const int mid = (lo + hi + 1) >> 1;
+                if (sm.start[mid] <= t) lo = bt = mid;
+                else hi = mid - 1;
+            }
+            const Stream s = stream_of<R>(a, G, bt);
+            if (!s.nq) return sm.start[bt];
+            return sm.start[bt] + min(quotient(t - sm.start[bt] + s.ub / 2, s.ub), (int64_t)a.L.kvh * s.nq) * s.ub;
+        };
+        int bt;
+        c0 = border(over.first(blockIdx.x), b);
+        c1 = border(over.first(blockIdx.x + 1), bt);
+        if (c1 > c0) {  // an upper bound of the run's items, exact within one stream
+            const Stream s = stream_of<R>(a, G, bt);
+            c_items = b == bt ? quotient(c1 - c0, s.ub) : kMaxCluster;
+        }
     }
+    // a block takes at least one unit per warp, or an item
+    const int64_t shares =
+        min((int64_t)cl.num_blocks(), max(c_items, (c1 - c0 + kWarps - 1) / kWarps));
+    const Split split(c1 - c0, max(shares, (int64_t)1));
+    int64_t w = c1, w1 = c1;
+    if (rank < shares) w = c0 + split.first(rank), w1 = c0 + split.first(rank + 1);
+    uint32_t magic;
+    asm volatile("mov.b32 %0, 0x64006400;" : "=r"(magic));
     int turn = 0;  // units that this warp's ring has taken
     bool dead = false;
-    for (int64_t w = w0; w < w1;) {
+    // The piece at w: its first units are on their way before the piece before it
+    // is joined.  (Only what the loop over units needs stays in registers.)
+    int h, u0, mine;
+    const uint8_t *src = nullptr;
+    auto fetch_units = [&](int k) {  // where units k .. k + 31 are (lane = offset)
+        if (k + lane >= mine) return;
+        const int u = u0 + warp + (k + lane) * kWarps;
+        int pg = __ldcg(a.L.table + (int64_t)b * a.L.pages_per_stream + ((u * kKv4Unit) >> a.L.page_shift));
+        if ((unsigned)pg >= (unsigned)a.L.pool_pages) {
+            raise_error(a.err, kDevRange);
+            pg = 0;
+        }
+        src = a.L.unit(pg, h, u & ((1 << (a.L.page_shift - 5)) - 1), D);
+    };
+    auto issue = [&](int k) {
+        const uint8_t *from = reinterpret_cast<const uint8_t *>(
+            __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), k & 31));
+        if (lane == 0) {
+            const int st = (turn + k) % ST;
+            mbar_arrive_expect_tx(&sm.full[warp][st], U::kBytes);
+            bulk_g2s(&sm.ring[warp][st][0], from, U::kBytes, &sm.full[warp][st]);
+        }
+    };
+    auto begin = [&]() {
         while (sm.start[b + 1] <= w) b++;
-        const Stream s = stream_of<R>(a, G, b);
-        const int64_t rel = w - sm.start[b];
-        const int item = (int)(rel / s.ub);
-        const int u0 = (int)(rel - (int64_t)item * s.ub);
-        const int h = item / s.nq, qt = item - h * s.nq;
-        const int u1 = (int)min((int64_t)s.ub, u0 + (w1 - w));
-        const int64_t item0 = w - u0;
-        const int rows = min(R, s.n * G - qt * R);
-        const int tok0 = qt * R / G, tok1 = (qt * R + rows - 1) / G;
-        const int first_limit = s.len + tok0;                       // every row sees these positions
-        const int stop = min(u1, (s.len + tok1) / kKv4Unit + 1);  // no row sees units from here on
-        const int mine = stop > u0 + warp ? (stop - u0 - warp + kWarps - 1) / kWarps : 0;
-        const int *table = a.L.table + (int64_t)b * a.L.pages_per_stream;
-
-        // ---- ring: unit k of this warp is u0 + warp + k kWarps
-        int pages = 0;
-        auto fetch_pages = [&](int k) {  // of units k .. k + 31 (lane = offset)
-            const int u = u0 + warp + (k + lane) * kWarps;
-            pages = 0;
-            if (k + lane < mine) {
-                pages = __ldcg(table + ((u * kKv4Unit) >> a.L.page_shift));
-                if ((unsigned)pages >= (unsigned)a.L.pool_pages) {
-                    raise_error(a.err, kDevRange);
-                    pages = 0;
-                }
-            }
-        };
-        auto issue = [&](int k) {
-            const int pg = __shfl_sync(0xffffffffu, pages, k & 31);
-            if (lane == 0) {
-                const int u = u0 + warp + k * kWarps;
-                const int st = (turn + k) % ST;
-                mbar_arrive_expect_tx(&sm.full[warp][st], U::kBytes);
-                bulk_g2s(&sm.ring[warp][st][0], a.L.unit(pg, h, u & ((1 << (a.L.page_shift - 5)) - 1), D), U::kBytes,
-                         &sm.full[warp][st]);
-            }
-        };
-        fetch_pages(0);
+        Piece<R> p;
+        p.locate(a, G, b, w - sm.start[b], w1 - w, warp);
+        h = p.h, u0 = p.u0, mine = p.mine;
+        fetch_units(0);
         if (!dead)
             for (int k = 0; k < ST && k < mine; k++) issue(k);
+    };
+    if (w < w1) begin();
+    while (w < w1) {
+        int first_limit;  // every row sees the positions up to here
+        Piece<R> p;
+        p.locate(a, G, b, w - sm.start[b], w1 - w, warp);
+        first_limit = p.s.len + p.tok0;
 
         // ---- query fragments: column n = 2 row + {hi, lo}
         uint32_t bq[NT][2 * C][2];
@@ -255,18 +327,21 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) k_kv4_attend(const 
         float acc[NT][C][4];
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-            const int row = qt * R + nt * 4 + (g >> 1);
-            const bool have = row < s.n * G;
-            const float *q = a.q + ((int64_t)(s.off + row / G) * a.heads + h * G + row % G) * D;
+            const int row = p.qt * R + nt * 4 + (g >> 1);
+            const bool have = row < p.s.n * G;
+            const float4 *q = reinterpret_cast<const float4 *>(
+                a.q + ((int64_t)(p.s.off + (have ? row / G : 0)) * a.heads + h * G + (have ? row % G : 0)) * D + 8 * t);
             float x[C][8];
             float amax = 0.0f;
 #pragma unroll
-            for (int c = 0; c < C; c++)
+            for (int c = 0; c < C; c++) {
+                const float4 v0 = have ? __ldg(q + 8 * c) : make_float4(0.f, 0.f, 0.f, 0.f);
+                const float4 v1 = have ? __ldg(q + 8 * c + 1) : make_float4(0.f, 0.f, 0.f, 0.f);
+                x[c][0] = v0.x, x[c][1] = v0.y, x[c][2] = v0.z, x[c][3] = v0.w;
+                x[c][4] = v1.x, x[c][5] = v1.y, x[c][6] = v1.z, x[c][7] = v1.w;
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    x[c][j] = have ? __ldg(q + 32 * c + 8 * t + j) : 0.0f;
-                    amax = fmaxf(amax, fabsf(x[c][j]));
-                }
+                for (int j = 0; j < 8; j++) amax = fmaxf(amax, fabsf(x[c][j]));
+            }
             amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
             amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
             // 2^e puts the row's largest value into [2^9, 2^10)
@@ -284,8 +359,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) k_kv4_attend(const 
                     bq[nt][2 * c + (j >> 1)][j & 1] = h2u(__floats2half2_rn(y0, y1));
                 }
             rs[nt] = __shfl_sync(0xffffffffu, down, t * 8) * a.scale_log2;
-            const int mr = qt * R + nt * 4 + t;  // this lane's row
-            limit[nt] = mr < s.n * G ? s.len + mr / G : -1;
+            const int mr = p.qt * R + nt * 4 + t;  // this lane's row
+            limit[nt] = mr < p.s.n * G ? p.s.len + mr / G : -1;
             m[nt] = -INFINITY;
             l[nt] = 0.0f;
 #pragma unroll
@@ -305,52 +380,42 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) k_kv4_attend(const 
             }
             const uint8_t *unit = &sm.ring[warp][st][0];
             float sc[NT][4];  // scores of positions g, g + 8, g + 16, g + 24
+            float sl[NT][4];  // from the queries' lo halves
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) sc[nt][i] = 0.0f;
+                for (int i = 0; i < 4; i++) sc[nt][i] = sl[nt][i] = 0.0f;
 #pragma unroll
-            for (int rt = 0; rt < 2; rt++) {
-                Words<C> k0, k1;
-                Scales<C> s0, s1;
-                k0.load(unit + U::kK + (rt * 16 + g) * (D / 2) + t * (D / 8));
-                k1.load(unit + U::kK + (rt * 16 + g + 8) * (D / 2) + t * (D / 8));
-                s0.load(unit + U::k_scale(rt * 16 + g, 0));
-                s1.load(unit + U::k_scale(rt * 16 + g + 8, 0));
+            for (int c = 0; c < C; c++) {
+                const uint4 kw = *reinterpret_cast<const uint4 *>(unit + U::kK + c * 512 + lane * 16);
+                const uint2 ks = *reinterpret_cast<const uint2 *>(unit + U::kKs + c * 64 + g * 8);
 #pragma unroll
-                for (int c = 0; c < C; c++) {
+                for (int rt = 0; rt < 2; rt++) {
                     uint32_t x0[4], x1[4];
-                    codes(k0.w[c], x0);
-                    codes(k1.w[c], x1);
-                    const float f0 = s0.at(c), f1 = s1.at(c);
+                    codes(rt ? kw.z : kw.x, magic, x0);
+                    codes(rt ? kw.w : kw.y, magic, x1);
+                    const float f0 = scale_of(ks, 2 * rt), f1 = scale_of(ks, 2 * rt + 1);
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++) {
-                        float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                        mma16816(d, x0[0], x1[0], x0[1], x1[1], bq[nt][2 * c][0], bq[nt][2 * c][1]);
+                        float d[4];
+                        mma16816_first(d, x0[0], x1[0], x0[1], x1[1], bq[nt][2 * c][0], bq[nt][2 * c][1]);
                         mma16816(d, x0[2], x1[2], x0[3], x1[3], bq[nt][2 * c + 1][0], bq[nt][2 * c + 1][1]);
-                        sc[nt][2 * rt] = fmaf(f0, d[0] + d[1], sc[nt][2 * rt]);
-                        sc[nt][2 * rt + 1] = fmaf(f1, d[2] + d[3], sc[nt][2 * rt + 1]);
+                        sc[nt][2 * rt] = fmaf(f0, d[0], sc[nt][2 * rt]);
+                        sl[nt][2 * rt] = fmaf(f0, d[1], sl[nt][2 * rt]);
+                        sc[nt][2 * rt + 1] = fmaf(f1, d[2], sc[nt][2 * rt + 1]);
+                        sl[nt][2 * rt + 1] = fmaf(f1, d[3], sl[nt][2 * rt + 1]);
                     }
                 }
             }
-            // values and their scales into registers: the stage is free after that
-            Words<C> v[2][2];
-            Scales<C> vs[4];
-#pragma unroll
-            for (int rt = 0; rt < 2; rt++)
-#pragma unroll
-                for (int p = 0; p < 2; p++) {
-                    v[rt][p].load(unit + U::kV + rt * (8 * D) + p * (4 * D) + lane * (D / 8));
-                    vs[rt * 2 + p].load(unit + U::v_scale(rt * 16 + p * 8 + g, 0));
-                }
-            __syncwarp();
-            if (k + ST < mine) {
-                if (((k + ST) & 31) == 0) fetch_pages(k + ST);
-                issue(k + ST);
-            }
             const bool edge = u * kKv4Unit + kKv4Unit - 1 > first_limit;
             // the largest value scale of the unit sets the power of two
-            __half2 big = __hmax2(__hmax2(vs[0].most(), vs[1].most()), __hmax2(vs[2].most(), vs[3].most()));
+            uint2 vs[C];
+            __half2 big = __half2half2(__ushort_as_half(0));
+#pragma unroll
+            for (int c = 0; c < C; c++) {
+                vs[c] = *reinterpret_cast<const uint2 *>(unit + U::kVs + c * 64 + g * 8);
+                big = __hmax2(big, __hmax2(u2h(vs[c].x), u2h(vs[c].y)));
+            }
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) big = __hmax2(big, u2h(__shfl_xor_sync(0xffffffffu, h2u(big), o)));
             const unsigned bits = h2u(__hmax2(big, __lowhigh2highlow(big))) & 0x7c00u;
@@ -362,8 +427,12 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) k_kv4_attend(const 
             for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    sc[nt][i] *= rs[nt];
-                    if (edge && u * kKv4Unit + g + 8 * i > limit[nt]) sc[nt][i] = -INFINITY;
+                    sc[nt][i] = (sc[nt][i] + sl[nt][i]) * rs[nt];
+                }
+                if (edge) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (u * kKv4Unit + g + 8 * i > limit[nt]) sc[nt][i] = -INFINITY;
                 }
                 float mx = fmaxf(fmaxf(sc[nt][0], sc[nt][1]), fmaxf(sc[nt][2], sc[nt][3]));
 #pragma unroll
@@ -384,30 +453,38 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) k_kv4_attend(const 
 #pragma unroll
             for (int c = 0; c < C; c++) {
                 uint32_t bp[NT][4];
+                if (edge) {  // whatever lies behind a row's last position counts as zero
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float f = vs[i].at(c);
+                    for (int i = 0; i < 4; i++)
 #pragma unroll
-                    for (int nt = 0; nt < NT; nt++) {
-                        float x = sc[nt][i] * f;
-                        if (edge && sc[nt][i] == 0.0f) x = 0.0f;  // whatever lies behind the last position
-                        bp[nt][i] = transpose8x8(split_hi_lo(x));
-                    }
+                        for (int nt = 0; nt < NT; nt++)
+                            bp[nt][i] = split_hi_lo(sc[nt][i] == 0.0f ? 0.0f : sc[nt][i] * scale_of(vs[c], i));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++) bp[nt][i] = split_hi_lo(sc[nt][i] * scale_of(vs[c], i));
                 }
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) bp[nt][i] = transpose8x8(bp[nt][i]);
+                const uint4 vw = *reinterpret_cast<const uint4 *>(unit + U::kV + c * 512 + lane * 16);
                 float d0[NT][4], d1[NT][4];
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) d0[nt][i] = d1[nt][i] = 0.0f;
 #pragma unroll
                 for (int rt = 0; rt < 2; rt++) {
                     uint32_t x0[4], x1[4];
-                    codes(v[rt][0].w[c], x0);
-                    codes(v[rt][1].w[c], x1);
+                    codes(rt ? vw.z : vw.x, magic, x0);
+                    codes(rt ? vw.w : vw.y, magic, x1);
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++) {
-                        mma16816(d0[nt], x0[0], x0[1], x1[0], x1[1], bp[nt][2 * rt], bp[nt][2 * rt + 1]);
-                        mma16816(d1[nt], x0[2], x0[3], x1[2], x1[3], bp[nt][2 * rt], bp[nt][2 * rt + 1]);
+                        if (rt == 0) {
+                            mma16816_first(d0[nt], x0[0], x0[1], x1[0], x1[1], bp[nt][0], bp[nt][1]);
+                            mma16816_first(d1[nt], x0[2], x0[3], x1[2], x1[3], bp[nt][0], bp[nt][1]);
+                        } else {
+                            mma16816(d0[nt], x0[0], x0[1], x1[0], x1[1], bp[nt][2], bp[nt][3]);
+                            mma16816(d1[nt], x0[2], x0[3], x1[2], x1[3], bp[nt][2], bp[nt][3]);
+                        }
                     }
                 }
 #pragma unroll
@@ -418,8 +495,19 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) k_kv4_attend(const 
                     acc[nt][c][3] = fmaf(acc[nt][c][3], keep[nt], d1[nt][2] + d1[nt][3]);
                 }
             }
+            __syncwarp();  // the stage is read
+            if (k + ST < mine) {
+                if (((k + ST) & 31) == 0) fetch_units(k + ST);
+                issue(k + ST);
+            }
         }
         turn += mine;
+        // the piece is joined below: what the loop did not need is found again
+        p.locate(a, G, b, w - sm.start[b], w1 - w, warp);
+        const int64_t item0 = w - p.u0;
+        w += p.u1 - p.u0;
+        const bool more = w < w1;
+        if (more) begin();
 
         // ---- join the warps
         const float unlift = __int_as_float((127 - ke) << 23);
@@ -431,88 +519,134 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) k_kv4_attend(const 
                 sm.wm[warp][nt * 4 + t] = m[nt];
                 sm.wl[warp][nt * 4 + t] = l[nt];
             }
+            if (nt * 4 + t < p.rows)
 #pragma unroll
-            for (int c = 0; c < C; c++)
-                *reinterpret_cast<float4 *>(&sm.wo[warp][nt * 4 + t][32 * c + 4 * g]) =
-                    make_float4(acc[nt][c][0] * unlift, acc[nt][c][1] * unlift, acc[nt][c][2] * unlift,
-                                acc[nt][c][3] * unlift);
+                for (int c = 0; c < C; c++)
+                    *reinterpret_cast<float4 *>(&sm.wo[warp][nt * 4 + t][32 * c + 4 * g]) =
+                        make_float4(acc[nt][c][0] * unlift, acc[nt][c][1] * unlift, acc[nt][c][2] * unlift,
+                                    acc[nt][c][3] * unlift);
         }
         __syncthreads();
-        const bool whole = u0 == 0 && u1 == s.ub;
-        float *part = a.part + ((int64_t)blockIdx.x * 2 + (u0 == 0)) * (R * (D + 2));
-        for (int i = tid; i < R * D; i += kThreads) {
+        const bool whole = p.u0 == 0 && p.u1 == p.s.ub;
+        const int part = p.u0 == 0;
+        for (int i = tid; i < p.rows * D; i += kThreads) {
             const int r = i / D, d = i % D;
             float mx = -INFINITY;
+#pragma unroll
             for (int x = 0; x < kWarps; x++) mx = fmaxf(mx, sm.wm[x][r]);
             const float ref = mx == -INFINITY ? 0.0f : mx;
             float o = 0.0f, sum = 0.0f;
+#pragma unroll
             for (int x = 0; x < kWarps; x++) {
                 const float f = ex2(sm.wm[x][r] - ref);
                 o = fmaf(f, sm.wo[x][r][d], o);
                 sum = fmaf(f, sm.wl[x][r], sum);
             }
             if (whole) {
-                if (r < rows) {
-                    const int row = qt * R + r;
-                    a.out[((int64_t)(s.off + row / G) * a.heads + h * G + row % G) * D + d] = __fdiv_rn(o, sum);
-                }
+                const int row = p.qt * R + r;
+                a.out[((int64_t)(p.s.off + row / G) * a.heads + p.h * G + row % G) * D + d] = __fdiv_rn(o, sum);
             } else {
-                __stcg(part + i, o);
+                sm.po[part][r][d] = o;
                 if (d == 0) {
-                    __stcg(part + R * D + r, mx);
-                    __stcg(part + R * D + R + r, sum);
+                    sm.pm[part][r] = mx;
+                    sm.pl[part][r] = sum;
                 }
             }
         }
-        if (!whole) {
-            // the item's blocks: the last of them to arrive joins all, in block order
-            const int i0 = (int)(((item0 + 1) * blocks - 1) / W);
-            const int i1 = (int)(((item0 + s.ub) * blocks - 1) / W);
-            __threadfence();
-            __syncthreads();
-            if (tid == 0) {
-                const unsigned n = atomicAdd(a.tickets + i0, 1u);
-                sm.last = n == (unsigned)(i1 - i0);
-                if (sm.last) a.tickets[i0] = 0u;
-            }
-            __syncthreads();
-            if (sm.last) {
-                __threadfence();
-                for (int i = tid; i < rows * D; i += kThreads) {
-                    const int r = i / D, d = i % D;
-                    float mx = -INFINITY, o = 0.0f, sum = 0.0f;
-                    for (int x = i0; x <= i1; x++) {
-                        const float *p = a.part + ((int64_t)x * 2 + (x == i0)) * (R * (D + 2));
-                        const float pm = __ldcg(p + R * D + r);
-                        const float to = fmaxf(mx, pm), ref = to == -INFINITY ? 0.0f : to;
-                        const float fa = ex2(mx - ref), fb = ex2(pm - ref);
-                        o = fmaf(fb, __ldcg(p + i), o * fa);
-                        sum = fmaf(fb, __ldcg(p + R * D + R + r), sum * fa);
-                        mx = to;
-                    }
-                    const int row = qt * R + r;
-                    a.out[((int64_t)(s.off + row / G) * a.heads + h * G + row % G) * D + d] = __fdiv_rn(o, sum);
-                }
-            }
-        }
+        if (!whole && part && tid == 0)
+            sm.open = Shared{1, p.h, p.qt, p.s.off, p.rows, split.block_of(item0 + p.s.ub - 1 - c0)};
         __syncthreads();
-        w += u1 - u0;
     }
+
+    // ---- the item that this block began and others ended: their first partials
+    cl.sync();
+    if (sm.open.there) {
+        const Shared e = sm.open;
+        for (int i = tid; i < e.rows * D; i += kThreads) {
+            const int r = i / D, d = i % D;
+            float pm[kMaxCluster], mx = sm.pm[1][r];
+#pragma unroll
+            for (int x = 1; x < kMaxCluster; x++) {
+                pm[x] = rank + x <= e.last ? cl.map_shared_rank(&sm, rank + x)->pm[0][r] : -INFINITY;
+                mx = fmaxf(mx, pm[x]);
+            }
+            const float f0 = ex2(sm.pm[1][r] - mx);
+            float o = f0 * sm.po[1][r][d], sum = f0 * sm.pl[1][r];
+#pragma unroll
+            for (int x = 1; x < kMaxCluster; x++) {
+                if (rank + x > e.last) break;
+                const Sm *q = cl.map_shared_rank(&sm, rank + x);
+                const float f = ex2(pm[x] - mx);
+                o = fmaf(f, q->po[0][r][d], o);
+                sum = fmaf(f, q->pl[0][r], sum);
+            }
+            const int row = e.qt * R + r;
+            a.out[((int64_t)(e.off + row / G) * a.heads + e.h * G + row % G) * D + d] = __fdiv_rn(o, sum);
+        }
+    }
+    cl.sync();  // no block leaves while another reads its partials
 }
 
+// A cluster launch of `kern` with `cs` blocks a cluster.
+void cluster_config(cudaLaunchConfig_t &cfg, cudaLaunchAttribute &at, int clusters, int cs, size_t smem) {
+    cfg = {};
+    cfg.gridDim = dim3(clusters, cs);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = 1;
+    at.val.clusterDim.y = cs;
+    at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+}
+
+constexpr int kSizes[3] = {8, 4, 2};  // blocks of a cluster
+
 template <int D, int NT, int ST>
-int launch(const AttendArgs &a, int blocks, cudaStream_t st) {
-    using Sm = Smem<D, NT, ST>;
-    const size_t smem = sizeof(Sm) + (size_t)a.streams * 8;
+size_t smem_of(int streams) { return sizeof(Smem<D, NT, ST>) + (size_t)streams * 8; }
+
+// How many clusters of each size run at once.
+template <int D, int NT, int ST>
+int clusters_of(const qora_kv4 *kv, int (&n)[3]) {
     auto kern = k_kv4_attend<D, NT, ST>;
-    if (smem > 48 * 1024)
-        QORA_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    return launch_ex(kern, dim3(blocks), dim3(kThreads), smem, st, 1u, a);
+    const size_t smem = smem_of<D, NT, ST>(kv->streams);
+    QORA_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    for (int i = 0; i < 3; i++) {
+        cudaLaunchConfig_t cfg;
+        cudaLaunchAttribute at;
+        cluster_config(cfg, at, 1, kSizes[i], smem);
+        QORA_CUDA(cudaOccupancyMaxActiveClusters(&n[i], kern, &cfg));
+        if (n[i] < 1) n[i] = 1;
+    }
+    return QORA_OK;
+}
+
+// The cluster size goes by the items (stream, kv head, row tile) that the call may
+// have: with few, a wide cluster puts more blocks on each; with many, narrow ones
+// leave no multiprocessor without a block (33 clusters of 8, 71 of 4 or 148 of 2
+// run at once).  Measured at 16 / 8 heads of 128, one token: 1 stream of 16384
+// positions 23.4 us with clusters of 8, 34.2 with 4; 8 streams of 4096 23.1 us with
+// 8, 19.5 with 4, 25.9 with 2; 32 streams of 4096 46.8 us with 8, 43.1 with 2.
+template <int D, int NT, int ST>
+int launch(const qora_kv4 *kv, const AttendArgs &a, const int (&n)[3], int64_t items, cudaStream_t st) {
+    auto kern = k_kv4_attend<D, NT, ST>;
+    const size_t smem = smem_of<D, NT, ST>(a.streams);
+    QORA_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    const int i = items <= n[0] ? 0 : items <= n[1] ? 1 : 2;
+    return launch_ex(kern, dim3(n[i], kSizes[i]), dim3(kThreads), smem, st, (unsigned)kSizes[i], a);
 }
 
 }  // namespace
 
-int kv4_attend_blocks(const qora_ctx *ctx) { return 2 * ctx->num_sms; }
+int kv4_attend_setup(qora_kv4 *kv) {
+    if (kv->hd == 64) {
+        QORA_TRY((clusters_of<64, 1, 2>(kv, kv->clusters[0])));
+        return clusters_of<64, 2, 4>(kv, kv->clusters[1]);
+    }
+    QORA_TRY((clusters_of<128, 1, 2>(kv, kv->clusters[0])));
+    return clusters_of<128, 2, 4>(kv, kv->clusters[1]);
+}
 
 }  // namespace qora
 
@@ -535,17 +669,17 @@ extern "C" int qora_kv4_attend(qora_kv4 *kv, int32_t layer, const float *q, cons
     a.offsets = offsets;
     a.len = kv->len.as<int>();
     a.out = out;
-    a.part = kv->part.as<float>();
-    a.tickets = kv->tickets.as<unsigned>();
     a.err = kv->ctx->err.as<int>();
     a.streams = kv->streams;
     a.heads = kv->heads;
     a.max_pos = kv->max_pos;
     a.tokens = tokens;
     a.scale_log2 = 1.4426950408889634f / sqrtf((float)kv->hd);
-    const int rows = kv->heads / kv->kvh * max_count;
-    const int sms = kv->ctx->num_sms;
+    const int64_t rows = kv->heads / kv->kvh * (int64_t)max_count;  // of a stream's kv head
+    const bool one = rows <= 4;
+    const int64_t items = (int64_t)kv->streams * kv->kvh * ((rows + (one ? 3 : 7)) / (one ? 4 : 8));
+    const auto &n = kv->clusters[one ? 0 : 1];
     cudaStream_t st = as_stream(stream);
-    if (kv->hd == 64) return rows <= 4 ? launch<64, 1, 2>(a, 2 * sms, st) : launch<64, 2, 4>(a, sms, st);
-    return rows <= 4 ? launch<128, 1, 2>(a, 2 * sms, st) : launch<128, 2, 4>(a, sms, st);
+    if (kv->hd == 64) return one ? launch<64, 1, 2>(kv, a, n, items, st) : launch<64, 2, 4>(kv, a, n, items, st);
+    return one ? launch<128, 1, 2>(kv, a, n, items, st) : launch<128, 2, 4>(kv, a, n, items, st);
 }
