@@ -70,6 +70,11 @@ inline Kv4Layer kv4_layer(const qora_kv4 *kv, int layer) {
 // Asks the device what the attention kernels' launches go by (at creation).
 int kv4_attend_setup(qora_kv4 *kv);
 
+// Attention of many new tokens per stream (at most max_rows query rows of a kv head
+// in one stream, as the host knows).
+int kv4_launch_prompt(qora_kv4 *kv, int layer, const float *q, const int *offsets, int tokens, int64_t max_rows,
+                      float *out, cudaStream_t st);
+
 // Byte offsets in a unit of head dimension D.
 template <int D>
 struct Kv4Unit {

@@ -676,6 +676,7 @@ extern "C" int qora_kv4_attend(qora_kv4 *kv, int32_t layer, const float *q, cons
     a.tokens = tokens;
     a.scale_log2 = 1.4426950408889634f / sqrtf((float)kv->hd);
     const int64_t rows = kv->heads / kv->kvh * (int64_t)max_count;  // of a stream's kv head
+    if (rows > 64) return kv4_launch_prompt(kv, layer, q, offsets, tokens, rows, out, as_stream(stream));
     const bool one = rows <= 4;
     const int64_t items = (int64_t)kv->streams * kv->kvh * ((rows + (one ? 3 : 7)) / (one ? 4 : 8));
     const auto &n = kv->clusters[one ? 0 : 1];

@@ -312,6 +312,9 @@ CASES = [
     (6, 2, 64, 32, [65, 129], [2, 7]),
     (32, 8, 128, 64, [1000], [1]),
     (4, 2, 128, 32, [0, 17], [70, 33]),                     # prompts
+    (16, 8, 128, 64, [0, 100], [129, 64]),
+    (6, 2, 64, 32, [40, 0, 3], [200, 1, 43]),
+    (2, 2, 128, 64, [300], [257]),
     (16, 8, 64, 64, [5] * 40, [1] * 40),
     (2, 1, 128, 32, [0, 0, 0], [0, 1, 0]),
     (16, 8, 128, 64, [2500, 40, 0], [1, 1, 1]),
@@ -340,7 +343,8 @@ def test_attend_any_range(ctx, q_size, k_size, v_size):
     lens, counts, heads, kvh, hd = [150, 3], [1, 2], 4, 2, 128
     kv, offsets, held, rng = _filled(ctx, lens, counts, heads, kvh, hd, 32, 5, k_size, v_size)
     q = (q_size * rng.standard_normal((3, heads, hd))).astype(np.float32)
-    _check(kv, q, offsets, held, lens, counts, heads, kvh, hd, 2)
+    for mc in (1, 2, 64):                                   # each of the kernels
+        _check(kv, q, offsets, held, lens, counts, heads, kvh, hd, mc)
     assert _error(ctx) == 0
 
 
@@ -355,17 +359,26 @@ def test_attend_sees_nothing_behind_the_last_position(ctx):
     bad = torch.full((len(behind), kvh * hd), float("nan"), device="cuda")
     kv.write(1, _i32(behind), bad, bad)
     q = rng.standard_normal((6, heads, hd)).astype(np.float32)
-    for mc in (1, 8):
+    for mc in (1, 8, 64):
         _check(kv, q, offsets, held, lens, counts, heads, kvh, hd, mc)
     # within a stream a NaN reaches the tokens that see it, and only those
-    k, v = kv.read(1, _i32([int(table[1, 0]) * page + 1]))
-    kv.write(1, _i32([int(table[1, 0]) * page + 1]), k * float("nan"), v)
-    out = kv.attend(1, _dev(q.reshape(6, -1)), offsets, 3)
-    nan = torch.isnan(out).any(-1).cpu().numpy()
-    assert list(nan) == [False, False, False, True, True, False]
+    at = _i32([int(table[1, 0]) * page + 1])
+    k, v = kv.read(1, at)
+    half = v.clone()
+    half[:, :32] = float("nan")                             # one scale group of the first kv head
+    for keys, values in ((k * float("nan"), v), (k, v * float("nan")), (k, half)):
+        kv.write(1, at, keys, values)
+        for mc in (1, 3, 64):
+            out = kv.attend(1, _dev(q.reshape(6, -1)), offsets, mc)
+            nan = torch.isnan(out).any(-1).cpu().numpy()
+            assert list(nan) == [False, False, False, True, True, False]
+            if values is half:
+                first = torch.isnan(out[3:5].view(2, heads, hd))
+                assert bool(first[:, :2, :32].all()) and int(first.sum()) == 2 * 2 * 32
     q[0, 1, 3] = np.inf
-    out = kv.attend(1, _dev(q.reshape(6, -1)), offsets, 3).view(6, heads, hd)
-    assert bool(torch.isnan(out[0, 1]).all()) and bool(torch.isfinite(out[0, 0]).all())
+    for mc in (1, 3, 64):
+        out = kv.attend(1, _dev(q.reshape(6, -1)), offsets, mc).view(6, heads, hd)
+        assert bool(torch.isnan(out[0, 1]).all()) and bool(torch.isfinite(out[0, 0]).all())
     assert _error(ctx) == 0
 
 
