@@ -32,8 +32,8 @@ constexpr int kRows = 128;                 // query rows of a block
 constexpr int kKeys = 64;                  // positions of a tile: two units
 constexpr int kSoftWarps = 8, kUnpackWarps = 4;
 constexpr int kThreads = (kSoftWarps + kUnpackWarps + 1) * 32;
-constexpr uint32_t kTmemCols = 512;        // S 2 x 64, P (high, low) 2 x 64, O 2 x 128
-constexpr uint32_t kColS = 0, kColP = 128, kColO = 256;
+constexpr uint32_t kTmemCols = 512;        // S 2 x 64, P (high, low) 2 x 64, O 128, Q (high, low) 128
+constexpr uint32_t kColS = 0, kColP = 128, kColO = 256, kColQ = 384;
 
 struct PromptArgs {
     Kv4Layer L;
@@ -45,25 +45,25 @@ struct PromptArgs {
     float scale_log2;  // log2(e) / sqrt(D)
 };
 
-// Operands in shared memory: core matrices of 8 rows x 16 bytes.  The distance
-// between neighbours along the contraction is 128 bytes for Q, 160 for K and 144
-// for V, so that the unpacking warps' 16-byte stores fall on distinct banks.
+// K and V in shared memory: core matrices of 8 rows x 16 bytes.  The distance
+// between neighbours along the contraction is 160 bytes for K and 144 for V, so
+// that the unpacking warps' 16-byte stores fall on distinct banks.  Q and P are
+// operands in tensor memory (Q from shared memory made the products' rate that of
+// its reads: 64 cycles for 128 x 64 x 16).
 template <int D>
 struct Sm {
-    static constexpr int kQ = kRows * D * 2;
     static constexpr int kKStep = 160, kVStep = 144;
     static constexpr int kK = (kKeys / 8) * (D / 8) * kKStep;
     static constexpr int kV = (D / 8) * (kKeys / 8) * kVStep;
-    alignas(1024) uint8_t q[2][kQ];        // high, low
     alignas(128) uint8_t k[2][2][kK];      // [buffer][high, low]
     alignas(128) uint8_t v[2][2][kV];
-    int rexp[kRows];                       // queries are scaled by 2^rexp
     float l[2][kRows], top[2][2][kRows];   // a row's sum, and largest score, by half
-    float unk[2], unv[2];                  // a tile's scales back
-    unsigned vnan[2][2][D / 32];           // positions of a unit whose value scale is NaN, by group
+    // of a tile (four deep: unpacking is up to three tiles ahead of the softmax)
+    float unk[4], unv[4];                  // its scales back
+    unsigned vnan[4][2][D / 32];           // positions of a unit whose value scale is NaN, by group
     unsigned most[2][kUnpackWarps];
-    int stop[2];
-    alignas(8) uint64_t full[2], empty[2], s_full[2], p_full[2], o_full[2];
+    alignas(8) uint64_t info[4];           // these are written (k_full may be a phase too far by then)
+    uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full, o_free;
     uint32_t tmem;
     int abort;
 };
@@ -90,6 +90,16 @@ __device__ __forceinline__ bool wait_one(uint64_t *bar, uint32_t parity, int *ab
         }
     }
     return true;
+}
+
+// Whether the phase is over, without waiting.
+__device__ __forceinline__ bool ready(uint64_t *bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+                 : "=r"(ok)
+                 : "r"(smem_u32(bar)), "r"(parity)
+                 : "memory");
+    return ok != 0;
 }
 
 // The same for a whole warp, with one answer.
@@ -151,12 +161,17 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const PromptArgs a) 
     if ((int)blockIdx.x >= nq) return;
     if (tid == 0) {
         for (int i = 0; i < 2; i++) {
-            mbar_init(&sm.full[i], kUnpackWarps);
-            mbar_init(&sm.empty[i], 1);
+            mbar_init(&sm.k_full[i], kUnpackWarps);
+            mbar_init(&sm.k_empty[i], 1);
+            mbar_init(&sm.v_full[i], kUnpackWarps);
+            mbar_init(&sm.v_empty[i], 1);
             mbar_init(&sm.s_full[i], 1);
             mbar_init(&sm.p_full[i], kSoftWarps);
-            mbar_init(&sm.o_full[i], 1);
         }
+        for (int i = 0; i < 4; i++) mbar_init(&sm.info[i], kUnpackWarps);
+        mbar_init(&sm.q_full, kSoftWarps);
+        mbar_init(&sm.o_full, 1);
+        mbar_init(&sm.o_free, kSoftWarps);
         sm.abort = 0;
         mbar_fence_init();
     }
@@ -172,57 +187,60 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const PromptArgs a) 
     tc::fence_after_sync();
     const uint32_t tmem = sm.tmem;
     int done = 0;  // tiles of this block's earlier row tiles: the barriers count on
-    for (int qi = blockIdx.x; qi < nq; qi += gridDim.x) {
+    int turn = 0;  // and row tiles
+    for (int qi = blockIdx.x; qi < nq; qi += gridDim.x, turn++) {
         const int row0 = (nq - 1 - qi) * kRows;  // the longest row tiles first
         const int rows = min(kRows, n * G - row0);
         const int first_limit = len + row0 / G;                // every row sees these positions
         const int kend = len + (row0 + rows - 1) / G + 1;      // positions that some row sees
         const int ntiles = (kend + kKeys - 1) / kKeys;
         const float *q = a.q + ((int64_t)off * a.heads + h * G) * D;  // row r: token r / G, head r % G
-        // ---- queries: a power of two per row, then high and low halves
-        for (int r = warp; r < kRows; r += kThreads / 32) {
-            float m = 0.0f;
-            if (r < rows) {
-                const float *x = q + ((int64_t)((row0 + r) / G) * a.heads + (row0 + r) % G) * D;
-                for (int d = lane; d < D; d += 32) m = fmaxf(m, fabsf(__ldg(x + d)));
-            }
-            m = warp_max(m);
-            // 2^e puts the row's largest value into [2^9, 2^10)
-            const int e = 136 - (int)(__float_as_uint(m) >> 23);
-            if (lane == 0) sm.rexp[r] = (m > 0.0f && isfinite(m)) ? max(-120, min(120, e)) : 0;
-        }
-        __syncthreads();
-        for (int i = tid; i < kRows * (D / 8); i += kThreads) {
-            const int r = (i & 7) | ((i / (8 * (D / 8))) << 3), kb = (i >> 3) % (D / 8);
-            float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-            if (r < rows) {
-                const float4 *src = reinterpret_cast<const float4 *>(
-                    q + ((int64_t)((row0 + r) / G) * a.heads + (row0 + r) % G) * D + 8 * kb);
-                const float4 u = __ldg(src), w = __ldg(src + 1);
-                x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w, x[4] = w.x, x[5] = w.y, x[6] = w.z, x[7] = w.w;
-            }
-            const float up = pow2(sm.rexp[r]);
-            uint32_t hi[4], lo[4];
-#pragma unroll
-            for (int j = 0; j < 4; j++) {  // a key's word gives its dimensions as pairs (j, j + 4)
-                const float y0 = x[j] * up, y1 = x[j + 4] * up;
-                const __half2 p = __floats2half2_rn(y0, y1);
-                hi[j] = h2u(p);
-                lo[j] = h2u(__floats2half2_rn(y0 - __low2float(p), y1 - __high2float(p)));
-            }
-            const int at = ((r >> 3) * (D / 8) + kb) * 128 + (r & 7) * 16;
-            *reinterpret_cast<uint4 *>(sm.q[0] + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-            *reinterpret_cast<uint4 *>(sm.q[1] + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-        }
-        tc::fence_proxy_async_smem();
-        __syncthreads();
-
         if (warp < kSoftWarps) {
             // ================================================= softmax
             const int hs = warp >> 2, r = 32 * (warp & 3) + lane;
             const uint32_t t_lane = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
             const int limit = r < rows ? len + (row0 + r) / G : -1;
-            const float rs = pow2(-sm.rexp[r]) * a.scale_log2;
+            // ---- the row's queries: a power of two, then high and low halves; a thread has
+            // half of the dimensions, in the order in which a key's words give them
+            float rs;
+            {
+                constexpr int H = D / 2;
+                float x[H], most = 0.0f;
+                const float4 *src = reinterpret_cast<const float4 *>(
+                    q + ((int64_t)((row0 + r) / G) * a.heads + (row0 + r) % G) * D + H * hs);
+#pragma unroll
+                for (int i = 0; i < H / 4; i++) {
+                    const float4 u = r < rows ? __ldg(src + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    x[4 * i] = u.x, x[4 * i + 1] = u.y, x[4 * i + 2] = u.z, x[4 * i + 3] = u.w;
+                    most = fmaxf(fmaxf(most, fmaxf(fabsf(u.x), fabsf(u.y))), fmaxf(fabsf(u.z), fabsf(u.w)));
+                }
+                sm.top[0][hs][r] = most;
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                most = fmaxf(most, sm.top[0][hs ^ 1][r]);
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                // 2^e puts the row's largest value into [2^9, 2^10)
+                const int e0 = 136 - (int)(__float_as_uint(most) >> 23);
+                const int e = (most > 0.0f && isfinite(most)) ? max(-120, min(120, e0)) : 0;
+                rs = pow2(-e) * a.scale_log2;
+                const float up = pow2(e);
+#pragma unroll
+                for (int p = 0; p < H / 32; p++) {
+                    uint32_t hi[16], lo[16];
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {  // columns of four to an 8-dimension block: pairs (j, j + 4)
+                        const int at = 32 * p + 8 * (i >> 2) + (i & 3);
+                        const float y0 = x[at] * up, y1 = x[at + 4] * up;
+                        const __half2 w = __floats2half2_rn(y0, y1);
+                        hi[i] = h2u(w);
+                        lo[i] = h2u(__floats2half2_rn(y0 - __low2float(w), y1 - __high2float(w)));
+                    }
+                    tc::st_32x32b_x16(t_lane + kColQ + (D / 4) * hs + 16 * p, hi);
+                    tc::st_32x32b_x16(t_lane + kColQ + D / 2 + (D / 4) * hs + 16 * p, lo);
+                }
+                tc::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sm.q_full);
+            }
             float m = -INFINITY, l = 0.0f, corr = 0.0f, unv = 0.0f;
             float o[D / 2];
 #pragma unroll
@@ -230,30 +248,33 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const PromptArgs a) 
             // adds O of tile `it` (which the products have finished)
             auto fold = [&](int it) {
                 const int gi = done + it;
-                wait_for(&sm.o_full[gi & 1], (gi >> 1) & 1, &sm.abort, a.err);
+                wait_for(&sm.o_full, gi & 1, &sm.abort, a.err);
                 tc::fence_after_sync();
 #pragma unroll
                 for (int p = 0; p < D / 64; p++) {
                     float u[32];
-                    tc::ld_32x32b_x32(t_lane + kColO + 128 * (gi & 1) + (D / 2) * hs + 32 * p, u);
+                    tc::ld_32x32b_x32(t_lane + kColO + (D / 2) * hs + 32 * p, u);
 #pragma unroll
                     for (int i = 0; i < 32; i++) o[32 * p + i] = fmaf(u[i], unv, o[32 * p + i] * corr);
                 }
+                tc::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sm.o_free);
             };
             for (int it = 0; it < ntiles; it++) {
-                const int gi = done + it, buf = gi & 1;
+                const int gi = done + it, buf = gi & 1, slot = gi & 3;
                 // (after a wait that ran out the loop goes on over what is there: its
                 // waits return at once, and no warp leaves another at a barrier)
-                wait_for(&sm.full[buf], (gi >> 1) & 1, &sm.abort, a.err);  // what unpacking says of the tile
+                wait_for(&sm.info[slot], (gi >> 2) & 1, &sm.abort, a.err);
                 wait_for(&sm.s_full[buf], (gi >> 1) & 1, &sm.abort, a.err);
                 tc::fence_after_sync();
-                const float f = rs * sm.unk[buf];
-                const float unv_now = sm.unv[buf];
+                const float f = rs * sm.unk[slot];
+                const float unv_now = sm.unv[slot];
                 unsigned bad[C / 2][2], any = 0;  // of this thread's groups of dimensions
 #pragma unroll
                 for (int c = 0; c < C / 2; c++)
 #pragma unroll
-                    for (int u = 0; u < 2; u++) any |= bad[c][u] = sm.vnan[buf][u][hs * (C / 2) + c];
+                    for (int u = 0; u < 2; u++) any |= bad[c][u] = sm.vnan[slot][u][hs * (C / 2) + c];
                 float x[32];
                 tc::ld_32x32b_x32(t_lane + kColS + 64 * buf + 32 * hs, x);
                 const int left = limit - it * kKeys;  // the row sees columns up to here
@@ -350,7 +371,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const PromptArgs a) 
                 r.vs0 = __ldg(reinterpret_cast<const uint2 *>(u + U::kVs + c * 64 + 2 * t * 8));
                 r.vs1 = __ldg(reinterpret_cast<const uint2 *>(u + U::kVs + c * 64 + (2 * t + 1) * 8));
             };
-            Raw raw[kJobs];
+            Raw raw[kJobs], next[kJobs];
             int page[kJobs];
 #pragma unroll
             for (int j = 0; j < kJobs; j++) {
@@ -358,7 +379,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const PromptArgs a) 
                 page[j] = page_of(1, j);
             }
             for (int it = 0; it < ntiles; it++) {
-                const int gi = done + it, buf = gi & 1;
+                const int gi = done + it, buf = gi & 1, slot = gi & 3;
+                // the next tile is in flight while this one is unpacked
+#pragma unroll
+                for (int j = 0; j < kJobs; j++) {
+                    load(it + 1, j, page[j], next[j]);
+                    page[j] = page_of(it + 2, j);
+                }
                 // scales behind the last position count as zero, NaN ones are told to the rows
                 unsigned kmost = 0, vmost = 0;
                 unsigned nan[kJobs];
@@ -390,10 +417,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const PromptArgs a) 
                 kmost = __reduce_max_sync(0xffffffffu, kmost);
                 vmost = __reduce_max_sync(0xffffffffu, vmost);
                 if (lane == 0) sm.most[buf][pw] = kmost << 16 | vmost;
-                const bool ok = gi < 2 || wait_for(&sm.empty[buf], ((gi >> 1) - 1) & 1, &sm.abort, a.err);
-                if (pw == 0 && lane == 0) sm.stop[buf] = !ok;  // one warp decides for all that meet below
                 asm volatile("bar.sync 2, 128;" ::: "memory");
-                if (sm.stop[buf]) break;
                 kmost = vmost = 0;
 #pragma unroll
                 for (int i = 0; i < kUnpackWarps; i++) {
@@ -402,11 +426,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const PromptArgs a) 
                 }
                 const int ek = scale_exponent(kmost), ev = scale_exponent(vmost);
                 const float upk = pow2(ek), upv = pow2(ev);
+                if (gi >= 2) wait_for(&sm.k_empty[buf], ((gi >> 1) - 1) & 1, &sm.abort, a.err);
 #pragma unroll
                 for (int j = 0; j < kJobs; j++) {
                     const int combo = pw + kUnpackWarps * j, c = combo % C, u = combo / C;
                     const uint32_t kw[4] = {raw[j].k.x, raw[j].k.y, raw[j].k.z, raw[j].k.w};
-                    const uint32_t vw[4] = {raw[j].v.x, raw[j].v.y, raw[j].v.z, raw[j].v.w};
                     // keys g + 8i: dimensions 32c + 8t .. + 7 are one operand row of 16 bytes
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
@@ -424,7 +448,24 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const PromptArgs a) 
                         *reinterpret_cast<uint4 *>(sm.k[buf][0] + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
                         *reinterpret_cast<uint4 *>(sm.k[buf][1] + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                     }
-                    // dimensions 32c + 4g + p: positions 2t + e + 8h are one operand row
+                    if (lane == 0) sm.vnan[slot][u][c] = nan[j];
+                }
+                if (pw == 0 && lane == 0) {
+                    sm.unk[slot] = pow2(-ek);
+                    sm.unv[slot] = pow2(-ev);
+                }
+                tc::fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&sm.info[slot]);
+                    mbar_arrive(&sm.k_full[buf]);
+                }
+                if (gi >= 2) wait_for(&sm.v_empty[buf], ((gi >> 1) - 1) & 1, &sm.abort, a.err);
+#pragma unroll
+                for (int j = 0; j < kJobs; j++) {
+                    const int combo = pw + kUnpackWarps * j, c = combo % C, u = combo / C;
+                    const uint32_t vw[4] = {raw[j].v.x, raw[j].v.y, raw[j].v.z, raw[j].v.w};
+                    // dimensions 32c + 4g + p: positions 2t + e + 8i are one operand row
                     uint32_t hi[4][4], lo[4][4];
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
@@ -445,61 +486,72 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const PromptArgs a) 
                         *reinterpret_cast<uint4 *>(sm.v[buf][0] + at) = make_uint4(hi[p][0], hi[p][1], hi[p][2], hi[p][3]);
                         *reinterpret_cast<uint4 *>(sm.v[buf][1] + at) = make_uint4(lo[p][0], lo[p][1], lo[p][2], lo[p][3]);
                     }
-                    if (lane == 0) sm.vnan[buf][u][c] = nan[j];
-                    load(it + 1, j, page[j], raw[j]);  // in flight while the next tile's buffer empties
-                    page[j] = page_of(it + 2, j);
-                }
-                if (pw == 0 && lane == 0) {
-                    sm.unk[buf] = pow2(-ek);
-                    sm.unv[buf] = pow2(-ev);
+                    raw[j] = next[j];
                 }
                 tc::fence_proxy_async_smem();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&sm.full[buf]);
+                if (lane == 0) mbar_arrive(&sm.v_full[buf]);
             }
         } else {
             // ================================================= products
             if (lane == 0) {
                 constexpr uint32_t id_s = tc::idesc_f16_f32(kRows, kKeys), id_o = tc::idesc_f16_f32(kRows, D);
-                const uint32_t qh = smem_u32(sm.q[0]), ql = smem_u32(sm.q[1]);
-                auto out_of = [&](int gi) {  // O of a tile whose P is there
-                    const int buf = gi & 1;
-                    if (!wait_one(&sm.p_full[buf], (gi >> 1) & 1, &sm.abort, a.err)) return false;
-                    tc::fence_after_sync();
-                    const uint32_t vh = smem_u32(sm.v[buf][0]), vl = smem_u32(sm.v[buf][1]);
-                    const uint32_t d = tmem + kColO + 128 * buf, p = tmem + kColP + 64 * buf;
-#pragma unroll
-                    for (int j = 0; j < kKeys / 16; j++) {
-                        const uint64_t bh = tc::smem_desc(vh + 2 * S::kVStep * j, S::kVStep, (kKeys / 8) * S::kVStep);
-                        const uint64_t bl = tc::smem_desc(vl + 2 * S::kVStep * j, S::kVStep, (kKeys / 8) * S::kVStep);
-                        tc::mma_f16_ts(d, p + 8 * j, bh, id_o, j != 0 ? 1u : 0u);
-                        tc::mma_f16_ts(d, p + 8 * j, bl, id_o, 1u);
-                        tc::mma_f16_ts(d, p + 32 + 8 * j, bh, id_o, 1u);
-                    }
-                    tc::commit(&sm.o_full[buf]);
-                    tc::commit(&sm.empty[buf]);
-                    return true;
-                };
-                for (int it = 0; it <= ntiles; it++) {
-                    const int gi = done + it, buf = gi & 1;
-                    if (it < ntiles) {
-                        if (!wait_one(&sm.full[buf], (gi >> 1) & 1, &sm.abort, a.err)) break;
+                const uint32_t qt = tmem + kColQ;
+                bool go = wait_one(&sm.q_full, turn & 1, &sm.abort, a.err);
+                tc::fence_after_sync();
+                // S of tile ns and O of tile no, each as soon as its operands are there; S has
+                // two buffers, so it is at most two tiles ahead
+                int ns = 0, no = 0;
+                uint64_t t0 = global_ns();
+                while (go && no < ntiles) {
+                    bool did = false;
+                    const int gs = done + ns, go_ = done + no;
+                    if (ns < ntiles && ns <= no + 1 && ready(&sm.k_full[gs & 1], (gs >> 1) & 1)) {
                         tc::fence_after_sync();
+                        const int buf = gs & 1;
                         const uint32_t kh = smem_u32(sm.k[buf][0]), kl = smem_u32(sm.k[buf][1]);
                         const uint32_t d = tmem + kColS + 64 * buf;
 #pragma unroll
                         for (int j = 0; j < D / 16; j++) {
-                            const uint64_t ah = tc::smem_desc(qh + 256 * j, 128, (D / 8) * 128);
-                            const uint64_t al = tc::smem_desc(ql + 256 * j, 128, (D / 8) * 128);
                             const uint64_t bh = tc::smem_desc(kh + 2 * S::kKStep * j, S::kKStep, (D / 8) * S::kKStep);
                             const uint64_t bl = tc::smem_desc(kl + 2 * S::kKStep * j, S::kKStep, (D / 8) * S::kKStep);
-                            tc::mma_f16(d, ah, bh, id_s, j != 0 ? 1u : 0u);
-                            tc::mma_f16(d, ah, bl, id_s, 1u);
-                            tc::mma_f16(d, al, bh, id_s, 1u);
+                            tc::mma_f16_ts(d, qt + 8 * j, bh, id_s, j != 0 ? 1u : 0u);
+                            tc::mma_f16_ts(d, qt + 8 * j, bl, id_s, 1u);
+                            tc::mma_f16_ts(d, qt + D / 2 + 8 * j, bh, id_s, 1u);
                         }
                         tc::commit(&sm.s_full[buf]);
+                        tc::commit(&sm.k_empty[buf]);
+                        ns++;
+                        did = true;
                     }
-                    if (it > 0 && !out_of(gi - 1)) break;
+                    if (no < ns && ready(&sm.p_full[go_ & 1], (go_ >> 1) & 1) && ready(&sm.v_full[go_ & 1], (go_ >> 1) & 1) &&
+                        (go_ == 0 || ready(&sm.o_free, (go_ - 1) & 1))) {
+                        tc::fence_after_sync();
+                        const int buf = go_ & 1;
+                        const uint32_t vh = smem_u32(sm.v[buf][0]), vl = smem_u32(sm.v[buf][1]);
+                        const uint32_t d = tmem + kColO, p = tmem + kColP + 64 * buf;
+#pragma unroll
+                        for (int j = 0; j < kKeys / 16; j++) {
+                            const uint64_t bh = tc::smem_desc(vh + 2 * S::kVStep * j, S::kVStep, (kKeys / 8) * S::kVStep);
+                            const uint64_t bl = tc::smem_desc(vl + 2 * S::kVStep * j, S::kVStep, (kKeys / 8) * S::kVStep);
+                            tc::mma_f16_ts(d, p + 8 * j, bh, id_o, j != 0 ? 1u : 0u);
+                            tc::mma_f16_ts(d, p + 8 * j, bl, id_o, 1u);
+                            tc::mma_f16_ts(d, p + 32 + 8 * j, bh, id_o, 1u);
+                        }
+                        tc::commit(&sm.o_full);
+                        tc::commit(&sm.v_empty[buf]);
+                        no++;
+                        did = true;
+                    }
+                    if (did) {
+                        t0 = global_ns();
+                    } else if (*(volatile int *)&sm.abort) {
+                        go = false;
+                    } else if (global_ns() - t0 > 1000000000ull) {
+                        raise_error(a.err, kDevTimeout);
+                        *(volatile int *)&sm.abort = 1;
+                        go = false;
+                    }
                 }
             }
             __syncwarp();
