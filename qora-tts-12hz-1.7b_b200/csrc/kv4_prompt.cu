@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const PromptArgs a) 
     S &sm = *reinterpret_cast<S *>(dyn);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, t = lane & 3;
-    const int h = blockIdx.y, b = blockIdx.z;
+    const int h = blockIdx.x % a.L.kvh, b = blockIdx.x / a.L.kvh;
     const int G = a.heads / a.L.kvh;
     griddep_wait();
     const int len = a.len[b], off = a.offsets[b];
@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const PromptArgs a) 
         return;
     }
     const int nq = (int)(((int64_t)n * G + kRows - 1) / kRows);
-    if ((int)blockIdx.x >= nq) return;
+    if ((int)blockIdx.y >= nq) return;
     if (tid == 0) {
         for (int i = 0; i < 2; i++) {
             mbar_init(&sm.k_full[i], kUnpackWarps);
@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const PromptArgs a) 
     const uint32_t tmem = sm.tmem;
     int done = 0;  // tiles of this block's earlier row tiles: the barriers count on
     int turn = 0;  // and row tiles
-    for (int qi = blockIdx.x; qi < nq; qi += gridDim.x, turn++) {
+    for (int qi = blockIdx.y; qi < nq; qi += gridDim.y, turn++) {
         const int row0 = (nq - 1 - qi) * kRows;  // the longest row tiles first
         const int rows = min(kRows, n * G - row0);
         const int first_limit = len + row0 / G;                // every row sees these positions
@@ -386,32 +386,35 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const PromptArgs a) 
                     load(it + 1, j, page[j], next[j]);
                     page[j] = page_of(it + 2, j);
                 }
-                // scales behind the last position count as zero, NaN ones are told to the rows
+                // the largest scales; ones behind the last position count as zero, and NaN
+                // ones are told to the rows (both are rare: a packed maximum finds them)
                 unsigned kmost = 0, vmost = 0;
                 unsigned nan[kJobs];
 #pragma unroll
                 for (int j = 0; j < kJobs; j++) {
                     const int pos = it * kKeys + ((pw + kUnpackWarps * j) / C) * kKv4Unit;
-                    unsigned short ks[4], v0[4], v1[4];
-                    const uint2 *src[3] = {&raw[j].ks, &raw[j].vs0, &raw[j].vs1};
-                    unsigned short *dst[3] = {ks, v0, v1};
-#pragma unroll
-                    for (int x = 0; x < 3; x++) {
-                        dst[x][0] = src[x]->x & 0xffff, dst[x][1] = src[x]->x >> 16;
-                        dst[x][2] = src[x]->y & 0xffff, dst[x][3] = src[x]->y >> 16;
-                    }
                     nan[j] = 0;
+                    const unsigned k2 = __vmaxu2(raw[j].ks.x, raw[j].ks.y);
+                    const unsigned v2 = __vmaxu2(__vmaxu2(raw[j].vs0.x, raw[j].vs0.y), __vmaxu2(raw[j].vs1.x, raw[j].vs1.y));
+                    const unsigned k1 = max(k2 & 0xffffu, k2 >> 16), v1 = max(v2 & 0xffffu, v2 >> 16);
+                    if (!__any_sync(0xffffffffu, max(k1, v1) >= 0x7c00u) && pos + kKv4Unit <= kend) {
+                        kmost = max(kmost, k1), vmost = max(vmost, v1);
+                        continue;
+                    }
+                    unsigned v0x[4] = {raw[j].vs0.x & 0xffffu, raw[j].vs0.x >> 16, raw[j].vs0.y & 0xffffu, raw[j].vs0.y >> 16};
+                    unsigned v1x[4] = {raw[j].vs1.x & 0xffffu, raw[j].vs1.x >> 16, raw[j].vs1.y & 0xffffu, raw[j].vs1.y >> 16};
+                    const unsigned kx[4] = {raw[j].ks.x & 0xffffu, raw[j].ks.x >> 16, raw[j].ks.y & 0xffffu, raw[j].ks.y >> 16};
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        if (pos + 2 * t + 8 * i >= kend) v0[i] = 0;
-                        if (pos + 2 * t + 1 + 8 * i >= kend) v1[i] = 0;
-                        if ((v0[i] & 0x7c00) == 0x7c00) nan[j] |= 1u << (2 * t + 8 * i), v0[i] = 0;
-                        if ((v1[i] & 0x7c00) == 0x7c00) nan[j] |= 2u << (2 * t + 8 * i), v1[i] = 0;
-                        if ((ks[i] & 0x7c00) != 0x7c00) kmost = max(kmost, (unsigned)ks[i]);
-                        vmost = max(vmost, max((unsigned)v0[i], (unsigned)v1[i]));
+                        if (pos + 2 * t + 8 * i >= kend) v0x[i] = 0;
+                        if (pos + 2 * t + 1 + 8 * i >= kend) v1x[i] = 0;
+                        if (v0x[i] >= 0x7c00u) nan[j] |= 1u << (2 * t + 8 * i), v0x[i] = 0;
+                        if (v1x[i] >= 0x7c00u) nan[j] |= 2u << (2 * t + 8 * i), v1x[i] = 0;
+                        if (kx[i] < 0x7c00u) kmost = max(kmost, kx[i]);
+                        vmost = max(vmost, max(v0x[i], v1x[i]));
                     }
-                    raw[j].vs0 = make_uint2(v0[0] | (unsigned)v0[1] << 16, v0[2] | (unsigned)v0[3] << 16);
-                    raw[j].vs1 = make_uint2(v1[0] | (unsigned)v1[1] << 16, v1[2] | (unsigned)v1[3] << 16);
+                    raw[j].vs0 = make_uint2(v0x[0] | v0x[1] << 16, v0x[2] | v0x[3] << 16);
+                    raw[j].vs1 = make_uint2(v1x[0] | v1x[1] << 16, v1x[2] | v1x[3] << 16);
                     nan[j] = __reduce_or_sync(0xffffffffu, nan[j]);
                 }
                 kmost = __reduce_max_sync(0xffffffffu, kmost);
@@ -571,8 +574,10 @@ int launch(const PromptArgs &a, int64_t max_rows, cudaStream_t st) {
     auto kern = k_kv4_prompt<D>;
     QORA_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Sm<D>)));
     const int64_t tiles = (max_rows + kRows - 1) / kRows;
-    const unsigned x = (unsigned)(tiles < 65536 ? tiles : 65536);  // a block takes further tiles in turn
-    return launch_ex(kern, dim3(x, a.L.kvh, a.streams), dim3(kThreads), sizeof(Sm<D>), st, 1u, a);
+    const unsigned y = (unsigned)(tiles < 65535 ? tiles : 65535);  // a block takes further tiles in turn
+    // blocks start in the order of x first: the longest row tile of every stream and
+    // head before the second longest of any
+    return launch_ex(kern, dim3(a.L.kvh * a.streams, y), dim3(kThreads), sizeof(Sm<D>), st, 1u, a);
 }
 
 }  // namespace
