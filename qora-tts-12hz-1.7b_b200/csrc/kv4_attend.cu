@@ -187,6 +187,8 @@ struct Smem {
     float wm[kWarps][R], wl[kWarps][R];
     float po[2][R][D];       // partials: [0] of the item that a block before began, [1] of the one begun here
     float pm[2][R], pl[2][R];
+    uint2 qf[NT][D / 16][NT > 1 ? 32 : 1];  // query fragments, by lane
+    float rs[R];                                            // and their scales back
     uint64_t full[kWarps][ST];
     int64_t scan[kWarps];
     Shared open;
@@ -194,7 +196,7 @@ struct Smem {
 };
 
 template <int D, int NT, int ST>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) k_kv4_attend(const AttendArgs a) {
+__global__ void __launch_bounds__(kThreads, 2) k_kv4_attend(const AttendArgs a) {
     using Sm = Smem<D, NT, ST>;
     using U = Kv4Unit<D>;
     constexpr int R = Sm::R, C = D / 32;
@@ -320,13 +322,9 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) k_kv4_attend(const 
         p.locate(a, G, b, w - sm.start[b], w1 - w, warp);
         first_limit = p.s.len + p.tok0;
 
-        // ---- query fragments: column n = 2 row + {hi, lo}
-        uint32_t bq[NT][2 * C][2];
-        float rs[NT], m[NT], l[NT];
-        int limit[NT];
-        float acc[NT][C][4];
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
+        // ---- query fragments: column n = 2 row + {hi, lo}.  A tile of one column group has
+        // them in registers, every warp its own; a wider one in shared memory.
+        auto load_q = [&](int nt, uint32_t (&f)[2 * C][2]) {
             const int row = p.qt * R + nt * 4 + (g >> 1);
             const bool have = row < p.s.n * G;
             const float4 *q = reinterpret_cast<const float4 *>(
@@ -356,9 +354,29 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) k_kv4_attend(const 
                     const float h0 = __half2float(__float2half_rn(y0)), h1 = __half2float(__float2half_rn(y1));
                     if (g & 1) y0 -= h0, y1 -= h1;
                     else y0 = h0, y1 = h1;
-                    bq[nt][2 * c + (j >> 1)][j & 1] = h2u(__floats2half2_rn(y0, y1));
+                    f[2 * c + (j >> 1)][j & 1] = h2u(__floats2half2_rn(y0, y1));
                 }
-            rs[nt] = __shfl_sync(0xffffffffu, down, t * 8) * a.scale_log2;
+            return down * a.scale_log2;  // of row g >> 1
+        };
+        uint32_t bq[2 * C][2];
+        float rs[NT], m[NT], l[NT];
+        int limit[NT];
+        float acc[NT][C][4];
+        if constexpr (NT == 1) {
+            rs[0] = load_q(0, bq);
+            rs[0] = __shfl_sync(0xffffffffu, rs[0], t * 8);
+        } else {
+            if (warp < NT) {
+                const float r = load_q(warp, bq);
+#pragma unroll
+                for (int i = 0; i < 2 * C; i++) sm.qf[warp][i][lane] = make_uint2(bq[i][0], bq[i][1]);
+                if ((lane & 7) == 0) sm.rs[warp * 4 + (lane >> 3)] = r;
+            }
+            __syncthreads();
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            if constexpr (NT > 1) rs[nt] = sm.rs[nt * 4 + t];
             const int mr = p.qt * R + nt * 4 + t;  // this lane's row
             limit[nt] = mr < p.s.n * G ? p.s.len + mr / G : -1;
             m[nt] = -INFINITY;
@@ -389,17 +407,26 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) k_kv4_attend(const 
             for (int c = 0; c < C; c++) {
                 const uint4 kw = *reinterpret_cast<const uint4 *>(unit + U::kK + c * 512 + lane * 16);
                 const uint2 ks = *reinterpret_cast<const uint2 *>(unit + U::kKs + c * 64 + g * 8);
+                uint32_t x[4][4];  // positions g, g + 8, g + 16, g + 24
+                codes(kw.x, magic, x[0]);
+                codes(kw.y, magic, x[1]);
+                codes(kw.z, magic, x[2]);
+                codes(kw.w, magic, x[3]);
 #pragma unroll
-                for (int rt = 0; rt < 2; rt++) {
-                    uint32_t x0[4], x1[4];
-                    codes(rt ? kw.z : kw.x, magic, x0);
-                    codes(rt ? kw.w : kw.y, magic, x1);
-                    const float f0 = scale_of(ks, 2 * rt), f1 = scale_of(ks, 2 * rt + 1);
+                for (int nt = 0; nt < NT; nt++) {
+                    uint2 b0, b1;
+                    if constexpr (NT == 1) {
+                        b0 = make_uint2(bq[2 * c][0], bq[2 * c][1]), b1 = make_uint2(bq[2 * c + 1][0], bq[2 * c + 1][1]);
+                    } else {
+                        b0 = sm.qf[nt][2 * c][lane], b1 = sm.qf[nt][2 * c + 1][lane];
+                    }
 #pragma unroll
-                    for (int nt = 0; nt < NT; nt++) {
+                    for (int rt = 0; rt < 2; rt++) {
+                        const uint32_t(&x0)[4] = x[2 * rt], (&x1)[4] = x[2 * rt + 1];
+                        const float f0 = scale_of(ks, 2 * rt), f1 = scale_of(ks, 2 * rt + 1);
                         float d[4];
-                        mma16816_first(d, x0[0], x1[0], x0[1], x1[1], bq[nt][2 * c][0], bq[nt][2 * c][1]);
-                        mma16816(d, x0[2], x1[2], x0[3], x1[3], bq[nt][2 * c + 1][0], bq[nt][2 * c + 1][1]);
+                        mma16816_first(d, x0[0], x1[0], x0[1], x1[1], b0.x, b0.y);
+                        mma16816(d, x0[2], x1[2], x0[3], x1[3], b1.x, b1.y);
                         sc[nt][2 * rt] = fmaf(f0, d[0], sc[nt][2 * rt]);
                         sl[nt][2 * rt] = fmaf(f0, d[1], sl[nt][2 * rt]);
                         sc[nt][2 * rt + 1] = fmaf(f1, d[2], sc[nt][2 * rt + 1]);
@@ -452,47 +479,34 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) k_kv4_attend(const 
             }
 #pragma unroll
             for (int c = 0; c < C; c++) {
-                uint32_t bp[NT][4];
-                if (edge) {  // whatever lies behind a row's last position counts as zero
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-#pragma unroll
-                        for (int nt = 0; nt < NT; nt++)
-                            bp[nt][i] = split_hi_lo(sc[nt][i] == 0.0f ? 0.0f : sc[nt][i] * scale_of(vs[c], i));
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-#pragma unroll
-                        for (int nt = 0; nt < NT; nt++) bp[nt][i] = split_hi_lo(sc[nt][i] * scale_of(vs[c], i));
-                }
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-#pragma unroll
-                    for (int nt = 0; nt < NT; nt++) bp[nt][i] = transpose8x8(bp[nt][i]);
                 const uint4 vw = *reinterpret_cast<const uint4 *>(unit + U::kV + c * 512 + lane * 16);
-                float d0[NT][4], d1[NT][4];
-#pragma unroll
-                for (int rt = 0; rt < 2; rt++) {
-                    uint32_t x0[4], x1[4];
-                    codes(rt ? vw.z : vw.x, magic, x0);
-                    codes(rt ? vw.w : vw.y, magic, x1);
-#pragma unroll
-                    for (int nt = 0; nt < NT; nt++) {
-                        if (rt == 0) {
-                            mma16816_first(d0[nt], x0[0], x0[1], x1[0], x1[1], bp[nt][0], bp[nt][1]);
-                            mma16816_first(d1[nt], x0[2], x0[3], x1[2], x1[3], bp[nt][0], bp[nt][1]);
-                        } else {
-                            mma16816(d0[nt], x0[0], x0[1], x1[0], x1[1], bp[nt][2], bp[nt][3]);
-                            mma16816(d1[nt], x0[2], x0[3], x1[2], x1[3], bp[nt][2], bp[nt][3]);
-                        }
-                    }
-                }
+                uint32_t x[4][4];
+                codes(vw.x, magic, x[0]);
+                codes(vw.y, magic, x[1]);
+                codes(vw.z, magic, x[2]);
+                codes(vw.w, magic, x[3]);
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
-                    acc[nt][c][0] = fmaf(acc[nt][c][0], keep[nt], d0[nt][0] + d0[nt][1]);
-                    acc[nt][c][1] = fmaf(acc[nt][c][1], keep[nt], d0[nt][2] + d0[nt][3]);
-                    acc[nt][c][2] = fmaf(acc[nt][c][2], keep[nt], d1[nt][0] + d1[nt][1]);
-                    acc[nt][c][3] = fmaf(acc[nt][c][3], keep[nt], d1[nt][2] + d1[nt][3]);
+                    uint32_t bp[4];
+                    if (edge) {  // whatever lies behind a row's last position counts as zero
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            bp[i] = split_hi_lo(sc[nt][i] == 0.0f ? 0.0f : sc[nt][i] * scale_of(vs[c], i));
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) bp[i] = split_hi_lo(sc[nt][i] * scale_of(vs[c], i));
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; i++) bp[i] = transpose8x8(bp[i]);
+                    float d0[4], d1[4];
+                    mma16816_first(d0, x[0][0], x[0][1], x[1][0], x[1][1], bp[0], bp[1]);
+                    mma16816_first(d1, x[0][2], x[0][3], x[1][2], x[1][3], bp[0], bp[1]);
+                    mma16816(d0, x[2][0], x[2][1], x[3][0], x[3][1], bp[2], bp[3]);
+                    mma16816(d1, x[2][2], x[2][3], x[3][2], x[3][3], bp[2], bp[3]);
+                    acc[nt][c][0] = fmaf(acc[nt][c][0], keep[nt], d0[0] + d0[1]);
+                    acc[nt][c][1] = fmaf(acc[nt][c][1], keep[nt], d0[2] + d0[3]);
+                    acc[nt][c][2] = fmaf(acc[nt][c][2], keep[nt], d1[0] + d1[1]);
+                    acc[nt][c][3] = fmaf(acc[nt][c][3], keep[nt], d1[2] + d1[3]);
                 }
             }
             __syncwarp();  // the stage is read
@@ -639,14 +653,24 @@ int launch(const qora_kv4 *kv, const AttendArgs &a, const int (&n)[3], int64_t i
 
 }  // namespace
 
-int kv4_attend_setup(qora_kv4 *kv) {
-    if (kv->hd == 64) {
-        QORA_TRY((clusters_of<64, 1, 2>(kv, kv->clusters[0])));
-        return clusters_of<64, 2, 4>(kv, kv->clusters[1]);
-    }
-    QORA_TRY((clusters_of<128, 1, 2>(kv, kv->clusters[0])));
-    return clusters_of<128, 2, 4>(kv, kv->clusters[1]);
+namespace {
+template <int D>
+int setup(qora_kv4 *kv) {
+    QORA_TRY((clusters_of<D, 1, 2>(kv, kv->clusters[0])));
+    return clusters_of<D, 2, 1>(kv, kv->clusters[1]);
 }
+// Row tiles of 4 or 8.  (Tiles of 12 read the cache once where these read it twice,
+// but do not fit 128 registers: 6 drafts of 16 streams of 4096 took 58 us against 40.)
+template <int D>
+int launch_rows(const qora_kv4 *kv, const AttendArgs &a, int64_t rows, cudaStream_t st) {
+    const int nt = rows <= 4 ? 1 : 2;
+    const int64_t items = (int64_t)kv->streams * kv->kvh * ((rows + 4 * nt - 1) / (4 * nt));
+    const auto &n = kv->clusters[nt - 1];
+    return nt == 1 ? launch<D, 1, 2>(kv, a, n, items, st) : launch<D, 2, 1>(kv, a, n, items, st);
+}
+}  // namespace
+
+int kv4_attend_setup(qora_kv4 *kv) { return kv->hd == 64 ? setup<64>(kv) : setup<128>(kv); }
 
 }  // namespace qora
 
@@ -677,10 +701,5 @@ extern "C" int qora_kv4_attend(qora_kv4 *kv, int32_t layer, const float *q, cons
     a.scale_log2 = 1.4426950408889634f / sqrtf((float)kv->hd);
     const int64_t rows = kv->heads / kv->kvh * (int64_t)max_count;  // of a stream's kv head
     if (rows > 64) return kv4_launch_prompt(kv, layer, q, offsets, tokens, rows, out, as_stream(stream));
-    const bool one = rows <= 4;
-    const int64_t items = (int64_t)kv->streams * kv->kvh * ((rows + (one ? 3 : 7)) / (one ? 4 : 8));
-    const auto &n = kv->clusters[one ? 0 : 1];
-    cudaStream_t st = as_stream(stream);
-    if (kv->hd == 64) return one ? launch<64, 1, 2>(kv, a, n, items, st) : launch<64, 2, 4>(kv, a, n, items, st);
-    return one ? launch<128, 1, 2>(kv, a, n, items, st) : launch<128, 2, 4>(kv, a, n, items, st);
+    return kv->hd == 64 ? launch_rows<64>(kv, a, rows, as_stream(stream)) : launch_rows<128>(kv, a, rows, as_stream(stream));
 }
