@@ -29,8 +29,9 @@ namespace {
 // out the free pages in it; tokens are spread over all threads, which look
 // their stream up in the scanned offsets.
 constexpr int kResThreads = 1024;
-constexpr int kResCluster = 8;
-constexpr int kResChunk = 256;  // table entries that a warp marks at a time
+constexpr int kResCluster = 16;  // (not a portable size; what bounds the large case is marking, a block's share of it)
+constexpr int kResChunk = 128;  // table entries of one stream that a warp marks at a time,
+constexpr int kResDeep = 6;     // and how many such pieces: 24 loads of a lane in flight
 
 struct ReserveArgs {
     const int *counts, *len;
@@ -38,9 +39,12 @@ struct ReserveArgs {
     int streams, max_pos, page_shift, pages_per_stream, pool_pages, max_tokens;
 };
 
+constexpr int kResList = 2048;  // free pages that are listed at a time
+
 struct ReserveShared {
     int64_t wsum[32];
     int bad, free_pages;
+    int list[kResList];
 };
 
 __device__ __forceinline__ int64_t block_scan_excl(int64_t v, int64_t *wsum, int64_t &total) {
@@ -126,23 +130,26 @@ __global__ void __launch_bounds__(kResThreads) k_kv4_reserve(const ReserveArgs a
     __syncthreads();
     // ---- mark the pages in use
     const int chunks = (a.pages_per_stream + kResChunk - 1) / kResChunk;
-    for (int p = rank * (kResThreads / 32) + warp; p < a.streams * chunks; p += nr * (kResThreads / 32)) {
-        const int b = p / chunks, j0 = (p - b * chunks) * kResChunk;
-        const int keep = (len[b] + P - 1) >> a.page_shift;
-        if (j0 >= keep) continue;
-        const int *t = a.table + (int64_t)b * a.pages_per_stream;
-        int pg[kResChunk / 32];
+    const int warps = nr * (kResThreads / 32);
+    for (int p0 = rank * (kResThreads / 32) + warp; p0 < a.streams * chunks; p0 += kResDeep * warps) {
+        int pg[kResDeep][kResChunk / 32], left[kResDeep];  // entries; how many from the lane's first on
 #pragma unroll
-        for (int i = 0; i < kResChunk / 32; i++) {
-            const int j = j0 + i * 32 + lane;
-            pg[i] = j < keep ? __ldcg(t + j) : -2;
+        for (int d = 0; d < kResDeep; d++) {
+            const int p = p0 + d * warps;
+            const int b = p / chunks, j0 = (p - b * chunks) * kResChunk + lane;
+            left[d] = p < a.streams * chunks ? ((len[b] + P - 1) >> a.page_shift) - j0 : 0;
+            const int *t = a.table + (int64_t)b * a.pages_per_stream;
+#pragma unroll
+            for (int i = 0; i < kResChunk / 32; i++) pg[d][i] = i * 32 < left[d] ? __ldcg(t + j0 + i * 32) : 0;
         }
 #pragma unroll
-        for (int i = 0; i < kResChunk / 32; i++) {
-            if (pg[i] == -2 && j0 + i * 32 + lane >= keep) continue;
-            if ((unsigned)pg[i] >= (unsigned)a.pool_pages) sh.bad = kDevRange;
-            else atomicOr(&bits[pg[i] >> 5], 1u << (pg[i] & 31));
-        }
+        for (int d = 0; d < kResDeep; d++)
+#pragma unroll
+            for (int i = 0; i < kResChunk / 32; i++) {
+                if (i * 32 >= left[d]) break;
+                if ((unsigned)pg[d][i] >= (unsigned)a.pool_pages) sh.bad = kDevRange;
+                else atomicOr(&bits[pg[d][i] >> 5], 1u << (pg[d][i] & 31));
+            }
     }
     cl.sync();
     // ---- this block's share of the pool: words [wa, wb)
@@ -151,7 +158,9 @@ __global__ void __launch_bounds__(kResThreads) k_kv4_reserve(const ReserveArgs a
     int mine = 0;
     for (int w = wa + tid; w < wb; w += kResThreads) {
         unsigned f = 0u;
-        for (int r = 0; r < nr; r++) f |= cl.map_shared_rank(bits, r)[w];
+#pragma unroll
+        for (int r = 0; r < kResCluster; r++)
+            if (r < nr) f |= cl.map_shared_rank(bits, r)[w];
         f = ~f;
         if (w == words - 1 && (a.pool_pages & 31)) f &= (1u << (a.pool_pages & 31)) - 1u;
         bits[w] = f;  // from here on: free pages (no other block reads these words)
@@ -162,11 +171,18 @@ __global__ void __launch_bounds__(kResThreads) k_kv4_reserve(const ReserveArgs a
     if (tid == 0) sh.free_pages = (int)total;
     cl.sync();
     int ordinal = 0, free_total = 0, bad = 0;
-    for (int r = 0; r < nr; r++) {
-        const ReserveShared *o = cl.map_shared_rank(&sh, r);
+    int theirs[kResCluster], wrong[kResCluster];  // (all reads in flight together)
+#pragma unroll
+    for (int r = 0; r < kResCluster; r++) {
+        const ReserveShared *o = cl.map_shared_rank(&sh, r < nr ? r : 0);
+        theirs[r] = o->free_pages, wrong[r] = o->bad;
+    }
+#pragma unroll
+    for (int r = 0; r < kResCluster; r++) {
+        if (r >= nr) break;
         if (r == rank) ordinal = free_total;
-        free_total += o->free_pages;
-        bad |= o->bad;
+        free_total += theirs[r];
+        bad |= wrong[r];
     }
     const int all = nr * kResThreads, me = rank * kResThreads + tid;
     const int why = bad ? kDevRange : tokens > a.max_tokens ? kDevRange : need > free_total ? kDevPool : 0;
@@ -181,20 +197,27 @@ __global__ void __launch_bounds__(kResThreads) k_kv4_reserve(const ReserveArgs a
         return;
     }
     for (int b = me; b <= a.streams; b += all) a.offsets[b] = b < a.streams ? off[b] : (int)tokens;
-    // ---- the i-th free page goes to the i-th new (stream, page)
+    // ---- the i-th free page goes to the i-th new (stream, page): threads list the
+    // pages of their words, then share the list out
     for (int w0 = wa; w0 < wb && ordinal < need; w0 += kResThreads) {
         const int w = w0 + tid;
-        unsigned f = w < wb ? bits[w] : 0u;
-        int at = ordinal + (int)block_scan_excl(__popc(f), sh.wsum, total);
-        ordinal += (int)total;
-        if (f && at < need) {
-            int b = last_at_most(first, a.streams, at);
-            for (; f && at < need; at++, f &= f - 1) {
-                while (b + 1 < a.streams && first[b + 1] <= at) b++;
+        const unsigned f = w < wb ? bits[w] : 0u;
+        const int at = (int)block_scan_excl(__popc(f), sh.wsum, total);
+        const int count = min((int)total, need - ordinal);
+        for (int l0 = 0; l0 < count; l0 += kResList) {
+            int i = at - l0;
+            for (unsigned m = f; m && i < kResList; m &= m - 1, i++)
+                if (i >= 0) sh.list[i] = w * 32 + __ffs(m) - 1;
+            __syncthreads();
+            for (int j = tid; j < min(count - l0, kResList); j += kResThreads) {
+                const int o = ordinal + l0 + j;
+                const int b = last_at_most(first, a.streams, o);
                 const int keep = (len[b] + P - 1) >> a.page_shift;
-                __stcg(a.table + (int64_t)b * a.pages_per_stream + keep + (at - first[b]), w * 32 + __ffs(f) - 1);
+                __stcg(a.table + (int64_t)b * a.pages_per_stream + keep + (o - first[b]), sh.list[j]);
             }
+            __syncthreads();
         }
+        ordinal += (int)total;
     }
     cl.sync();
     // ---- the tokens' slots and positions
@@ -227,6 +250,16 @@ __global__ void k_kv4_advance(int *len, const int *counts, int streams, int max_
 // has dimensions 4l .. 4l + 3 of each half, so the rotation's pairs (i, i + D/2)
 // and the four codes of a stored halfword lie in one lane, loads and stores are
 // 16 bytes, and a scale group is eight lanes.
+__device__ __forceinline__ float inv_sqrt(float x) { return __fdiv_rn(1.0f, __fsqrt_rn(x)); }
+__device__ __forceinline__ double inv_sqrt(double x) { return rsqrt(x); }
+
+// The larger of two magnitudes, NaN when one is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
 template <int D>
 struct Angles {
     float4 c, s;
@@ -268,7 +301,7 @@ struct HeadVec {
             for (int e = 0; e < 4; e++) ss += (T)x[h][e] * (T)x[h][e];
 #pragma unroll
         for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        const T inv = (T)1 / sqrt(ss / (T)D + (T)1e-6);
+        const T inv = inv_sqrt(ss * (T)(1.0 / D) + (T)1e-6);
         const uint2 g0 = __ldg(reinterpret_cast<const uint2 *>(gamma) + l);
         const uint2 g1 = __ldg(reinterpret_cast<const uint2 *>(gamma + D / 2) + l);
         const __half2 ga[4] = {*reinterpret_cast<const __half2 *>(&g0.x), *reinterpret_cast<const __half2 *>(&g0.y),
@@ -290,46 +323,78 @@ struct HeadVec {
     template <bool V>
     __device__ __forceinline__ void store4(uint8_t *unit, int r, int l, bool on) const {
         using U = Kv4Unit<D>;
+        float s[2];
+        __half sh[2];
+        bool plain = true;  // scales that are normal f16 numbers: no code can pass 7
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            unsigned top = 0;  // largest magnitude's bits; infinities and NaN lie above all
+            float amax = max_nan(max_nan(fabsf(x[h][0]), fabsf(x[h][1])), max_nan(fabsf(x[h][2]), fabsf(x[h][3])));
 #pragma unroll
-            for (int e = 0; e < 4; e++) top = max(top, __float_as_uint(x[h][e]) & 0x7fffffffu);
-#pragma unroll
-            for (int o = 1; o < 8; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-            const bool fin = top < 0x7f800000u;
+            for (int o = 1; o < 8; o <<= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
             // amax / 7 correctly rounded: one step from a quotient within an ulp.
             // Rounding that to f16 equals rounding amax / 7 once: no f32 neighbour
             // of 7m has a quotient that rounds to the 12-bit m.
-            const float amax = __uint_as_float(top), seventh = 0.14285715f;
+            const float seventh = 0.14285715f;
             float d = __fmul_rn(amax, seventh);
             d = fmaf(fmaf(-7.0f, d, amax), seventh, d);
-            const __half sh = fin ? __float2half_rn(fminf(d, 65504.0f)) : __ushort_as_half((unsigned short)0x7e00);
-            const float s = __half2float(sh);
-            const bool live = fin && s > 0.0f;
-            float inv;
-            asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(live ? s : 1.0f));
-            unsigned nib = 0;
+            sh[h] = __float2half_rn(fminf(d, 65504.0f));
+            if (!(amax < INFINITY)) sh[h] = __ushort_as_half((unsigned short)0x7e00);
+            s[h] = __half2float(sh[h]);
+            plain = plain && s[h] >= 0x1p-14f && s[h] < 65504.0f;
+        }
+        unsigned nib[2];
+        bool sure = true;
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                // nearest integer to x / s: rint of the approximate quotient is off
-                // by one at most; x - q s is exact in f32 and decides
-                const float v = live ? x[h][e] : 0.0f;
-                float q = rintf(fminf(fmaxf(v * inv, -8.0f), 8.0f));
-                const float rest = 2.0f * fmaf(-q, s, v);
-                const bool odd = (int)q & 1;
-                if (rest > s || (rest == s && odd)) q += 1.0f;
-                if (rest < -s || (rest == -s && odd)) q -= 1.0f;
-                q = live ? fminf(fmaxf(q, -7.0f), 7.0f) : 0.0f;
-                nib |= (unsigned)((int)q + 8) << (4 * e);
+        for (int h = 0; h < 2; h++) {
+            // Nearest integer to x / s by the approximate quotient: adding 1.5 2^23
+            // leaves it in the low bits.  x - q s is exact in f32; where it is under
+            // s / 2 the integer is the nearest.
+            float inv;
+            asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s[h]));
+            unsigned sum = 0;
+#pragma unroll
+            for (int e = 3; e >= 0; e--) {
+                const float t = fmaf(x[h][e], inv, 12582912.0f);
+                const float rest = fmaf(12582912.0f - t, s[h], x[h][e]);
+                sure = sure && fabsf(rest) < 0.5f * s[h];
+                sum = sum * 16u + __float_as_uint(t);
             }
-            if (!on) continue;
+            nib[h] = sum - (0x4b400000u - 8u) * 0x1111u;  // each digit: code + 8
+        }
+        if (!__all_sync(0xffffffffu, plain && sure)) {  // ties, zeros, infinities, scales at f16's ends
+#pragma unroll
+            for (int h = 0; h < 2; h++) nib[h] = codes_exactly(x[h], s[h]);
+        }
+        if (!on) return;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
             const int dim = h * (D / 2) + 4 * l;
             *reinterpret_cast<uint16_t *>(unit + (V ? U::v_half(r, dim) : U::k_word(r, dim) + ((dim & 4) >> 1))) =
-                (uint16_t)nib;
+                (uint16_t)nib[h];
             if ((l & 7) == 0)
-                *reinterpret_cast<__half *>(unit + (V ? U::v_scale(r, dim >> 5) : U::k_scale(r, dim >> 5))) = sh;
+                *reinterpret_cast<__half *>(unit + (V ? U::v_scale(r, dim >> 5) : U::k_scale(r, dim >> 5))) = sh[h];
         }
+    }
+
+    // The same codes for any scale (0 and NaN: codes 0), ties to even, in [-7, 7].
+    static __device__ __noinline__ unsigned codes_exactly(const float (&v4)[4], float s) {
+        const bool live = s > 0.0f;
+        float inv;
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(live ? s : 1.0f));
+        unsigned nib = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            // rint of the approximate quotient is off by one at most; the rest decides
+            const float v = live ? v4[e] : 0.0f;
+            float q = rintf(fminf(fmaxf(v * inv, -8.0f), 8.0f));
+            const float rest = 2.0f * fmaf(-q, s, v);
+            const bool odd = (int)q & 1;
+            if (rest > s || (rest == s && odd)) q += 1.0f;
+            if (rest < -s || (rest == -s && odd)) q -= 1.0f;
+            q = live ? fminf(fmaxf(q, -7.0f), 7.0f) : 0.0f;
+            nib |= (unsigned)((int)q + 8) << (4 * e);
+        }
+        return nib;
     }
 
     template <bool V>
@@ -362,8 +427,7 @@ struct RowArgs {
 };
 
 // Whether row i is to be handled; its unit and place in it.
-__device__ __forceinline__ bool row_place(const RowArgs &a, int i, int &page, int &unit, int &r) {
-    const int slot = a.slots[i];
+__device__ __forceinline__ bool row_place(const RowArgs &a, int slot, int &page, int &unit, int &r) {
     if (slot == -1) return false;  // a row behind the last token
     if (slot < 0 || (slot >> a.L.page_shift) >= a.L.pool_pages) {
         raise_error(a.err, kDevRange);
@@ -385,21 +449,21 @@ __global__ void __launch_bounds__(kRowWarps * 32) k_kv4_append(const RowArgs a) 
     griddep_launch_dependents();
     griddep_wait();
     const int lane = threadIdx.x & 31, l = lane % (D / 8), sub = lane / (D / 8);
-    const int qt = (a.heads + HW - 1) / HW, kt = (a.L.kvh + HW - 1) / HW, per = qt + 2 * kt;
-    const int64_t task = (int64_t)blockIdx.x * kRowWarps + (threadIdx.x >> 5);
-    const int i = (int)(task / per);
-    int w = (int)(task - (int64_t)i * per);
+    const int qt = (a.heads + HW - 1) / HW, kt = (a.L.kvh + HW - 1) / HW;
+    const unsigned per = qt + 2 * kt;
+    const unsigned task = blockIdx.x * kRowWarps + (threadIdx.x >> 5);  // (below 2^31: row_blocks)
+    const int i = (int)(task / per), w = (int)(task - i * per);
     if (i >= a.rows) return;
     const int kind = w < qt ? 0 : w < qt + kt ? 1 : 2;
     const int n = kind == 0 ? a.heads : a.L.kvh;
     const int h = (w - (kind == 0 ? 0 : kind == 1 ? qt : qt + kt)) * HW + sub;  // this lane's head of its kind
     const bool on = h < n;
     const int first = kind == 0 ? 0 : kind == 1 ? a.heads : a.heads + a.L.kvh;
+    const int slot = a.slots[i], pos = a.positions[i];
     HeadVec<D> x;
     x.load(a.qkv + ((int64_t)i * (a.heads + 2 * a.L.kvh) + first + (on ? h : 0)) * D, l);
     int page, unit, r;
-    if (!row_place(a, i, page, unit, r)) return;
-    const int pos = a.positions[i];
+    if (!row_place(a, slot, page, unit, r)) return;
     if (pos < 0 || pos >= a.rope_max) {
         raise_error(a.err, kDevRange);
         return;
@@ -426,12 +490,12 @@ __global__ void __launch_bounds__(kRowWarps * 32) k_kv4_rows(const RowArgs a) {
     griddep_launch_dependents();
     griddep_wait();
     const int lane = threadIdx.x & 31, l = lane % (D / 8), sub = lane / (D / 8);
-    const int per = (a.L.kvh + HW - 1) / HW;
-    const int64_t task = (int64_t)blockIdx.x * kRowWarps + (threadIdx.x >> 5);
-    const int i = (int)(task / per), h = (int)(task - (int64_t)i * per) * HW + sub;
+    const unsigned per = (a.L.kvh + HW - 1) / HW;
+    const unsigned task = blockIdx.x * kRowWarps + (threadIdx.x >> 5);
+    const int i = (int)(task / per), h = (int)(task - i * per) * HW + sub;
     if (i >= a.rows) return;
     int page, unit, r;
-    if (!row_place(a, i, page, unit, r)) return;
+    if (!row_place(a, a.slots[i], page, unit, r)) return;
     const bool on = h < a.L.kvh;
     uint8_t *u = a.L.unit(page, on ? h : 0, unit, D);
     const int64_t at = ((int64_t)i * a.L.kvh + (on ? h : 0)) * D;
@@ -453,7 +517,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) k_kv4_rows(const RowArgs a) {
 
 int row_blocks(const char *who, int64_t warps, dim3 &grid) {
     const int64_t blocks = (warps + kRowWarps - 1) / kRowWarps;
-    if (blocks > 0x7fffffff) return set_error(QORA_ERR_UNSUPPORTED, "%s: too many rows", who);
+    if (blocks > 0x7fffffff / kRowWarps) return set_error(QORA_ERR_UNSUPPORTED, "%s: too many rows", who);
     grid = dim3((unsigned)blocks);
     return QORA_OK;
 }
@@ -599,6 +663,7 @@ int qora_kv4_reserve(qora_kv4 *kv, const int32_t *counts, int32_t max_tokens, in
     // takes in a few rounds
     const bool wide = (int64_t)kv->streams * kv->pages_per_stream + max_tokens > 16384;
     const unsigned nr = wide ? kResCluster : 1;
+    if (wide) QORA_CUDA(cudaFuncSetAttribute(k_kv4_reserve, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     return launch_ex(k_kv4_reserve, dim3(1, nr), dim3(kResThreads), smem, as_stream(stream), nr, a);
 }
 

@@ -36,7 +36,7 @@ constexpr int kMaxCluster = 8;
 // by values next to each other.
 constexpr int kBins = 2048;
 constexpr int kCand = 2048;          // candidates that one sort takes
-constexpr int kSliceMax = 40960;     // logits of a slice in shared memory
+constexpr int kSliceMax = 40960;     // logits of a slice in shared memory (a multiple of 4)
 
 struct ProbsArgs {
     const float *logits;
@@ -47,7 +47,7 @@ struct ProbsArgs {
     qora_sample_params params;
 };
 
-struct ProbsSmem {
+struct alignas(16) ProbsSmem {  // (the slice behind it is read in 16-byte pieces)
     unsigned hist[kBins];
     unsigned long long cand[kCand];   // order key of x, then ~index
     double wsum[kVWarps + 1];
@@ -59,6 +59,8 @@ struct ProbsSmem {
     double sum, slice_sum;
     unsigned eq_count;
 };
+
+static_assert(sizeof(ProbsSmem) % 16 == 0 && kSliceMax % 4 == 0, "the slice is 16-byte aligned");
 
 // Order of f32 values as unsigned integers.
 __device__ __forceinline__ unsigned order_key(float x) {
@@ -118,7 +120,9 @@ __device__ __forceinline__ void select_bin(cg::cluster_group &cl, ProbsSmem *sm,
     for (int b0 = 0; b0 < bins; b0 += 32) {
         const int bin = DESC ? bins - 1 - (b0 + lane) : b0 + lane;
         unsigned c = 0;
-        for (unsigned r = 0; r < nr; r++) c += cl.map_shared_rank(sm, r)->hist[bin];
+#pragma unroll
+        for (unsigned r = 0; r < kMaxCluster; r++)  // (reads in flight together)
+            if (r < nr) c += cl.map_shared_rank(sm, r)->hist[bin];
         unsigned x = c;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -138,12 +142,18 @@ __device__ __forceinline__ void select_bin(cg::cluster_group &cl, ProbsSmem *sm,
     }
 }
 
+// VEC: rows and slices are multiples of 16 bytes.
+template <bool VEC>
 __global__ void __launch_bounds__(kVThreads) k_sample_probs(const ProbsArgs a) {
     extern __shared__ uint4 dyn[];
     ProbsSmem *sm = reinterpret_cast<ProbsSmem *>(dyn);
     float *x = reinterpret_cast<float *>(sm + 1);
     cg::cluster_group cl = cg::this_cluster();
     const unsigned rank = cl.block_rank(), nr = cl.num_blocks();
+    auto meet = [&]() {  // all blocks of the row
+        if (nr == 1) __syncthreads();
+        else cl.sync();
+    };
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int64_t row = blockIdx.x;
     const int v0 = (int)rank * a.slice, n = max(0, min(a.slice, a.V - v0));
@@ -151,32 +161,72 @@ __global__ void __launch_bounds__(kVThreads) k_sample_probs(const ProbsArgs a) {
     griddep_wait();
     const float *in = a.logits + row * a.V + v0;
     float *out = a.probs + row * a.V + v0;
-    for (int i = tid; i < n; i += kVThreads) x[i] = __ldg(in + i);
+    // f(i, value) over the slice in shared memory, sixteen bytes at a time
+    auto each = [&](auto f) {
+        if constexpr (VEC) {
+            const float4 *x4 = reinterpret_cast<const float4 *>(x);
+            for (int i = tid; i < n / 4; i += kVThreads) {
+                const float4 v = x4[i];
+                f(4 * i, v.x), f(4 * i + 1, v.y), f(4 * i + 2, v.z), f(4 * i + 3, v.w);
+            }
+        } else {
+            for (int i = tid; i < n; i += kVThreads) f(i, x[i]);
+        }
+    };
+    // eight loads of a thread in flight
+    if constexpr (VEC) {
+        const float4 *in4 = reinterpret_cast<const float4 *>(in);
+        float4 *x4 = reinterpret_cast<float4 *>(x);
+        for (int i0 = 0; i0 < n / 4; i0 += 8 * kVThreads) {
+            float4 v[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (i0 + j * kVThreads + tid < n / 4) v[j] = __ldcs(in4 + i0 + j * kVThreads + tid);
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (i0 + j * kVThreads + tid < n / 4) x4[i0 + j * kVThreads + tid] = v[j];
+        }
+    } else {
+        for (int i0 = 0; i0 < n; i0 += 8 * kVThreads) {
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (i0 + j * kVThreads + tid < n) v[j] = __ldcs(in + i0 + j * kVThreads + tid);
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (i0 + j * kVThreads + tid < n) x[i0 + j * kVThreads + tid] = v[j];
+        }
+    }
     __syncthreads();
-    // penalty: the first mention of a token applies all of them
+    // penalty: a warp per mention; a token's first mention applies all of them
     if (a.prev && a.params.repetition_penalty != 1.0f) {
         const uint32_t *prev = a.prev + row * a.n_prev;
-        for (int j = tid; j < a.n_prev; j += kVThreads) {
-            const uint32_t tok = prev[j];
+        for (int j = warp; j < a.n_prev; j += kVWarps) {
+            const uint32_t tok = __ldg(prev + j);
             if (tok >= (unsigned)a.V || (int)tok < v0 || (int)tok >= v0 + n) continue;
             bool first = true;
-            for (int i = 0; i < j && first; i++) first = prev[i] != tok;
-            if (!first) continue;
-            float y = x[tok - v0];
-            for (int i = j; i < a.n_prev; i++)
-                if (prev[i] == tok) y = y > 0.0f ? __fdiv_rn(y, a.params.repetition_penalty)
-                                                 : __fmul_rn(y, a.params.repetition_penalty);
-            x[tok - v0] = y;
+            int times = 0;
+            for (int i0 = 0; i0 < a.n_prev && first; i0 += 32) {
+                const unsigned same = __ballot_sync(0xffffffffu, i0 + lane < a.n_prev && __ldg(prev + i0 + lane) == tok);
+                first = !same || i0 + __ffs(same) - 1 >= j || times > 0;
+                times += __popc(same);
+            }
+            if (first && lane == 0) {
+                float y = x[tok - v0];
+                for (int i = 0; i < times; i++)
+                    y = y > 0.0f ? __fdiv_rn(y, a.params.repetition_penalty) : __fmul_rn(y, a.params.repetition_penalty);
+                x[tok - v0] = y;
+            }
         }
         __syncthreads();
     }
     // maximum of the row
     float mx = -INFINITY;
     bool nan = false;
-    for (int i = tid; i < n; i += kVThreads) {
-        mx = fmaxf(mx, x[i]);
-        nan = nan || x[i] != x[i];
-    }
+    each([&](int, float v) {
+        mx = fmaxf(mx, v);
+        nan = nan || v != v;
+    });
     mx = warp_max(mx);
     if (lane == 0) sm->red[warp] = mx;
     nan = __syncthreads_or(nan);
@@ -187,16 +237,16 @@ __global__ void __launch_bounds__(kVThreads) k_sample_probs(const ProbsArgs a) {
         sm->n_cand = 0;
     }
     for (int i = tid; i < kBins; i += kVThreads) sm->hist[i] = 0;
-    cl.sync();
-    if (tid == 0) {
-        float m = -INFINITY;
-        int bad = 0;
-        for (unsigned r = 0; r < nr; r++) {
-            m = fmaxf(m, cl.map_shared_rank(sm, r)->slice_max);
-            bad |= cl.map_shared_rank(sm, r)->slice_bad;
+    meet();
+    if (warp == 0) {  // a lane per block: remote reads in flight together
+        const bool there = lane < (int)nr;
+        const ProbsSmem *o = cl.map_shared_rank(sm, there ? lane : 0);
+        const float m = warp_max(there ? o->slice_max : -INFINITY);
+        const bool bad = __any_sync(0xffffffffu, there && o->slice_bad);
+        if (lane == 0) {
+            sm->mx = m;
+            sm->bad = bad || !isfinite(m);
         }
-        sm->mx = m;
-        sm->bad = bad || !isfinite(m);
     }
     __syncthreads();
     mx = sm->mx;
@@ -206,7 +256,7 @@ __global__ void __launch_bounds__(kVThreads) k_sample_probs(const ProbsArgs a) {
     if (bad) {  // NaN or +inf among the logits, or none that is finite
         if (tid == 0 && rank == 0) raise_error(a.err, kDevNaN);
         for (int i = tid; i < n; i += kVThreads) out[i] = 0.0f;
-        cl.sync();  // no block leaves while another reads its slice_max
+        meet();  // no block leaves while another reads its slice_max
         return;
     }
     if (!topk) {
@@ -219,7 +269,7 @@ __global__ void __launch_bounds__(kVThreads) k_sample_probs(const ProbsArgs a) {
         }
         s = block_sum_f64(s, sm->wsum);
         if (tid == 0) sm->slice_sum = s;
-        cl.sync();
+        meet();
         if (tid == 0) {
             double t = 0.0;
             for (unsigned r = 0; r < nr; r++) t += cl.map_shared_rank(sm, r)->slice_sum;
@@ -228,16 +278,18 @@ __global__ void __launch_bounds__(kVThreads) k_sample_probs(const ProbsArgs a) {
         __syncthreads();
         const double inv = sm->sum;
         for (int i = tid; i < n; i += kVThreads) out[i] = (float)(x[i] * inv);
-        cl.sync();
+        meet();
         return;
     }
     const unsigned k = a.params.top_k;
     auto bin_of = [&](float v) { return (int)fminf((mx - v) * 32.0f, (float)(kBins - 1)); };
-    for (int i = tid; i < n; i += kVThreads) {
-        atomicAdd(&sm->hist[bin_of(x[i])], 1u);
-        out[i] = 0.0f;
+    each([&](int, float v) { atomicAdd(&sm->hist[bin_of(v)], 1u); });
+    if constexpr (VEC) {
+        for (int i = tid; i < n / 4; i += kVThreads) reinterpret_cast<float4 *>(out)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    } else {
+        for (int i = tid; i < n; i += kVThreads) out[i] = 0.0f;
     }
-    cl.sync();
+    meet();
     if (warp == 0) select_bin<false>(cl, sm, kBins, k);
     __syncthreads();
     const int sel = sm->sel_bin;
@@ -248,10 +300,11 @@ __global__ void __launch_bounds__(kVThreads) k_sample_probs(const ProbsArgs a) {
         if (at < kCand)
             lead->cand[at] = ((unsigned long long)order_key(x[i]) << 32) | (unsigned)~(unsigned)(v0 + i);
     };
-    cl.sync();  // every block has read the histograms
+    meet();  // every block has read the histograms
     if (few) {
-        for (int i = tid; i < n; i += kVThreads)
-            if (bin_of(x[i]) <= sel) offer(i);
+        each([&](int i, float v) {
+            if (bin_of(v) <= sel) offer(i);
+        });
     } else {
         // radix selection of the k-th key, 8 bits at a time
         unsigned prefix = 0, mask = 0, need = k;
@@ -262,20 +315,20 @@ __global__ void __launch_bounds__(kVThreads) k_sample_probs(const ProbsArgs a) {
                 const unsigned key = order_key(x[i]);
                 if ((key & mask) == prefix) atomicAdd(&sm->hist[(key >> shift) & 255u], 1u);
             }
-            cl.sync();
+            meet();
             if (warp == 0) select_bin<true>(cl, sm, 256, need);
             __syncthreads();
             prefix |= sm->sel_bin << shift;
             mask |= 255u << shift;
             need -= sm->sel_below;
-            cl.sync();
+            meet();
         }
         // keys above the k-th are kept, and the first `need` equal to it in index order
         unsigned eq = 0;
         for (int i = tid; i < n; i += kVThreads) eq += order_key(x[i]) == prefix;
         eq = (unsigned)block_sum_f64((double)eq, sm->wsum);
         if (tid == 0) sm->eq_count = eq;
-        cl.sync();
+        meet();
         if (tid == 0) {
             unsigned before = 0;
             for (unsigned r = 0; r < rank; r++) before += cl.map_shared_rank(sm, r)->eq_count;
@@ -293,24 +346,35 @@ __global__ void __launch_bounds__(kVThreads) k_sample_probs(const ProbsArgs a) {
             if (i < n && (key > prefix || (same && at < need))) offer(i);
         }
     }
-    cl.sync();
+    meet();
     if (rank != 0) return;  // the rest is the leader's; it reads no other block's memory
     const unsigned found = min(sm->n_cand, (unsigned)kCand);
-    int size = 32;
-    while (size < (int)found) size <<= 1;
-    for (int i = found + tid; i < size; i += kVThreads) sm->cand[i] = 0ull;
-    __syncthreads();
-    // descending bitonic sort
-    for (int span = 2; span <= size; span <<= 1)
-        for (int step = span >> 1; step > 0; step >>= 1) {
-            for (int i = tid; i < size / 2; i += kVThreads) {
-                const int lo = (i / step) * step * 2 + (i % step), hi = lo + step;
-                const unsigned long long p = sm->cand[lo], q = sm->cand[hi];
-                const bool down = (lo & span) == 0;
-                if ((p < q) == down) sm->cand[lo] = q, sm->cand[hi] = p;
-            }
-            __syncthreads();
+    const int size = found <= 256 ? 256 : kCand;
+    if (found <= 256) {  // few: each counts those before it
+        unsigned long long mine = 0;
+        unsigned at = 0;
+        if (tid < (int)found) {
+            mine = sm->cand[tid];
+#pragma unroll 8
+            for (unsigned j = 0; j < found; j++) at += sm->cand[j] > mine;
         }
+        __syncthreads();
+        if (tid < (int)found) sm->cand[at] = mine;
+        __syncthreads();
+    } else {  // descending bitonic sort
+        for (int i = found + tid; i < size; i += kVThreads) sm->cand[i] = 0ull;
+        __syncthreads();
+        for (int span = 2; span <= size; span <<= 1)
+            for (int step = span >> 1; step > 0; step >>= 1) {
+                for (int i = tid; i < size / 2; i += kVThreads) {
+                    const int lo = (i / step) * step * 2 + (i % step), hi = lo + step;
+                    const unsigned long long p = sm->cand[lo], q = sm->cand[hi];
+                    const bool down = (lo & span) == 0;
+                    if ((p < q) == down) sm->cand[lo] = q, sm->cand[hi] = p;
+                }
+                __syncthreads();
+            }
+    }
     // k <= kMaxSurvivors = 2 kVThreads: thread i has ranks 2i and 2i + 1
     double e[2];
 #pragma unroll
@@ -353,17 +417,24 @@ struct VerifyArgs {
 };
 
 struct VerifySmem {
-    double wsum[kVWarps + 1];
+    double wsum[kVWarps], psum[kVWarps];
     double sum;
+    int wlast[kVWarps], plast[kVWarps];
     int last;           // highest index with a positive weight, -1
     int accepted;
     int count;
 };
 
+// VEC: rows and slices are multiples of 16 bytes.
+template <bool VEC>
 __global__ void __launch_bounds__(kVThreads) k_verify_drafts(const VerifyArgs a) {
     __shared__ VerifySmem sm;
     cg::cluster_group cl = cg::this_cluster();
     const unsigned rank = cl.block_rank(), nr = cl.num_blocks();
+    auto meet = [&]() {  // all blocks of the stream
+        if (nr == 1) __syncthreads();
+        else cl.sync();
+    };
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int64_t b = blockIdx.x;
     griddep_launch_dependents();
@@ -409,81 +480,154 @@ __global__ void __launch_bounds__(kVThreads) k_verify_drafts(const VerifyArgs a)
     const float *p = target + (int64_t)acc * a.V;
     const float *q = rejected && draft ? draft + (int64_t)acc * a.V : nullptr;
     int without = rejected && !draft ? drafts[acc] : -1;
-    // the block's slice, a contiguous run per warp
+    // The block's slice, a contiguous run per warp.  Weights of 32 (VEC: 128)
+    // neighbours at a time, eight loads of a lane in flight.
+    constexpr int kStep = VEC ? 128 : 32;
     const int v0 = (int)rank * a.slice, n = max(0, min(a.slice, a.V - v0));
-    const int run = ((n + kVWarps - 1) / kVWarps + 31) / 32 * 32;
-    const int r0 = v0 + min(n, warp * run), r1 = v0 + min(n, (warp + 1) * run);
+    const int run = ((n + kVWarps - 1) / kVWarps + kStep - 1) / kStep * kStep;
+    auto weigh = [&](float pv, float qv, int i) {
+        double w = (double)pv;
+        if (q) w -= (double)qv;
+        return w > 0.0 && i != without ? w : 0.0;
+    };
+    // sum of the weights in [i0, i1) over the lanes; `mine`: the lane's highest index with one
+    auto sum_of = [&](int i0, int i1, int &mine) {
+        double s = 0.0;
+        if constexpr (VEC) {
+            for (int i = i0 + 4 * lane; i < i1; i += 4 * kStep) {
+                float4 pv[4], qv[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const bool in = i + j * kStep < i1;
+                    pv[j] = in ? __ldg(reinterpret_cast<const float4 *>(p + i + j * kStep)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    qv[j] = in && q ? __ldg(reinterpret_cast<const float4 *>(q + i + j * kStep)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const float pe[4] = {pv[j].x, pv[j].y, pv[j].z, pv[j].w}, qe[4] = {qv[j].x, qv[j].y, qv[j].z, qv[j].w};
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const double w = weigh(pe[e], qe[e], i + j * kStep + e);
+                        if (w > 0.0) s += w, mine = i + j * kStep + e;
+                    }
+                }
+            }
+        } else {
+            for (int i = i0 + lane; i < i1; i += 4 * kStep) {
+                float pv[4], qv[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const bool in = i + j * kStep < i1;
+                    pv[j] = in ? __ldg(p + i + j * kStep) : 0.0f;
+                    qv[j] = in && q ? __ldg(q + i + j * kStep) : 0.0f;
+                }
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const double w = weigh(pv[j], qv[j], i + j * kStep);
+                    if (w > 0.0) s += w, mine = i + j * kStep;
+                }
+            }
+        }
+        return warp_sum_f64(s);
+    };
     double base = 0.0, total = 0.0;
     int last = -1;
     for (int pass = 0; pass < 2; pass++) {
-        double s = 0.0;
         int mine = -1;
-        for (int i = r0 + lane; i < r1; i += 32) {
-            double w = (double)__ldg(p + i);
-            if (q) w -= (double)__ldg(q + i);
-            if (w > 0.0 && i != without) s += w, mine = i;
-        }
-        s = warp_sum_f64(s);
+        const double s = sum_of(v0 + min(n, warp * run), v0 + min(n, (warp + 1) * run), mine);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, o));
-        if (tid == 0) sm.last = -1;
-        __syncthreads();
         if (lane == 0) {
             sm.wsum[warp] = s;
-            atomicMax(&sm.last, mine);
+            sm.wlast[warp] = mine;
         }
         __syncthreads();
         if (tid == 0) {
             double t = 0.0;
-            for (int w = 0; w < kVWarps; w++) t += sm.wsum[w];
+            int l = -1;
+            for (int w = 0; w < kVWarps; w++) t += sm.wsum[w], l = max(l, sm.wlast[w]);
             sm.sum = t;
+            sm.last = l;
         }
-        cl.sync();
+        meet();
         base = total = 0.0;
         last = -1;
-        for (unsigned r = 0; r < nr; r++) {
-            const VerifySmem *o = cl.map_shared_rank(&sm, r);
+        double sums[kMaxCluster];
+        int lasts[kMaxCluster];
+#pragma unroll
+        for (unsigned r = 0; r < kMaxCluster; r++) {  // (reads in flight together)
+            const VerifySmem *o = nr == 1 ? &sm : cl.map_shared_rank(&sm, r < nr ? r : 0);
+            sums[r] = r < nr ? o->sum : 0.0;
+            lasts[r] = r < nr ? o->last : -1;
+        }
+#pragma unroll
+        for (unsigned r = 0; r < kMaxCluster; r++) {
             if (r == rank) base = total;
-            total += o->sum;
-            last = max(last, o->last);
+            total += sums[r];
+            last = max(last, lasts[r]);
         }
         if (total > 0.0 || !rejected || pass) break;
         q = nullptr;  // nothing is left of the difference: draw from the target
         without = -1;
-        cl.sync();
+        meet();
     }
     // The first index whose cumulative sum passes goal.  Warp w of a block has
     // [base + pre[w], base + pre[w + 1]) of the line of sums, base and pre the
-    // same numbers for neighbours, so one warp of the cluster has the goal.
+    // same numbers for neighbours, so one warp's run in the cluster has the goal.
+    // The block of that run searches it together: each warp sums a piece, the
+    // piece that has the goal is scanned.
     const double goal = fmax((double)u[a.K] * total, 0.0);
-    double pre = 0.0;
-    for (int w = 0; w < warp; w++) pre += sm.wsum[w];
-    const double lo = base + pre, hi = base + (pre + sm.wsum[warp]);
-    if (lo <= goal && goal < hi) {
-        double at = lo;
-        int token = -1, highest = -1;
-        for (int i0 = r0; i0 < r1 && token < 0; i0 += 32) {
-            const int i = i0 + lane;
-            double w = 0.0;
-            if (i < r1) {
-                w = (double)__ldg(p + i);
-                if (q) w -= (double)__ldg(q + i);
-                if (!(w > 0.0) || i == without) w = 0.0;
+    if (base <= goal && goal < base + sm.sum) {
+        double lo = base, hi = base;
+        int at = 0;
+        {
+            double pre = 0.0;
+            for (int w = 0; w < kVWarps; w++) {
+                const double next = pre + sm.wsum[w];
+                if (base + pre <= goal && goal < base + next) lo = base + pre, hi = base + next, at = w;
+                pre = next;
             }
-            double x = w;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const double y = __shfl_up_sync(0xffffffffu, x, o);
-                if (lane >= o) x += y;
-            }
-            const unsigned some = __ballot_sync(0xffffffffu, w > 0.0);
-            const unsigned hit = __ballot_sync(0xffffffffu, w > 0.0 && at + x > goal);
-            if (some) highest = i0 + 31 - __clz(some);
-            if (hit) token = i0 + __ffs(hit) - 1;
-            at += __shfl_sync(0xffffffffu, x, 31);
         }
-        // the run's own sum may round below its share's end: then its last token
-        if (lane == 0) a.tokens[b * (a.K + 1) + acc] = token >= 0 ? token : highest;
+        const int r0 = v0 + min(n, at * run), r1 = v0 + min(n, (at + 1) * run);
+        const int piece = ((r1 - r0 + kVWarps - 1) / kVWarps + kStep - 1) / kStep * kStep;
+        const int p0 = min(r1, r0 + warp * piece), p1 = min(r1, r0 + (warp + 1) * piece);
+        int mine = -1;
+        const double s = sum_of(p0, p1, mine);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, o));
+        if (lane == 0) {
+            sm.psum[warp] = s;
+            sm.plast[warp] = mine;
+        }
+        __syncthreads();
+        // (rounding apart the pieces' sums end at hi: the last piece with a weight has what is left)
+        double pre = lo;
+        int who = -1;
+        double from = lo;
+        for (int w = 0; w < kVWarps; w++) {
+            if (sm.plast[w] >= 0 && (who < 0 || pre <= goal)) who = w, from = pre;
+            pre += sm.psum[w];
+        }
+        if (warp == who) {
+            double sum = from;
+            int token = -1;
+            for (int i0 = p0; i0 < p1 && token < 0; i0 += 32) {
+                const int i = i0 + lane;
+                const double w = i < p1 ? weigh(__ldg(p + i), q ? __ldg(q + i) : 0.0f, i) : 0.0;
+                double x = w;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const double y = __shfl_up_sync(0xffffffffu, x, o);
+                    if (lane >= o) x += y;
+                }
+                const unsigned hit = __ballot_sync(0xffffffffu, w > 0.0 && sum + x > goal);
+                if (hit) token = i0 + __ffs(hit) - 1;
+                sum += __shfl_sync(0xffffffffu, x, 31);
+            }
+            // a scan that rounds below its share's end has the piece's last token
+            if (lane == 0) a.tokens[b * (a.K + 1) + acc] = token >= 0 ? token : sm.plast[warp];
+        }
+        (void)hi;
     }
     if (rank == 0) {
         for (int j = tid; j <= a.K; j += kVThreads)
@@ -493,7 +637,7 @@ __global__ void __launch_bounds__(kVThreads) k_verify_drafts(const VerifyArgs a)
             if (!(goal < total)) a.tokens[b * (a.K + 1) + acc] = max(last, 0);  // u >= 1, or no weight at all
         }
     }
-    cl.sync();  // no block leaves while another reads its sums
+    meet();  // no block leaves while another reads its sums
 }
 
 // Blocks of one row's cluster: a slice per block of at most `most`, at least 1.
@@ -525,6 +669,7 @@ int qora_sample_probs(qora_ctx *ctx, const float *logits, int32_t B, int32_t V, 
     DeviceGuard dg;
     QORA_TRY(dg.set(ctx->device));
     const int nr = cluster_for(V, 20480);
+    const bool vec = V % 4 == 0 && !((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(probs)) & 15);
     ProbsArgs a;
     a.logits = logits;
     a.prev = n_prev ? prev : nullptr;
@@ -532,12 +677,13 @@ int qora_sample_probs(qora_ctx *ctx, const float *logits, int32_t B, int32_t V, 
     a.err = ctx->err.as<int>();
     a.V = V;
     a.n_prev = n_prev;
-    a.slice = (V + nr - 1) / nr;
+    a.slice = ((V + nr - 1) / nr + 3) / 4 * 4;
     a.params = *params;
     const size_t smem = sizeof(ProbsSmem) + (size_t)a.slice * 4;
-    QORA_CUDA(cudaFuncSetAttribute(k_sample_probs, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    auto kern = vec ? k_sample_probs<true> : k_sample_probs<false>;
+    QORA_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                    (int)(sizeof(ProbsSmem) + kSliceMax * 4)));
-    return launch_ex(k_sample_probs, dim3(B, nr), dim3(kVThreads), smem, as_stream(stream), (unsigned)nr, a);
+    return launch_ex(kern, dim3(B, nr), dim3(kVThreads), smem, as_stream(stream), (unsigned)nr, a);
 }
 
 int qora_verify_drafts(qora_ctx *ctx, const int32_t *drafts, const float *draft_probs, const float *target_probs,
@@ -559,8 +705,10 @@ int qora_verify_drafts(qora_ctx *ctx, const int32_t *drafts, const float *draft_
     a.err = ctx->err.as<int>();
     a.K = K;
     a.V = V;
-    a.slice = (int)(((int64_t)V + nr - 1) / nr);
-    return launch_ex(k_verify_drafts, dim3(B, nr), dim3(kVThreads), 0, as_stream(stream), (unsigned)nr, a);
+    a.slice = (int)((((int64_t)V + nr - 1) / nr + 3) / 4 * 4);
+    const bool vec = V % 4 == 0 && !((reinterpret_cast<uintptr_t>(target_probs) | reinterpret_cast<uintptr_t>(draft_probs)) & 15);
+    auto kern = vec ? k_verify_drafts<true> : k_verify_drafts<false>;
+    return launch_ex(kern, dim3(B, nr), dim3(kVThreads), 0, as_stream(stream), (unsigned)nr, a);
 }
 
 }  // extern "C"
