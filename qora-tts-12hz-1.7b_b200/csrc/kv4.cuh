@@ -14,10 +14,12 @@
 // of a group in one 16-byte load and the scales of its positions in one of 8:
 //   K: [c][g][t][i 0..3] words; nibble j of a word is dimension 32c + 8t + j of
 //      position g + 8i;
-//   V: [c][g][t][h 0..3] words of two halfwords e; nibble j of a halfword is
+//   V: [c][t][g ^ 2t][h 0..3] words of two halfwords e; nibble j of a halfword is
 //      dimension 32c + 4g + j of position 8h + 2t + e (a word holds two
 //      neighbouring positions, so one mask gives the pair that a matrix fragment
-//      register needs);
+//      register needs).  A position's halfwords of a group lie in 128 bytes, which
+//      halves the sectors that an append writes against [g][t], and the exclusive
+//      or keeps a quarter-warp's 16-byte reads on distinct banks;
 //   scales: [c][g][i] f16 of position g + 8i.
 // A page holds page_pos positions of every layer and kv head, in the order
 // [layer][kv head][unit].  Logical page j of stream b is physical page
@@ -84,8 +86,10 @@ struct Kv4Unit {
         return kK + (((dim >> 5) * 8 + (r & 7)) * 4 + ((dim & 31) >> 3)) * 16 + (r >> 3) * 4;
     }
     __host__ __device__ static __forceinline__ int v_half(int r, int dim) {
-        return kV + (((dim >> 5) * 8 + ((dim & 31) >> 2)) * 4 + ((r & 7) >> 1)) * 16 + (r >> 3) * 4 + (r & 1) * 2;
+        return kV + (dim >> 5) * 512 + v_chunk((dim & 31) >> 2, (r & 7) >> 1) + (r >> 3) * 4 + (r & 1) * 2;
     }
+    // where lane (g, t)'s 16 bytes of a group's V codes are
+    __host__ __device__ static __forceinline__ int v_chunk(int g, int t) { return (t * 8 + (g ^ (2 * t))) * 16; }
     __host__ __device__ static __forceinline__ int k_scale(int r, int c) { return kKs + ((c * 8 + (r & 7)) * 4 + (r >> 3)) * 2; }
     __host__ __device__ static __forceinline__ int v_scale(int r, int c) { return kVs + ((c * 8 + (r & 7)) * 4 + (r >> 3)) * 2; }
 };

@@ -479,7 +479,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_attend(const AttendArgs a) 
             }
 #pragma unroll
             for (int c = 0; c < C; c++) {
-                const uint4 vw = *reinterpret_cast<const uint4 *>(unit + U::kV + c * 512 + lane * 16);
+                const uint4 vw = *reinterpret_cast<const uint4 *>(unit + U::kV + c * 512 + U::v_chunk(g, t));
                 uint32_t x[4][4];
                 codes(vw.x, magic, x[0]);
                 codes(vw.y, magic, x[1]);

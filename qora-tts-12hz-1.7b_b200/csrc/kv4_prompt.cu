@@ -366,7 +366,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const PromptArgs a) 
                 const int pos = it * kKeys + (combo / C) * kKv4Unit;
                 const uint8_t *u = a.L.unit(pg, h, (pos >> 5) & ((1 << (a.L.page_shift - 5)) - 1), D);
                 r.k = __ldg(reinterpret_cast<const uint4 *>(u + U::kK + c * 512 + lane * 16));
-                r.v = __ldg(reinterpret_cast<const uint4 *>(u + U::kV + c * 512 + lane * 16));
+                r.v = __ldg(reinterpret_cast<const uint4 *>(u + U::kV + c * 512 + U::v_chunk(g, t)));
                 r.ks = __ldg(reinterpret_cast<const uint2 *>(u + U::kKs + c * 64 + g * 8));
                 r.vs0 = __ldg(reinterpret_cast<const uint2 *>(u + U::kVs + c * 64 + 2 * t * 8));
                 r.vs1 = __ldg(reinterpret_cast<const uint2 *>(u + U::kVs + c * 64 + (2 * t + 1) * 8));
