@@ -27,14 +27,15 @@ constexpr int kMaxCluster = 8;
 //   p = exp(z - max) / sum over the kept
 //   top_p in (0, 1): in that order, a token stays while the probabilities
 //       before it sum to less than top_p; p is divided by the sum of what stays
-// The row's slice stays in shared memory after one read.  The kept tokens are
-// found by a histogram of max - x in steps of 1/32 (few tokens lie near the
-// top, so its counters are hardly contended), and only tokens down to the bin
-// that holds the top_k-th are sorted; when that bin is too full (many equal
-// logits) a radix selection over the slices decides exactly.  Exponentials and
+// The row's slice stays in shared memory after one read.  The top_k-th largest of
+// the threads' own maxima bounds the top_k-th logit from below: a histogram of
+// the maxima (256 bins between the least and the largest of them) gives a bin
+// that it lies in, and only logits down to that bin are sorted, hardly more than
+// top_k.  Where there are too few maxima, or too many candidates (equal logits), a
+// radix selection over the slices decides exactly.  Exponentials and
 // sums of the kept are in 64 bits: the order and the top_p border are decided
 // by values next to each other.
-constexpr int kBins = 2048;
+constexpr int kBins = 256;
 constexpr int kCand = 2048;          // candidates that one sort takes
 constexpr int kSliceMax = 40960;     // logits of a slice in shared memory (a multiple of 4)
 
@@ -43,7 +44,7 @@ struct ProbsArgs {
     const uint32_t *prev;
     float *probs;
     int *err;
-    int V, n_prev, slice;
+    int V, n_prev, slice, by_maxima;
     qora_sample_params params;
 };
 
@@ -51,13 +52,13 @@ struct alignas(16) ProbsSmem {  // (the slice behind it is read in 16-byte piece
     unsigned hist[kBins];
     unsigned long long cand[kCand];   // order key of x, then ~index
     double wsum[kVWarps + 1];
-    float red[kVWarps];
-    float mx, slice_max;
+    float red[2][kVWarps];
+    float mx, mn, slice_max, slice_min;
     int bad, slice_bad;
     unsigned n_cand, eq_before;
     unsigned sel_bin, sel_below, sel_in;
     double sum, slice_sum;
-    unsigned eq_count;
+    unsigned eq_count, scan[kBins / 32];
 };
 
 static_assert(sizeof(ProbsSmem) % 16 == 0 && kSliceMax % 4 == 0, "the slice is 16-byte aligned");
@@ -220,36 +221,42 @@ __global__ void __launch_bounds__(kVThreads) k_sample_probs(const ProbsArgs a) {
         }
         __syncthreads();
     }
-    // maximum of the row
-    float mx = -INFINITY;
+    // the thread's maximum, the row's, and the least finite one of a thread
+    float top = -INFINITY;
     bool nan = false;
     each([&](int, float v) {
-        mx = fmaxf(mx, v);
+        top = fmaxf(top, v);
         nan = nan || v != v;
     });
-    mx = warp_max(mx);
-    if (lane == 0) sm->red[warp] = mx;
-    nan = __syncthreads_or(nan);
-    if (tid == 0) {
-        for (int w = 0; w < kVWarps; w++) mx = fmaxf(mx, sm->red[w]);
-        sm->slice_max = mx;
-        sm->slice_bad = nan;
-        sm->n_cand = 0;
-    }
+    float mx = warp_max(top), mn = -warp_max(top > -INFINITY ? -top : -INFINITY);
+    if (lane == 0) sm->red[0][warp] = mx, sm->red[1][warp] = mn;
     for (int i = tid; i < kBins; i += kVThreads) sm->hist[i] = 0;
+    nan = __syncthreads_or(nan);
+    if (warp == 0) {
+        mx = warp_max(lane < kVWarps ? sm->red[0][lane] : -INFINITY);
+        mn = -warp_max(lane < kVWarps ? -sm->red[1][lane] : -INFINITY);
+        if (lane == 0) {
+            sm->slice_max = mx;
+            sm->slice_min = mn;
+            sm->slice_bad = nan;
+            sm->n_cand = 0;
+        }
+    }
     meet();
     if (warp == 0) {  // a lane per block: remote reads in flight together
         const bool there = lane < (int)nr;
         const ProbsSmem *o = cl.map_shared_rank(sm, there ? lane : 0);
         const float m = warp_max(there ? o->slice_max : -INFINITY);
+        const float least = -warp_max(there ? -o->slice_min : -INFINITY);
         const bool bad = __any_sync(0xffffffffu, there && o->slice_bad);
         if (lane == 0) {
             sm->mx = m;
+            sm->mn = least;
             sm->bad = bad || !isfinite(m);
         }
     }
     __syncthreads();
-    mx = sm->mx;
+    mx = sm->mx, mn = sm->mn;
     const bool bad = sm->bad;
     const double temp = a.params.temperature > 0.0f ? (double)a.params.temperature : 1.0;
     const bool topk = a.params.top_k > 0 && a.params.top_k < a.V;
@@ -282,30 +289,57 @@ __global__ void __launch_bounds__(kVThreads) k_sample_probs(const ProbsArgs a) {
         return;
     }
     const unsigned k = a.params.top_k;
-    auto bin_of = [&](float v) { return (int)fminf((mx - v) * 32.0f, (float)(kBins - 1)); };
-    each([&](int, float v) { atomicAdd(&sm->hist[bin_of(v)], 1u); });
     if constexpr (VEC) {
         for (int i = tid; i < n / 4; i += kVThreads) reinterpret_cast<float4 *>(out)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
     } else {
         for (int i = tid; i < n; i += kVThreads) out[i] = 0.0f;
     }
-    meet();
-    if (warp == 0) select_bin<false>(cl, sm, kBins, k);
-    __syncthreads();
-    const int sel = sm->sel_bin;
-    const bool few = sm->sel_below + sm->sel_in <= kCand;
+    const float per_bin = mx > mn ? (float)(kBins - 1) / (mx - mn) : 0.0f;
+    auto bin_of = [&](float v) { return (int)fminf((mx - v) * per_bin, (float)(kBins - 1)); };
+    bool few = a.by_maxima;
+    int sel = 0;
+    if (few) {
+        if (top > -INFINITY) atomicAdd(&sm->hist[bin_of(top)], 1u);
+        meet();
+        // the bin of the k-th largest maximum; with fewer finite maxima than k, all bins
+        unsigned c = 0;
+        if (tid < kBins) {
+#pragma unroll
+            for (unsigned r = 0; r < kMaxCluster; r++)
+                if (r < nr) c += cl.map_shared_rank(sm, r)->hist[tid];
+        }
+        unsigned x = c;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        if (lane == 31 && warp < kBins / 32) sm->scan[warp] = x;
+        if (tid == 0) sm->sel_bin = kBins - 1;
+        __syncthreads();
+        unsigned before = 0;
+        for (int w = 0; w < warp && w < kBins / 32; w++) before += sm->scan[w];
+        if (tid < kBins && before + x >= k && before + x - c < k) sm->sel_bin = tid;
+        __syncthreads();
+        sel = sm->sel_bin;
+    }
     ProbsSmem *lead = cl.map_shared_rank(sm, 0);
     auto offer = [&](int i) {
         const unsigned at = atomicAdd(&lead->n_cand, 1u);
         if (at < kCand)
             lead->cand[at] = ((unsigned long long)order_key(x[i]) << 32) | (unsigned)~(unsigned)(v0 + i);
     };
-    meet();  // every block has read the histograms
     if (few) {
         each([&](int i, float v) {
             if (bin_of(v) <= sel) offer(i);
         });
-    } else {
+        meet();
+        few = lead->n_cand <= kCand;
+    }
+    if (!few) {
+        meet();  // (every block has seen the count)
+        if (tid == 0) sm->n_cand = 0;
+        meet();
         // radix selection of the k-th key, 8 bits at a time
         unsigned prefix = 0, mask = 0, need = k;
         for (int shift = 24; shift >= 0; shift -= 8) {
@@ -345,8 +379,9 @@ __global__ void __launch_bounds__(kVThreads) k_sample_probs(const ProbsArgs a) {
             before += (unsigned)total;
             if (i < n && (key > prefix || (same && at < need))) offer(i);
         }
+        meet();
     }
-    meet();
+    if (nr > 1) cl.sync();  // (no block leaves before its count is read)
     if (rank != 0) return;  // the rest is the leader's; it reads no other block's memory
     const unsigned found = min(sm->n_cand, (unsigned)kCand);
     const int size = found <= 256 ? 256 : kCand;
@@ -578,29 +613,35 @@ __global__ void __launch_bounds__(kVThreads) k_verify_drafts(const VerifyArgs a)
     // piece that has the goal is scanned.
     const double goal = fmax((double)u[a.K] * total, 0.0);
     if (base <= goal && goal < base + sm.sum) {
-        double lo = base, hi = base;
+        double lo = base;
         int at = 0;
         {
             double pre = 0.0;
             for (int w = 0; w < kVWarps; w++) {
                 const double next = pre + sm.wsum[w];
-                if (base + pre <= goal && goal < base + next) lo = base + pre, hi = base + next, at = w;
+                if (base + pre <= goal && goal < base + next) lo = base + pre, at = w;
                 pre = next;
             }
         }
         const int r0 = v0 + min(n, at * run), r1 = v0 + min(n, (at + 1) * run);
-        const int piece = ((r1 - r0 + kVWarps - 1) / kVWarps + kStep - 1) / kStep * kStep;
+        // (a short run is the one piece that there is)
+        const int piece = run <= 512 ? run : ((r1 - r0 + kVWarps - 1) / kVWarps + kStep - 1) / kStep * kStep;
         const int p0 = min(r1, r0 + warp * piece), p1 = min(r1, r0 + (warp + 1) * piece);
-        int mine = -1;
-        const double s = sum_of(p0, p1, mine);
+        if (run > 512) {
+            int mine = -1;
+            const double s = sum_of(p0, p1, mine);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, o));
-        if (lane == 0) {
-            sm.psum[warp] = s;
-            sm.plast[warp] = mine;
+            for (int o = 16; o > 0; o >>= 1) mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, o));
+            if (lane == 0) {
+                sm.psum[warp] = s;
+                sm.plast[warp] = mine;
+            }
+        } else if (lane == 0) {
+            sm.psum[warp] = 0.0;
+            sm.plast[warp] = warp == 0 ? sm.wlast[at] : -1;
         }
         __syncthreads();
-        // (rounding apart the pieces' sums end at hi: the last piece with a weight has what is left)
+        // (should the pieces' sums round below the run's, its last piece with a weight has the goal)
         double pre = lo;
         int who = -1;
         double from = lo;
@@ -627,7 +668,6 @@ __global__ void __launch_bounds__(kVThreads) k_verify_drafts(const VerifyArgs a)
             // a scan that rounds below its share's end has the piece's last token
             if (lane == 0) a.tokens[b * (a.K + 1) + acc] = token >= 0 ? token : sm.plast[warp];
         }
-        (void)hi;
     }
     if (rank == 0) {
         for (int j = tid; j <= a.K; j += kVThreads)
@@ -679,6 +719,10 @@ int qora_sample_probs(qora_ctx *ctx, const float *logits, int32_t B, int32_t V, 
     a.n_prev = n_prev;
     a.slice = ((V + nr - 1) / nr + 3) / 4 * 4;
     a.params = *params;
+    // threads that hold a logit, at least: half of them have to be enough for top_k
+    const int64_t holders = (int64_t)(nr - 1) * (a.slice / 4 < kVThreads ? a.slice / 4 : kVThreads) +
+                            (nr == 1 ? (V / 4 < kVThreads ? V / 4 : kVThreads) : 0);
+    a.by_maxima = topk && params->top_k <= holders / 2;
     const size_t smem = sizeof(ProbsSmem) + (size_t)a.slice * 4;
     auto kern = vec ? k_sample_probs<true> : k_sample_probs<false>;
     QORA_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -693,7 +737,11 @@ int qora_verify_drafts(qora_ctx *ctx, const int32_t *drafts, const float *draft_
         return set_error(QORA_ERR_INVALID, "qora_verify_drafts: bad arguments");
     DeviceGuard dg;
     QORA_TRY(dg.set(ctx->device));
-    const int nr = cluster_for(V, 8192);
+    // Wide rows go to a cluster, as wide as leaves all streams running at once (two
+    // blocks a multiprocessor): 64 streams of 151936 took 37 us with clusters of 8,
+    // in two waves.
+    int nr = cluster_for(V, 8192);
+    while (nr > 1 && (int64_t)B * nr > 2 * ctx->num_sms) nr >>= 1;
     VerifyArgs a;
     a.drafts = drafts;
     a.counts = counts;
