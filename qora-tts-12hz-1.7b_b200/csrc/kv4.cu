@@ -440,13 +440,15 @@ __device__ __forceinline__ bool row_place(const RowArgs &a, int slot, int &page,
     return true;
 }
 
-// Norm, rotation and append.  A warp takes 256 / D heads of one kind of RW rows:
-// q heads are normed, rotated and stored in f32; k heads normed, rotated and
-// stored in 4 bits; v heads stored in 4 bits.  What bounds the large case is how
-// much a multiprocessor has in flight (two rows a warp), then the 2-byte pieces
-// that the 4-bit rows are written in.
-template <int D, int RW>
-__global__ void __launch_bounds__(kRowWarps * 32) k_kv4_append(const RowArgs a) {
+// Norm, rotation and append.  A warp takes 256 / D heads of one kind of one row: q
+// heads are normed, rotated and stored in f32; k heads normed, rotated and stored
+// in 4 bits; v heads stored in 4 bits.  What bounds the large case is the way from
+// a multiprocessor to the L2 cache (69 % of its cycles): q rows in f32, and the
+// 2-byte pieces that 4-bit rows are written in, each a request of its own.  8191
+// rows of 16 / 8 heads of 128 take 54 us, against 56 to 66 with two rows or two
+// groups of heads a warp, and 83 with warps that fetch ahead and stay.
+template <int D>
+__global__ void __launch_bounds__(kRowWarps * 32, 6) k_kv4_append(const RowArgs a) {
     constexpr int HW = 256 / D;  // heads of a warp
     griddep_launch_dependents();
     griddep_wait();
@@ -454,43 +456,34 @@ __global__ void __launch_bounds__(kRowWarps * 32) k_kv4_append(const RowArgs a) 
     const int qt = (a.heads + HW - 1) / HW, kt = (a.L.kvh + HW - 1) / HW;
     const unsigned per = qt + 2 * kt;
     const unsigned task = blockIdx.x * kRowWarps + (threadIdx.x >> 5);  // (below 2^31: row_blocks)
-    const int i0 = (int)(task / per) * RW, w = (int)(task % per);
-    if (i0 >= a.rows) return;
+    const int i = (int)(task / per), w = (int)(task % per);
+    if (i >= a.rows) return;
     const int kind = w < qt ? 0 : w < qt + kt ? 1 : 2;
     const int n = kind == 0 ? a.heads : a.L.kvh;
     const int h = (w - (kind == 0 ? 0 : kind == 1 ? qt : qt + kt)) * HW + sub;  // this lane's head of its kind
     const bool on = h < n;
     const int first = kind == 0 ? 0 : kind == 1 ? a.heads : a.heads + a.L.kvh;
-    HeadVec<D> x[RW];
-    int slot[RW], pos[RW];
-#pragma unroll
-    for (int j = 0; j < RW; j++) {
-        const int i = min(i0 + j, a.rows - 1);
-        slot[j] = i0 + j < a.rows ? a.slots[i] : -1;
-        pos[j] = a.positions[i];
-        x[j].load(a.qkv + ((int64_t)i * (a.heads + 2 * a.L.kvh) + first + (on ? h : 0)) * D, l);
+    const int slot = a.slots[i], pos = a.positions[i];
+    HeadVec<D> x;
+    x.load(a.qkv + ((int64_t)i * (a.heads + 2 * a.L.kvh) + first + (on ? h : 0)) * D, l);
+    int page, unit, r;
+    if (!row_place(a, slot, page, unit, r)) return;
+    if (pos < 0 || pos >= a.rope_max) {
+        raise_error(a.err, kDevRange);
+        return;
     }
-#pragma unroll
-    for (int j = 0; j < RW; j++) {
-        int page, unit, r;
-        if (!row_place(a, slot[j], page, unit, r)) continue;
-        if (pos[j] < 0 || pos[j] >= a.rope_max) {
-            raise_error(a.err, kDevRange);
-            continue;
-        }
-        if (kind == 2) {
-            x[j].template store4<true>(a.L.unit(page, on ? h : 0, unit, D), r, l, on);
-            continue;
-        }
-        Angles<D> ang;
-        ang.load(a.cos + (int64_t)pos[j] * (D / 2), a.sin + (int64_t)pos[j] * (D / 2), l);
-        if (kind == 0) {
-            x[j].template norm_rope<float>(a.q_gamma, ang, l);
-            if (on) x[j].store(a.q_out + ((int64_t)(i0 + j) * a.heads + h) * D, l);
-        } else {
-            x[j].template norm_rope<double>(a.k_gamma, ang, l);
-            x[j].template store4<false>(a.L.unit(page, on ? h : 0, unit, D), r, l, on);
-        }
+    if (kind == 2) {
+        x.template store4<true>(a.L.unit(page, on ? h : 0, unit, D), r, l, on);
+        return;
+    }
+    Angles<D> ang;
+    ang.load(a.cos + (int64_t)pos * (D / 2), a.sin + (int64_t)pos * (D / 2), l);
+    if (kind == 0) {
+        x.template norm_rope<float>(a.q_gamma, ang, l);
+        if (on) x.store(a.q_out + ((int64_t)i * a.heads + h) * D, l);
+    } else {
+        x.template norm_rope<double>(a.k_gamma, ang, l);
+        x.template store4<false>(a.L.unit(page, on ? h : 0, unit, D), r, l, on);
     }
 }
 
@@ -709,10 +702,8 @@ int qora_kv4_append(qora_kv4 *kv, int32_t layer, const float *qkv, const uint16_
     const int hw = 256 / kv->hd;
     const int64_t per = (kv->heads + hw - 1) / hw + 2 * ((kv->kvh + hw - 1) / hw);
     dim3 grid;
-    const bool many = tokens * per > 16384;  // more than one warp for every place there is
-    QORA_TRY(row_blocks("qora_kv4_append", (many ? (tokens + 1) / 2 : tokens) * per, grid));
-    auto kern = kv->hd == 64 ? (many ? k_kv4_append<64, 2> : k_kv4_append<64, 1>)
-                             : (many ? k_kv4_append<128, 2> : k_kv4_append<128, 1>);
+    QORA_TRY(row_blocks("qora_kv4_append", tokens * per, grid));
+    auto kern = kv->hd == 64 ? k_kv4_append<64> : k_kv4_append<128>;
     return launch_ex(kern, grid, dim3(kRowWarps * 32), 0, as_stream(stream), 1u, a);
 }
 
