@@ -320,6 +320,17 @@ __device__ __forceinline__ void griddep_launch_dependents() {
 // (QORA_PDL=0 in the environment turns it off).
 bool pdl_enabled();
 
+// Lets a kernel take up to `bytes` of dynamic shared memory on the current device,
+// once per device (`done`: a static of the caller, one bit a device).
+template <class K>
+int allow_smem(K kern, size_t bytes, int device, std::atomic<uint64_t> &done) {
+    const uint64_t bit = 1ull << (device & 63);
+    if (device < 64 && (done.load(std::memory_order_relaxed) & bit)) return QORA_OK;
+    QORA_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    done.fetch_or(bit, std::memory_order_relaxed);
+    return QORA_OK;
+}
+
 // Launch with cudaLaunchKernelEx: PDL attribute and an optional (1, cy, 1)
 // thread-block cluster.
 template <typename... KArgs, typename... Args>

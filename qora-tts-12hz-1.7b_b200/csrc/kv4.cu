@@ -661,8 +661,8 @@ int qora_kv4_reserve(qora_kv4 *kv, const int32_t *counts, int32_t max_tokens, in
     a.pool_pages = kv->pool_pages;
     a.max_tokens = max_tokens;
     const size_t smem = ((size_t)((kv->pool_pages + 31) / 32) + 3 * (size_t)kv->streams) * 4;
-    if (smem > 40 * 1024)
-        QORA_CUDA(cudaFuncSetAttribute(k_kv4_reserve, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    static std::atomic<uint64_t> done;
+    QORA_TRY(allow_smem(k_kv4_reserve, ((1 << 20) / 32 + 3 * kKv4MaxStreams) * 4, kv->ctx->device, done));
     // a cluster pays when there are more table entries and tokens than one block
     // takes in a few rounds
     const bool wide = (int64_t)kv->streams * kv->pages_per_stream + max_tokens > 16384;

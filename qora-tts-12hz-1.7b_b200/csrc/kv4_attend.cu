@@ -625,7 +625,8 @@ template <int D, int NT, int ST>
 int clusters_of(const qora_kv4 *kv, int (&n)[3]) {
     auto kern = k_kv4_attend<D, NT, ST>;
     const size_t smem = smem_of<D, NT, ST>(kv->streams);
-    QORA_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    static std::atomic<uint64_t> done;  // (as much as the most streams need: caches share the kernel)
+    QORA_TRY(allow_smem(kern, smem_of<D, NT, ST>(kKv4MaxStreams), kv->ctx->device, done));
     for (int i = 0; i < 3; i++) {
         cudaLaunchConfig_t cfg;
         cudaLaunchAttribute at;
@@ -646,7 +647,6 @@ template <int D, int NT, int ST>
 int launch(const qora_kv4 *kv, const AttendArgs &a, const int (&n)[3], int64_t items, cudaStream_t st) {
     auto kern = k_kv4_attend<D, NT, ST>;
     const size_t smem = smem_of<D, NT, ST>(a.streams);
-    QORA_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     const int i = items <= n[0] ? 0 : items <= n[1] ? 1 : 2;
     return launch_ex(kern, dim3(n[i], kSizes[i]), dim3(kThreads), smem, st, (unsigned)kSizes[i], a);
 }

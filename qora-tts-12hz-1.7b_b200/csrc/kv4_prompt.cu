@@ -570,9 +570,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const PromptArgs a) 
 }
 
 template <int D>
-int launch(const PromptArgs &a, int64_t max_rows, cudaStream_t st) {
+int launch(const PromptArgs &a, int device, int64_t max_rows, cudaStream_t st) {
     auto kern = k_kv4_prompt<D>;
-    QORA_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Sm<D>)));
+    static std::atomic<uint64_t> done;
+    QORA_TRY(allow_smem(kern, sizeof(Sm<D>), device, done));
     const int64_t tiles = (max_rows + kRows - 1) / kRows;
     const unsigned y = (unsigned)(tiles < 65535 ? tiles : 65535);  // a block takes further tiles in turn
     // blocks start in the order of x first: the longest row tile of every stream and
@@ -596,7 +597,8 @@ int kv4_launch_prompt(qora_kv4 *kv, int layer, const float *q, const int *offset
     a.max_pos = kv->max_pos;
     a.tokens = tokens;
     a.scale_log2 = 1.4426950408889634f / sqrtf((float)kv->hd);
-    return kv->hd == 64 ? launch<64>(a, max_rows, st) : launch<128>(a, max_rows, st);
+    const int device = kv->ctx->device;
+    return kv->hd == 64 ? launch<64>(a, device, max_rows, st) : launch<128>(a, device, max_rows, st);
 }
 
 }  // namespace qora

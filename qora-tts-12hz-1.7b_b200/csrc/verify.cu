@@ -725,8 +725,8 @@ int qora_sample_probs(qora_ctx *ctx, const float *logits, int32_t B, int32_t V, 
     a.by_maxima = topk && params->top_k <= holders / 2;
     const size_t smem = sizeof(ProbsSmem) + (size_t)a.slice * 4;
     auto kern = vec ? k_sample_probs<true> : k_sample_probs<false>;
-    QORA_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                   (int)(sizeof(ProbsSmem) + kSliceMax * 4)));
+    static std::atomic<uint64_t> done[2];
+    QORA_TRY(allow_smem(kern, sizeof(ProbsSmem) + kSliceMax * 4, ctx->device, done[vec]));
     return launch_ex(kern, dim3(B, nr), dim3(kVThreads), smem, as_stream(stream), (unsigned)nr, a);
 }
 

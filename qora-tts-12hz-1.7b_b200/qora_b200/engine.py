@@ -22,6 +22,11 @@ def _stream(stream=None) -> int:
     return s.cuda_stream
 
 
+def _raw_stream(device: int) -> int:
+    """The device's current stream (without a Stream object: these calls are short)."""
+    return torch._C._cuda_getCurrentRawStream(device)
+
+
 def _dp(t: torch.Tensor | None):
     if t is None:
         return None
@@ -364,10 +369,12 @@ def sample_token(ctx: Context, logits: torch.Tensor, prev: torch.Tensor | None,
     return out
 
 
-def _rows_of(name: str, t: torch.Tensor, dtype, shape) -> int:
-    if t.dtype != dtype or tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{name}: expected {tuple(shape)} of {dtype}, got {tuple(t.shape)} of {t.dtype}")
-    return _dp(t)
+def _rows_of(name: str, t: torch.Tensor, dtype, shape, device: int) -> int:
+    """Pointer of a contiguous tensor of this type and shape on the device."""
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != device or not t.is_contiguous():
+        raise ValueError(f"{name}: expected contiguous {tuple(shape)} of {dtype} on cuda:{device}, got {tuple(t.shape)} "
+                         f"of {t.dtype} on {t.device}")
+    return t.data_ptr()
 
 
 def sample_probs(ctx: Context, logits: torch.Tensor, prev: torch.Tensor | None, params: _lib.SampleParams,
@@ -375,12 +382,16 @@ def sample_probs(ctx: Context, logits: torch.Tensor, prev: torch.Tensor | None, 
     """The distribution that sample_token draws from (generate_new.rs:771-851)
     for each row of logits [B][V]: [B][V], zero where top-k or top-p leave a
     token out.  prev int32 [B][n] (repetition penalty) or None."""
-    B, V = logits.shape
+    B, V = shape = logits.shape
+    dev, f32 = ctx.device, torch.float32
     out = out if out is not None else torch.empty_like(logits)
     n_prev = 0 if prev is None else prev.shape[-1]
-    _lib.call("qora_sample_probs", ctx.h, _rows_of("logits", logits, torch.float32, (B, V)), B, V,
-              None if not n_prev else _rows_of("prev", prev, torch.int32, (B, n_prev)), n_prev,
-              C.byref(params), _rows_of("out", out, torch.float32, (B, V)), _stream(stream))
+    rc = ctx._L.qora_sample_probs(ctx.h, _rows_of("logits", logits, f32, shape, dev), B, V,
+                                  _rows_of("prev", prev, torch.int32, (B, n_prev), dev) if n_prev else None, n_prev,
+                                  C.byref(params), _rows_of("out", out, f32, shape, dev),
+                                  _raw_stream(dev) if stream is None else stream.cuda_stream)
+    if rc:
+        _lib.check(rc, "qora_sample_probs")
     return out
 
 
@@ -394,17 +405,20 @@ def verify_drafts(ctx: Context, drafts: torch.Tensor, draft_probs: torch.Tensor 
     drawn token, then -1) and n_out int32 [B] (tokens of each stream)."""
     B, K = drafts.shape
     V = target_probs.shape[-1]
+    dev, i32, f32 = ctx.device, torch.int32, torch.float32
     if out is None:
-        out = (torch.empty(B, K + 1, dtype=torch.int32, device=drafts.device),
-               torch.empty(B, dtype=torch.int32, device=drafts.device))
+        out = (torch.empty(B, K + 1, dtype=i32, device=drafts.device), torch.empty(B, dtype=i32, device=drafts.device))
     tokens, n_out = out
-    _lib.call("qora_verify_drafts", ctx.h, _rows_of("drafts", drafts, torch.int32, (B, K)),
-              None if draft_probs is None else _rows_of("draft_probs", draft_probs, torch.float32, (B, K, V)),
-              _rows_of("target_probs", target_probs, torch.float32, (B, K + 1, V)),
-              None if counts is None else _rows_of("counts", counts, torch.int32, (B,)),
-              _rows_of("uniforms", uniforms, torch.float32, (B, K + 1)), B, K, V,
-              _rows_of("tokens", tokens, torch.int32, (B, K + 1)), _rows_of("n_out", n_out, torch.int32, (B,)),
-              _stream(stream))
+    rc = ctx._L.qora_verify_drafts(
+        ctx.h, _rows_of("drafts", drafts, i32, (B, K), dev),
+        _rows_of("draft_probs", draft_probs, f32, (B, K, V), dev) if draft_probs is not None else None,
+        _rows_of("target_probs", target_probs, f32, (B, K + 1, V), dev),
+        _rows_of("counts", counts, i32, (B,), dev) if counts is not None else None,
+        _rows_of("uniforms", uniforms, f32, (B, K + 1), dev), B, K, V,
+        _rows_of("tokens", tokens, i32, (B, K + 1), dev), _rows_of("n_out", n_out, i32, (B,), dev),
+        _raw_stream(dev) if stream is None else stream.cuda_stream)
+    if rc:
+        _lib.check(rc, "qora_verify_drafts")
     return out
 
 

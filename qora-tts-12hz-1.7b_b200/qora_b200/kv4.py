@@ -21,9 +21,9 @@ import numpy as np
 import torch
 
 from . import _lib
-from .engine import Context, _device_view, _dp
+from .engine import Context, _device_view, _raw_stream
 
-
+_F32, _I32 = torch.float32, torch.int32
 
 
 class Kv4Cache:
@@ -34,8 +34,11 @@ class Kv4Cache:
         self.ctx, self.layers, self.num_heads, self.kv_heads = ctx, layers, num_heads, kv_heads
         self.head_dim, self.max_pos, self.streams = head_dim, max_pos, streams
         self.page_positions, self.pool_pages = page_positions, pool_pages
-        self.device = f"cuda:{ctx.device}"
-        self._L = _lib.load()
+        self.device, self._dev = f"cuda:{ctx.device}", ctx.device
+        self._L = L = _lib.load()
+        # a decode step makes a call per layer: the entry points are looked up once
+        self._reserve, self._advance, self._append = L.qora_kv4_reserve, L.qora_kv4_advance, L.qora_kv4_append
+        self._write, self._read, self._attend = L.qora_kv4_write, L.qora_kv4_read, L.qora_kv4_attend
         h = C.c_void_p()
         _lib.call("qora_kv4_create", ctx.h, layers, num_heads, kv_heads, head_dim, max_pos, streams,
                   page_positions, pool_pages, C.byref(h))
@@ -47,14 +50,19 @@ class Kv4Cache:
             self.h = None
 
     def _typed(self, name: str, t: torch.Tensor, dtype, n: int) -> int:
-        """Pointer of a tensor of the cache's device that must hold at least n values of dtype."""
-        if t.dtype != dtype or t.numel() < n or not t.is_cuda or t.device.index != self.ctx.device:
-            raise ValueError(f"{name}: expected {n} values of {dtype} on {self.device}, got {tuple(t.shape)} of "
-                             f"{t.dtype} on {t.device}")
-        return _dp(t)
+        """Pointer of a contiguous tensor of the cache's device that holds at least n values of dtype."""
+        if t.dtype is not dtype or t.numel() < n or t.get_device() != self._dev or not t.is_contiguous():
+            raise ValueError(f"{name}: expected {n} contiguous values of {dtype} on {self.device}, got {tuple(t.shape)} "
+                             f"of {t.dtype} on {t.device}")
+        return t.data_ptr()
+
+    def _norm(self, name: str, t: torch.Tensor) -> int:
+        if t.element_size() != 2 or t.numel() < self.head_dim or t.get_device() != self._dev or not t.is_contiguous():
+            raise ValueError(f"{name}: expected {self.head_dim} f16 values on {self.device}")
+        return t.data_ptr()
 
     def _stream(self, stream) -> int:
-        return (stream if stream is not None else torch.cuda.current_stream(self.ctx.device)).cuda_stream
+        return _raw_stream(self._dev) if stream is None else stream.cuda_stream
 
     def reset(self, ids=None, stream=None):
         """Empties the streams `ids` (all: None)."""
@@ -85,16 +93,19 @@ class Kv4Cache:
             out = (torch.empty(max_tokens, **i32), torch.empty(max_tokens, **i32),
                    torch.empty(self.streams + 1, **i32))
         slots, positions, offsets = out
-        _lib.call("qora_kv4_reserve", self.h, self._typed("counts", counts, torch.int32, self.streams), max_tokens,
-                  self._typed("slots", slots, torch.int32, max_tokens),
-                  self._typed("positions", positions, torch.int32, max_tokens),
-                  self._typed("offsets", offsets, torch.int32, self.streams + 1), self._stream(stream))
+        rc = self._reserve(self.h, self._typed("counts", counts, _I32, self.streams), max_tokens,
+                           self._typed("slots", slots, _I32, max_tokens),
+                           self._typed("positions", positions, _I32, max_tokens),
+                           self._typed("offsets", offsets, _I32, self.streams + 1), self._stream(stream))
+        if rc:
+            _lib.check(rc, "qora_kv4_reserve")
         return out
 
     def advance(self, counts: torch.Tensor, stream=None):
         """Adds counts[b] (int32 [streams]; negative: rolls back) to the lengths."""
-        _lib.call("qora_kv4_advance", self.h, self._typed("counts", counts, torch.int32, self.streams),
-                  self._stream(stream))
+        rc = self._advance(self.h, self._typed("counts", counts, _I32, self.streams), self._stream(stream))
+        if rc:
+            _lib.check(rc, "qora_kv4_advance")
 
     def append(self, layer: int, qkv: torch.Tensor, q_norm: torch.Tensor, k_norm: torch.Tensor,
                rope_cos: torch.Tensor, rope_sin: torch.Tensor, positions: torch.Tensor,
@@ -102,25 +113,28 @@ class Kv4Cache:
         """qk-norm, RoPE and 4-bit append of one layer: qkv [n][q|k|v] raw
         projections; q_norm / k_norm f16 (or its bits as int16); returns the
         normed and rotated queries [n][num_heads * head_dim]."""
-        n, width = qkv.shape[0], (self.num_heads + 2 * self.kv_heads) * self.head_dim
+        n, hd = qkv.shape[0], self.head_dim
         if out is None:
-            out = torch.empty(n, self.num_heads * self.head_dim, device=qkv.device)
-        if q_norm.element_size() != 2 or k_norm.element_size() != 2 or min(q_norm.numel(), k_norm.numel()) < self.head_dim:
-            raise ValueError(f"q_norm / k_norm: expected {self.head_dim} f16 values")
-        rope_max = rope_cos.numel() // (self.head_dim // 2)
-        _lib.call("qora_kv4_append", self.h, layer, self._typed("qkv", qkv, torch.float32, n * width), _dp(q_norm),
-                  _dp(k_norm), self._typed("rope_cos", rope_cos, torch.float32, 0),
-                  self._typed("rope_sin", rope_sin, torch.float32, rope_cos.numel()), rope_max,
-                  self._typed("positions", positions, torch.int32, n), self._typed("slots", slots, torch.int32, n), n,
-                  self._typed("out", out, torch.float32, n * self.num_heads * self.head_dim), self._stream(stream))
+            out = torch.empty(n, self.num_heads * hd, device=qkv.device)
+        table = rope_cos.numel()
+        rc = self._append(self.h, layer, self._typed("qkv", qkv, _F32, n * (self.num_heads + 2 * self.kv_heads) * hd),
+                          self._norm("q_norm", q_norm), self._norm("k_norm", k_norm),
+                          self._typed("rope_cos", rope_cos, _F32, 0), self._typed("rope_sin", rope_sin, _F32, table),
+                          table // (hd // 2), self._typed("positions", positions, _I32, n),
+                          self._typed("slots", slots, _I32, n), n,
+                          self._typed("out", out, _F32, n * self.num_heads * hd), self._stream(stream))
+        if rc:
+            _lib.check(rc, "qora_kv4_append")
         return out
 
     def write(self, layer: int, slots: torch.Tensor, k: torch.Tensor, v: torch.Tensor, stream=None):
         """Stores rows of keys (normed, rotated) and values [n][kv_heads * head_dim]."""
         n = slots.numel()
         want = n * self.kv_heads * self.head_dim
-        _lib.call("qora_kv4_write", self.h, layer, self._typed("slots", slots, torch.int32, n), n,
-                  self._typed("k", k, torch.float32, want), self._typed("v", v, torch.float32, want), self._stream(stream))
+        rc = self._write(self.h, layer, self._typed("slots", slots, _I32, n), n, self._typed("k", k, _F32, want),
+                         self._typed("v", v, _F32, want), self._stream(stream))
+        if rc:
+            _lib.check(rc, "qora_kv4_write")
 
     def read(self, layer: int, slots: torch.Tensor, out=None, stream=None):
         """The keys and values that the slots hold, f32 [n][kv_heads * head_dim]
@@ -130,8 +144,10 @@ class Kv4Cache:
         if out is None:
             out = tuple(torch.zeros(n, self.kv_heads * self.head_dim, device=slots.device) for _ in range(2))
         k, v = out
-        _lib.call("qora_kv4_read", self.h, layer, self._typed("slots", slots, torch.int32, n), n,
-                  self._typed("k", k, torch.float32, want), self._typed("v", v, torch.float32, want), self._stream(stream))
+        rc = self._read(self.h, layer, self._typed("slots", slots, _I32, n), n, self._typed("k", k, _F32, want),
+                        self._typed("v", v, _F32, want), self._stream(stream))
+        if rc:
+            _lib.check(rc, "qora_kv4_read")
         return out
 
     def attend(self, layer: int, q: torch.Tensor, offsets: torch.Tensor, max_count: int,
@@ -142,7 +158,9 @@ class Kv4Cache:
         n, width = q.shape[0], self.num_heads * self.head_dim
         if out is None:
             out = torch.empty(n, width, device=q.device)
-        _lib.call("qora_kv4_attend", self.h, layer, self._typed("q", q, torch.float32, n * width),
-                  self._typed("offsets", offsets, torch.int32, self.streams + 1), n, max_count,
-                  self._typed("out", out, torch.float32, n * width), self._stream(stream))
+        rc = self._attend(self.h, layer, self._typed("q", q, _F32, n * width),
+                          self._typed("offsets", offsets, _I32, self.streams + 1), n, max_count,
+                          self._typed("out", out, _F32, n * width), self._stream(stream))
+        if rc:
+            _lib.check(rc, "qora_kv4_attend")
         return out
