@@ -435,18 +435,28 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_attend(const AttendArgs a) 
                 }
             }
             const bool edge = u * kKv4Unit + kKv4Unit - 1 > first_limit;
-            // the largest value scale of the unit sets the power of two
+            // the largest value scale of the unit sets the power of two; what an earlier
+            // user of the page left behind the last position that a row sees counts as zero
             uint2 vs[C];
-            __half2 big = __half2half2(__ushort_as_half(0));
+            __half2 b0 = __half2half2(__ushort_as_half(0)), b1 = b0;  // of positions g, g + 8 and g + 16, g + 24
 #pragma unroll
             for (int c = 0; c < C; c++) {
                 vs[c] = *reinterpret_cast<const uint2 *>(unit + U::kVs + c * 64 + g * 8);
-                big = __hmax2(big, __hmax2(u2h(vs[c].x), u2h(vs[c].y)));
+                b0 = __hmax2(b0, u2h(vs[c].x)), b1 = __hmax2(b1, u2h(vs[c].y));
             }
+            if (edge) {
+                int lim = limit[0];
+#pragma unroll
+                for (int nt = 1; nt < NT; nt++) lim = max(lim, limit[nt]);
+                lim = __reduce_max_sync(0xffffffffu, lim) - u * kKv4Unit - g;
+                b0 = u2h(h2u(b0) & ((lim >= 0 ? 0xffffu : 0u) | (lim >= 8 ? 0xffff0000u : 0u)));
+                b1 = u2h(h2u(b1) & ((lim >= 16 ? 0xffffu : 0u) | (lim >= 24 ? 0xffff0000u : 0u)));
+            }
+            __half2 big = __hmax2(b0, b1);
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) big = __hmax2(big, u2h(__shfl_xor_sync(0xffffffffu, h2u(big), o)));
             const unsigned bits = h2u(__hmax2(big, __lowhigh2highlow(big))) & 0x7c00u;
-            const int kn = min(ke, 24 - (int)(bits >> 10));
+            const int kn = 24 - (int)(bits >> 10);  // (sums stay under 2^20 2^19 2^24)
             const float shrink = __int_as_float((127 + kn - ke) << 23), lift = __int_as_float((127 + kn) << 23);
             ke = kn;
             float keep[NT];

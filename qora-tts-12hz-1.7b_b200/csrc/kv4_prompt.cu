@@ -410,7 +410,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const PromptArgs a) 
                         if (pos + 2 * t + 1 + 8 * i >= kend) v1x[i] = 0;
                         if (v0x[i] >= 0x7c00u) nan[j] |= 1u << (2 * t + 8 * i), v0x[i] = 0;
                         if (v1x[i] >= 0x7c00u) nan[j] |= 2u << (2 * t + 8 * i), v1x[i] = 0;
-                        if (kx[i] < 0x7c00u) kmost = max(kmost, kx[i]);
+                        if (kx[i] < 0x7c00u && pos + g + 8 * i < kend) kmost = max(kmost, kx[i]);
                         vmost = max(vmost, max(v0x[i], v1x[i]));
                     }
                     raw[j].vs0 = make_uint2(v0x[0] | v0x[1] << 16, v0x[2] | v0x[3] << 16);

@@ -382,6 +382,28 @@ def test_attend_sees_nothing_behind_the_last_position(ctx):
     assert _error(ctx) == 0
 
 
+@pytest.mark.parametrize("hd,lens,counts", [(64, [37, 0, 90], [2, 3, 1]), (128, [0, 161, 5], [1, 2, 70])])
+def test_what_a_page_held_before_does_not_matter(ctx, hd, lens, counts):
+    """The largest finite scales behind the streams' ends, as pages of other streams
+    may leave them: the same bits as behind zeros, small values and all."""
+    import torch
+    heads, kvh, page = 4, 2, 64
+    kv, offsets, held, rng = _filled(ctx, lens, counts, heads, kvh, hd, page, 31, 1e-3, 1e-4)
+    table = kv.state()["table"].cpu().numpy()
+    behind = _i32([int(table[b, p // page]) * page + p % page for b in range(3)
+                   for p in range(lens[b] + counts[b], -(-(lens[b] + counts[b]) // page) * page)])
+    n = sum(counts)
+    q = (50.0 * rng.standard_normal((n, heads, hd))).astype(np.float32)
+    for mc in (1, 8, 64):
+        got = []
+        for size in (0.0, 1e30):
+            rows = torch.full((behind.numel(), kvh * hd), size, device="cuda")
+            kv.write(1, behind, rows, rows)
+            got.append(_check(kv, q, offsets, held, lens, counts, heads, kvh, hd, mc))
+        assert np.array_equal(got[0].view(np.uint32), got[1].view(np.uint32))
+    assert _error(ctx) == 0
+
+
 def test_unaligned_pointers_are_refused(ctx, orc):
     import torch
     from qora_b200 import _lib
