@@ -244,6 +244,9 @@ int qora_kv_attend_noalloc(qora_kv *kv, int32_t layer, const float *qkv, int32_t
  * depend on the step before (drafted tokens that were accepted) needs no
  * return to the host:
  *     _reserve -> per layer: _append, _attend -> qora_verify_drafts -> _advance.
+ * Nothing is kept between calls but pages, table and lengths, so calls on
+ * different caches may overlap; calls on one cache that write what another
+ * reads are ordered by the caller (one stream, or events).
  * max_pos <= 2^20; streams <= 4096; head_dim 64 or 128; num_heads a multiple of
  * kv_heads; page_positions a power of two >= 32; pool_pages <= 2^20, and
  * pool_pages * page_positions < 2^31 (slots are int32). */
@@ -268,7 +271,7 @@ int qora_kv4_state(qora_kv4 *kv, int32_t **table, int32_t *pages_per_stream, int
  * not change.  All or nothing: when a length would pass max_pos (QORA_ERR_RANGE),
  * the tokens pass max_tokens (QORA_ERR_RANGE) or the pool has too few free
  * pages (QORA_ERR_OOM; each at the next qora_ctx_check_device_error), no page
- * is mapped, offsets are all 0 and slots all -1. */
+ * is mapped, offsets are all 0 and slots all -1.  max_tokens <= 2^30. */
 int qora_kv4_reserve(qora_kv4 *kv, const int32_t *counts, int32_t max_tokens, int32_t *slots,
                      int32_t *positions, int32_t *offsets, void *stream);
 /* Adds counts[b] (device; negative: rolls back) to every stream's length.  A

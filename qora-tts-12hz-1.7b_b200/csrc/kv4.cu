@@ -121,11 +121,11 @@ __global__ void __launch_bounds__(kResThreads) k_kv4_reserve(const ReserveArgs a
         if (b < a.streams) {
             len[b] = l;
             first[b] = (int)(at & 0xffffffff);
-            off[b] = (int)min(at >> 32, (int64_t)0x7fffffff);
+            off[b] = (int)min((uint64_t)at >> 32, (uint64_t)0x7fffffff);
         }
         base += total;
     }
-    const int64_t tokens = base >> 32;
+    const uint64_t tokens = (uint64_t)base >> 32;  // (streams 2^12, max_pos 2^20: below 2^32 where pages suffice)
     const int need = (int)(base & 0xffffffff);
     __syncthreads();
     // ---- mark the pages in use
@@ -185,7 +185,7 @@ __global__ void __launch_bounds__(kResThreads) k_kv4_reserve(const ReserveArgs a
         bad |= wrong[r];
     }
     const int all = nr * kResThreads, me = rank * kResThreads + tid;
-    const int why = bad ? kDevRange : tokens > a.max_tokens ? kDevRange : need > free_total ? kDevPool : 0;
+    const int why = bad ? kDevRange : tokens > (uint64_t)a.max_tokens ? kDevRange : need > free_total ? kDevPool : 0;
     if (why) {  // nothing is mapped, and every listed token is skipped
         if (me == 0) raise_error(a.err, why);
         for (int b = me; b <= a.streams; b += all) a.offsets[b] = 0;
@@ -223,7 +223,7 @@ __global__ void __launch_bounds__(kResThreads) k_kv4_reserve(const ReserveArgs a
     // ---- the tokens' slots and positions
     for (int i = me; i < a.max_tokens; i += all) {
         int slot = -1, pos = 0;
-        if (i < tokens) {
+        if (i < (int)tokens) {
             const int b = last_at_most(off, a.streams, i);
             pos = len[b] + i - off[b];
             const int pg = __ldcg(a.table + (int64_t)b * a.pages_per_stream + (pos >> a.page_shift));
@@ -644,6 +644,8 @@ int qora_kv4_reserve(qora_kv4 *kv, const int32_t *counts, int32_t max_tokens, in
                      int32_t *offsets, void *stream) {
     if (!kv || !counts || !offsets || max_tokens < 0 || (max_tokens > 0 && (!slots || !positions)))
         return set_error(QORA_ERR_INVALID, "qora_kv4_reserve: bad arguments");
+    if (max_tokens > (1 << 30))
+        return set_error(QORA_ERR_UNSUPPORTED, "qora_kv4_reserve: max_tokens %d (max 2^30)", max_tokens);
     DeviceGuard dg;
     QORA_TRY(dg.set(kv->ctx->device));
     ReserveArgs a;

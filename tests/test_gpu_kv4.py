@@ -7,7 +7,7 @@ import kv4_ref as R
 
 pytestmark = pytest.mark.gpu
 
-INVALID, OOM, RANGE = 1, 4, 5
+INVALID, OOM, RANGE, UNSUPPORTED = 1, 4, 5, 6
 
 
 @pytest.fixture(scope="module")
@@ -102,6 +102,23 @@ def test_reserve_refuses_as_a_whole(ctx, why, counts, max_tokens, status):
     assert bool((st["table"] == before).all()) and list(kv.lengths()) == [33, 0, 5]
     kv.reserve(_i32([1, 1, 1]), 3)                          # the cache goes on
     assert _error(ctx) == 0
+
+
+def test_reserve_counts_past_31_bits(ctx):
+    """4096 streams that share one page of 2^20 positions (their tables say so)
+    ask for all the rest of it: 2^32 - 4096 tokens, and no new page."""
+    S, P = 4096, 1 << 20
+    kv = _cache(ctx, 1, 1, 1, 64, P, S, P, 1)
+    st = kv.state()
+    st["table"].zero_()
+    st["lengths"].fill_(1)
+    slots, positions, offsets = kv.reserve(_i32([P - 1] * S), 100)
+    assert _error(ctx) == RANGE
+    assert (slots == -1).all() and (positions == 0).all() and (offsets == 0).all()
+    slots, positions, offsets = kv.reserve(_i32([1] + [0] * (S - 2) + [1]), 2)
+    assert _error(ctx) == 0 and slots.tolist() == [1, 1] and positions.tolist() == [1, 1]
+    p = slots.data_ptr()
+    assert kv._L.qora_kv4_reserve(kv.h, p, 2 ** 30 + 1, p, p, p, None) == UNSUPPORTED    # refused before any access
 
 
 def test_bad_table_entry_is_an_error_not_an_access(ctx):
