@@ -444,6 +444,8 @@ __global__ void __launch_bounds__(kVThreads) k_sample_probs(const ProbsArgs a) {
 // left), from p_a when all passed.  The products and sums are in 64 bits, so
 // that neither comparison turns on rounding.  Weights that are not positive
 // (NaN among them) count as zero.
+constexpr int kVocabMax = 1 << 30, kDraftsMax = 1 << 20;  // (indexes of a row stay in 32 bits)
+
 struct VerifyArgs {
     const int *drafts, *counts;
     const float *draft_probs, *target_probs, *uniforms;
@@ -735,6 +737,9 @@ int qora_verify_drafts(qora_ctx *ctx, const int32_t *drafts, const float *draft_
                        int32_t *tokens, int32_t *n_out, void *stream) {
     if (!ctx || !target_probs || !uniforms || !tokens || !n_out || B <= 0 || K < 0 || V <= 0 || (K > 0 && !drafts))
         return set_error(QORA_ERR_INVALID, "qora_verify_drafts: bad arguments");
+    if (V > kVocabMax || K > kDraftsMax)
+        return set_error(QORA_ERR_UNSUPPORTED, "qora_verify_drafts: %d drafts (max %d), vocab %d (max %d)", K, kDraftsMax,
+                         V, kVocabMax);
     DeviceGuard dg;
     QORA_TRY(dg.set(ctx->device));
     // Wide rows go to a cluster, as wide as leaves all streams running at once (two

@@ -55,6 +55,8 @@ def test_sampling_refusals_come_before_any_cuda_call(lib):
     assert v(ctx, one, one, one, None, one, 0, 1, 8, one, one, None) == INVALID
     assert v(ctx, one, one, one, None, one, 1, -1, 8, one, one, None) == INVALID
     assert v(ctx, one, one, one, None, one, 1, 1, 0, one, one, None) == INVALID
+    for K, V in ((1, 2 ** 30 + 1), (1, 2 ** 31 - 1), (2 ** 20 + 1, 8), (2 ** 31 - 1, 1)):
+        assert v(ctx, one, one, one, None, one, 1, K, V, one, one, None) == UNSUPPORTED
 
 
 def test_cache_shapes_are_refused(lib):
