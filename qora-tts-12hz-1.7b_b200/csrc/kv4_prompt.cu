@@ -13,14 +13,16 @@
 // stored scale), queries by one per row, both undone exactly.  The dropped
 // products of two low halves are 2^-22 of the result.
 //
-// Three kinds of warps work on different tiles at the same time: four unpack keys
-// and values into shared memory as matrix operands (two buffers), one issues the
-// products, eight do the softmax: a thread has one row, half of its positions for
-// P and half of its dimensions for O.  P goes back to tensor memory as an operand.
+// Four kinds of warps work on different tiles at the same time: four unpack keys
+// and four values into shared memory as matrix operands (two buffers each), one
+// issues the products, eight do the softmax: a thread has one row, half of its
+// positions for P and half of its dimensions for O.  P goes back to tensor memory as an operand.
 // The unit's layout gives a lane whole 16-byte operand rows: eight dimensions of a
 // key, and eight positions of a value's dimension (in the order 2t + e + 8h, which
 // P's columns follow).  O of each tile is added in f32 registers, because the
 // tensor core's own additions do not round to nearest.
+#include <type_traits>
+
 #include "kv4.cuh"
 #include "tc.cuh"
 
@@ -30,8 +32,12 @@ namespace {
 
 constexpr int kRows = 128;                 // query rows of a block
 constexpr int kKeys = 64;                  // positions of a tile: two units
-constexpr int kSoftWarps = 8, kUnpackWarps = 4;
-constexpr int kThreads = (kSoftWarps + kUnpackWarps + 1) * 32;
+constexpr int kSoftWarps = 8, kUnpackWarps = 4;      // (as many for keys as for values)
+constexpr int kThreads = (kSoftWarps + 2 * kUnpackWarps + 4) * 32;  // whole groups of four warps; one of the last has work
+// Registers of a thread: at launch, and as the groups of warps share them out.
+constexpr int kRegs = 96, kSoftRegs = 136, kUnpackRegs = 72, kLastRegs = 64;
+static_assert(kSoftWarps * kSoftRegs + 2 * kUnpackWarps * kUnpackRegs + 4 * kLastRegs <= kThreads / 32 * kRegs,
+              "no group waits for registers that the block does not have");
 constexpr uint32_t kTmemCols = 512;        // S 2 x 64, P (high, low) 2 x 64, O 128, Q (high, low) 128
 constexpr uint32_t kColS = 0, kColP = 128, kColO = 256, kColQ = 384;
 
@@ -61,9 +67,9 @@ struct Sm {
     // of a tile (four deep: unpacking is up to three tiles ahead of the softmax)
     float unk[4], unv[4];                  // its scales back
     unsigned vnan[4][2][D / 32];           // positions of a unit whose value scale is NaN, by group
-    unsigned most[2][kUnpackWarps];
+    unsigned most[2][2][kUnpackWarps];     // largest scales: keys, values
     alignas(8) uint64_t info[4];           // these are written (k_full may be a phase too far by then)
-    uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full, o_free;
+    uint64_t q_full, k_full[2], v_full[2], s_full[2], p_full[2], o_full[2], o_free;
     uint32_t tmem;
     int abort;
 };
@@ -92,14 +98,11 @@ __device__ __forceinline__ bool wait_one(uint64_t *bar, uint32_t parity, int *ab
     return true;
 }
 
-// Whether the phase is over, without waiting.
-__device__ __forceinline__ bool ready(uint64_t *bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
-                 : "=r"(ok)
-                 : "r"(smem_u32(bar)), "r"(parity)
-                 : "memory");
-    return ok != 0;
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t yes;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.b32 %0, 1, 0, p;\n}" : "=r"(yes));
+    return yes != 0;
 }
 
 // The same for a whole warp, with one answer.
@@ -125,10 +128,12 @@ __device__ __forceinline__ void codes(uint32_t w, uint32_t magic, __half2 (&x)[4
     x[3] = __hfma2(u2h(and_or<0x00f000f0u>(v, magic)), s16, hi);
 }
 
-// What a lane of an unpacking warp has of one (unit, scale group).
+// What a lane of an unpacking warp has of one (unit, scale group): codes, and the
+// scales of keys g + 8i, or of values 2t + 8i and 2t + 1 + 8i.
+template <bool V>
 struct Raw {
-    uint4 k, v;
-    uint2 ks, vs0, vs1;  // scales: keys g + 8i; values 2t + 8i and 2t + 1 + 8i
+    uint4 c;
+    uint2 s[V ? 2 : 1];
 };
 
 __device__ __forceinline__ float half_of(uint2 v, int i) {
@@ -139,15 +144,179 @@ __device__ __forceinline__ float half_of(uint2 v, int i) {
 // The power of two that brings scales up to `bits` (f16, finite) under 2^12.
 __device__ __forceinline__ int scale_exponent(unsigned bits) { return 26 - (int)((bits >> 10) & 31u); }
 
+// A row tile's keys or values, as matrix operands: the loop of an unpacking warp.
+template <int D, bool V>
+__device__ __forceinline__ void unpack(Sm<D> &sm, const PromptArgs &a, int b, int h, int ntiles, int kend, int done) {
+    using S = Sm<D>;
+    using U = Kv4Unit<D>;
+    constexpr int C = D / 32;
+    constexpr int kJobs = 2 * C / kUnpackWarps;  // (unit, group) pairs of a warp and tile
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int pw = (threadIdx.x >> 5) % kUnpackWarps;
+    uint32_t magic;
+    asm volatile("mov.b32 %0, 0x64006400;" : "=r"(magic));
+    const int *table = a.L.table + (int64_t)b * a.L.pages_per_stream;
+    auto page_of = [&](int it, int job) {  // physical page of a job's unit, -1 behind the last position
+        const int pos = it * kKeys + ((pw + kUnpackWarps * job) / C) * kKv4Unit;
+        if (it >= ntiles || pos >= kend) return -1;
+        int pg = __ldg(table + (pos >> a.L.page_shift));
+        if ((unsigned)pg >= (unsigned)a.L.pool_pages) {
+            raise_error(a.err, kDevRange);
+            pg = 0;
+        }
+        return pg;
+    };
+    auto load = [&](int it, int job, int pg, Raw<V> &r) {
+        r = Raw<V>{};
+        if (pg < 0) return;
+        const int combo = pw + kUnpackWarps * job, c = combo % C;
+        const int pos = it * kKeys + (combo / C) * kKv4Unit;
+        const uint8_t *u = a.L.unit(pg, h, (pos >> 5) & ((1 << (a.L.page_shift - 5)) - 1), D);
+        if constexpr (V) {
+            r.c = __ldg(reinterpret_cast<const uint4 *>(u + U::kV + c * 512 + U::v_chunk(g, t)));
+            r.s[0] = __ldg(reinterpret_cast<const uint2 *>(u + U::kVs + c * 64 + 2 * t * 8));
+            r.s[1] = __ldg(reinterpret_cast<const uint2 *>(u + U::kVs + c * 64 + (2 * t + 1) * 8));
+        } else {
+            r.c = __ldg(reinterpret_cast<const uint4 *>(u + U::kK + c * 512 + lane * 16));
+            r.s[0] = __ldg(reinterpret_cast<const uint2 *>(u + U::kKs + c * 64 + g * 8));
+        }
+    };
+    Raw<V> raw[kJobs], next[kJobs];
+    int page[kJobs];
+#pragma unroll
+    for (int j = 0; j < kJobs; j++) {
+        load(0, j, page_of(0, j), raw[j]);
+        page[j] = page_of(1, j);
+    }
+    for (int it = 0; it < ntiles; it++) {
+        const int gi = done + it, buf = gi & 1, slot = gi & 3;
+        // the next tile is in flight while this one is unpacked
+#pragma unroll
+        for (int j = 0; j < kJobs; j++) {
+            load(it + 1, j, page[j], next[j]);
+            page[j] = page_of(it + 2, j);
+        }
+        // the largest scale; ones behind the last position count as zero, and NaN ones of
+        // values are told to the rows (both are rare: a packed maximum finds them)
+        unsigned most = 0;
+        unsigned nan[kJobs];
+#pragma unroll
+        for (int j = 0; j < kJobs; j++) {
+            const int pos = it * kKeys + ((pw + kUnpackWarps * j) / C) * kKv4Unit;
+            nan[j] = 0;
+            unsigned m2 = __vmaxu2(raw[j].s[0].x, raw[j].s[0].y);
+            if constexpr (V) m2 = __vmaxu2(m2, __vmaxu2(raw[j].s[1].x, raw[j].s[1].y));
+            const unsigned m1 = max(m2 & 0xffffu, m2 >> 16);
+            if (!__any_sync(0xffffffffu, m1 >= 0x7c00u) && pos + kKv4Unit <= kend) {
+                most = max(most, m1);
+                continue;
+            }
+#pragma unroll
+            for (int e = 0; e < (V ? 2 : 1); e++) {
+                const uint2 w = raw[j].s[e];
+                unsigned x[4] = {w.x & 0xffffu, w.x >> 16, w.y & 0xffffu, w.y >> 16};
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int at = (V ? 2 * t + e : g) + 8 * i;
+                    if (pos + at >= kend) x[i] = 0;
+                    if (V && x[i] >= 0x7c00u) nan[j] |= 1u << at, x[i] = 0;
+                    if (x[i] < 0x7c00u) most = max(most, x[i]);
+                }
+                if (V) raw[j].s[e] = make_uint2(x[0] | x[1] << 16, x[2] | x[3] << 16);
+            }
+            if (V) nan[j] = __reduce_or_sync(0xffffffffu, nan[j]);
+        }
+        most = __reduce_max_sync(0xffffffffu, most);
+        if (lane == 0) sm.most[V][buf][pw] = most;
+        asm volatile("bar.sync %0, 128;" ::"n"(V ? 7 : 2) : "memory");
+#pragma unroll
+        for (int i = 0; i < kUnpackWarps; i++) most = max(most, sm.most[V][buf][i]);
+        const int e = scale_exponent(most);
+        const float up = pow2(e);
+        if constexpr (!V) {
+            if (gi >= 2) wait_for(&sm.s_full[buf], ((gi >> 1) - 1) & 1, &sm.abort, a.err);
+            if (pw == 0 && lane == 0) sm.unk[slot] = pow2(-e);  // (tile gi - 4 of the slot has been read by now)
+#pragma unroll
+            for (int j = 0; j < kJobs; j++) {
+                const int combo = pw + kUnpackWarps * j, c = combo % C, u = combo / C;
+                const uint32_t kw[4] = {raw[j].c.x, raw[j].c.y, raw[j].c.z, raw[j].c.w};
+                // keys g + 8i: dimensions 32c + 8t .. + 7 are one operand row of 16 bytes
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    __half2 x[4];
+                    codes(kw[i], magic, x);
+                    const __half2 s = __float2half2_rn(half_of(raw[j].s[0], i) * up);
+                    uint32_t hi[4], lo[4];
+#pragma unroll
+                    for (int p = 0; p < 4; p++) {
+                        const __half2 w = __hmul2(s, x[p]);
+                        hi[p] = h2u(w);
+                        lo[p] = h2u(__hfma2(s, x[p], __hneg2(w)));
+                    }
+                    const int at = ((4 * u + i) * (D / 8) + 4 * c + t) * S::kKStep + g * 16;
+                    *reinterpret_cast<uint4 *>(sm.k[buf][0] + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    *reinterpret_cast<uint4 *>(sm.k[buf][1] + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                }
+                raw[j] = next[j];
+            }
+            tc::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&sm.info[slot]);
+                mbar_arrive(&sm.k_full[buf]);
+            }
+        } else {
+            if (lane == 0) {
+                if (pw == 0) sm.unv[slot] = pow2(-e);
+#pragma unroll
+                for (int j = 0; j < kJobs; j++) {
+                    const int combo = pw + kUnpackWarps * j;
+                    sm.vnan[slot][combo / C][combo % C] = nan[j];
+                }
+                mbar_arrive(&sm.info[slot]);
+            }
+            if (gi >= 2) wait_for(&sm.o_full[buf], ((gi >> 1) - 1) & 1, &sm.abort, a.err);
+#pragma unroll
+            for (int j = 0; j < kJobs; j++) {
+                const int combo = pw + kUnpackWarps * j, c = combo % C, u = combo / C;
+                const uint32_t vw[4] = {raw[j].c.x, raw[j].c.y, raw[j].c.z, raw[j].c.w};
+                // dimensions 32c + 4g + p: positions 2t + e + 8i are one operand row
+                uint32_t hi[4][4], lo[4][4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    __half2 x[4];
+                    codes(vw[i], magic, x);
+                    // a word is two positions: the pair of nibble p has both
+                    const __half2 s = __floats2half2_rn(half_of(raw[j].s[0], i) * up, half_of(raw[j].s[1], i) * up);
+#pragma unroll
+                    for (int p = 0; p < 4; p++) {
+                        const __half2 w = __hmul2(s, x[p]);
+                        hi[p][i] = h2u(w);
+                        lo[p][i] = h2u(__hfma2(s, x[p], __hneg2(w)));
+                    }
+                }
+#pragma unroll
+                for (int p = 0; p < 4; p++) {
+                    const int at = ((4 * c + (g >> 1)) * (kKeys / 8) + 4 * u + t) * S::kVStep + (4 * (g & 1) + p) * 16;
+                    *reinterpret_cast<uint4 *>(sm.v[buf][0] + at) = make_uint4(hi[p][0], hi[p][1], hi[p][2], hi[p][3]);
+                    *reinterpret_cast<uint4 *>(sm.v[buf][1] + at) = make_uint4(lo[p][0], lo[p][1], lo[p][2], lo[p][3]);
+                }
+                raw[j] = next[j];
+            }
+            tc::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.v_full[buf]);
+        }
+    }
+}
+
 template <int D>
 __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const PromptArgs a) {
     using S = Sm<D>;
-    using U = Kv4Unit<D>;
     constexpr int C = D / 32;
     extern __shared__ __align__(1024) uint8_t dyn[];
     S &sm = *reinterpret_cast<S *>(dyn);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int g = lane >> 2, t = lane & 3;
     const int h = blockIdx.x % a.L.kvh, b = blockIdx.x / a.L.kvh;
     const int G = a.heads / a.L.kvh;
     griddep_wait();
@@ -162,15 +331,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const PromptArgs a) 
     if (tid == 0) {
         for (int i = 0; i < 2; i++) {
             mbar_init(&sm.k_full[i], kUnpackWarps);
-            mbar_init(&sm.k_empty[i], 1);
             mbar_init(&sm.v_full[i], kUnpackWarps);
-            mbar_init(&sm.v_empty[i], 1);
+            mbar_init(&sm.o_full[i], 1);
             mbar_init(&sm.s_full[i], 1);
             mbar_init(&sm.p_full[i], kSoftWarps);
         }
-        for (int i = 0; i < 4; i++) mbar_init(&sm.info[i], kUnpackWarps);
+        for (int i = 0; i < 4; i++) mbar_init(&sm.info[i], 2 * kUnpackWarps);
         mbar_init(&sm.q_full, kSoftWarps);
-        mbar_init(&sm.o_full, 1);
         mbar_init(&sm.o_free, kSoftWarps);
         sm.abort = 0;
         mbar_fence_init();
@@ -186,16 +353,34 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const PromptArgs a) 
     __syncthreads();
     tc::fence_after_sync();
     const uint32_t tmem = sm.tmem;
-    int done = 0;  // tiles of this block's earlier row tiles: the barriers count on
-    int turn = 0;  // and row tiles
-    for (int qi = blockIdx.y; qi < nq; qi += gridDim.y, turn++) {
-        const int row0 = (nq - 1 - qi) * kRows;  // the longest row tiles first
-        const int rows = min(kRows, n * G - row0);
-        const int first_limit = len + row0 / G;                // every row sees these positions
-        const int kend = len + (row0 + rows - 1) / G + 1;      // positions that some row sees
-        const int ntiles = (kend + kKeys - 1) / kKeys;
-        const float *q = a.q + ((int64_t)off * a.heads + h * G) * D;  // row r: token r / G, head r % G
-        if (warp < kSoftWarps) {
+    // f for each of the block's row tiles, by every warp; `done`: tiles of the block's
+    // earlier row tiles (the barriers count on), `turn`: and row tiles
+    struct Tile {
+        int row0, rows, first_limit, kend, ntiles, done, turn;
+    };
+    auto each_tile = [&](auto f) {
+        int done = 0, turn = 0;
+        for (int qi = blockIdx.y; qi < nq; qi += gridDim.y, turn++) {
+            Tile x;
+            x.row0 = (nq - 1 - qi) * kRows;  // the longest row tiles first
+            x.rows = min(kRows, n * G - x.row0);
+            x.first_limit = len + x.row0 / G;                  // every row sees these positions
+            x.kend = len + (x.row0 + x.rows - 1) / G + 1;      // positions that some row sees
+            x.ntiles = (x.kend + kKeys - 1) / kKeys;
+            x.done = done, x.turn = turn;
+            f(x);
+            done += x.ntiles;
+            tc::fence_before_sync();
+            asm volatile("bar.sync 0;" ::: "memory");  // operands and tensor memory are free for the next row tile
+            tc::fence_after_sync();
+            if (sm.abort) break;
+        }
+    };
+    const float *q = a.q + ((int64_t)off * a.heads + h * G) * D;  // row r: token r / G, head r % G
+    if (warp < kSoftWarps) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
+        each_tile([&](const Tile &T) {
+            const int row0 = T.row0, rows = T.rows, first_limit = T.first_limit, ntiles = T.ntiles, done = T.done;
             // ================================================= softmax
             const int hs = warp >> 2, r = 32 * (warp & 3) + lane;
             const uint32_t t_lane = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
@@ -248,7 +433,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const PromptArgs a) 
             // adds O of tile `it` (which the products have finished)
             auto fold = [&](int it) {
                 const int gi = done + it;
-                wait_for(&sm.o_full, gi & 1, &sm.abort, a.err);
+                wait_for(&sm.o_full[gi & 1], (gi >> 1) & 1, &sm.abort, a.err);
                 tc::fence_after_sync();
 #pragma unroll
                 for (int p = 0; p < D / 64; p++) {
@@ -342,228 +527,76 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const PromptArgs a) 
                         make_float4(__fdiv_rn(o[i], sum), __fdiv_rn(o[i + 1], sum), __fdiv_rn(o[i + 2], sum),
                                     __fdiv_rn(o[i + 3], sum));
             }
-        } else if (warp < kSoftWarps + kUnpackWarps) {
-            // ================================================= unpacking
-            constexpr int kJobs = 2 * C / kUnpackWarps;  // (unit, group) pairs of a warp and tile
-            const int pw = warp - kSoftWarps;
-            uint32_t magic;
-            asm volatile("mov.b32 %0, 0x64006400;" : "=r"(magic));
-            const int *table = a.L.table + (int64_t)b * a.L.pages_per_stream;
-            auto page_of = [&](int it, int job) {  // physical page of a job's unit, -1 behind the last position
-                const int pos = it * kKeys + ((pw + kUnpackWarps * job) / C) * kKv4Unit;
-                if (it >= ntiles || pos >= kend) return -1;
-                int pg = __ldg(table + (pos >> a.L.page_shift));
-                if ((unsigned)pg >= (unsigned)a.L.pool_pages) {
-                    raise_error(a.err, kDevRange);
-                    pg = 0;
-                }
-                return pg;
-            };
-            auto load = [&](int it, int job, int pg, Raw &r) {
-                r = Raw{};
-                if (pg < 0) return;
-                const int combo = pw + kUnpackWarps * job, c = combo % C;
-                const int pos = it * kKeys + (combo / C) * kKv4Unit;
-                const uint8_t *u = a.L.unit(pg, h, (pos >> 5) & ((1 << (a.L.page_shift - 5)) - 1), D);
-                r.k = __ldg(reinterpret_cast<const uint4 *>(u + U::kK + c * 512 + lane * 16));
-                r.v = __ldg(reinterpret_cast<const uint4 *>(u + U::kV + c * 512 + U::v_chunk(g, t)));
-                r.ks = __ldg(reinterpret_cast<const uint2 *>(u + U::kKs + c * 64 + g * 8));
-                r.vs0 = __ldg(reinterpret_cast<const uint2 *>(u + U::kVs + c * 64 + 2 * t * 8));
-                r.vs1 = __ldg(reinterpret_cast<const uint2 *>(u + U::kVs + c * 64 + (2 * t + 1) * 8));
-            };
-            Raw raw[kJobs], next[kJobs];
-            int page[kJobs];
-#pragma unroll
-            for (int j = 0; j < kJobs; j++) {
-                load(0, j, page_of(0, j), raw[j]);
-                page[j] = page_of(1, j);
-            }
-            for (int it = 0; it < ntiles; it++) {
-                const int gi = done + it, buf = gi & 1, slot = gi & 3;
-                // the next tile is in flight while this one is unpacked
-#pragma unroll
-                for (int j = 0; j < kJobs; j++) {
-                    load(it + 1, j, page[j], next[j]);
-                    page[j] = page_of(it + 2, j);
-                }
-                // the largest scales; ones behind the last position count as zero, and NaN
-                // ones are told to the rows (both are rare: a packed maximum finds them)
-                unsigned kmost = 0, vmost = 0;
-                unsigned nan[kJobs];
-#pragma unroll
-                for (int j = 0; j < kJobs; j++) {
-                    const int pos = it * kKeys + ((pw + kUnpackWarps * j) / C) * kKv4Unit;
-                    nan[j] = 0;
-                    const unsigned k2 = __vmaxu2(raw[j].ks.x, raw[j].ks.y);
-                    const unsigned v2 = __vmaxu2(__vmaxu2(raw[j].vs0.x, raw[j].vs0.y), __vmaxu2(raw[j].vs1.x, raw[j].vs1.y));
-                    const unsigned k1 = max(k2 & 0xffffu, k2 >> 16), v1 = max(v2 & 0xffffu, v2 >> 16);
-                    if (!__any_sync(0xffffffffu, max(k1, v1) >= 0x7c00u) && pos + kKv4Unit <= kend) {
-                        kmost = max(kmost, k1), vmost = max(vmost, v1);
-                        continue;
-                    }
-                    unsigned v0x[4] = {raw[j].vs0.x & 0xffffu, raw[j].vs0.x >> 16, raw[j].vs0.y & 0xffffu, raw[j].vs0.y >> 16};
-                    unsigned v1x[4] = {raw[j].vs1.x & 0xffffu, raw[j].vs1.x >> 16, raw[j].vs1.y & 0xffffu, raw[j].vs1.y >> 16};
-                    const unsigned kx[4] = {raw[j].ks.x & 0xffffu, raw[j].ks.x >> 16, raw[j].ks.y & 0xffffu, raw[j].ks.y >> 16};
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        if (pos + 2 * t + 8 * i >= kend) v0x[i] = 0;
-                        if (pos + 2 * t + 1 + 8 * i >= kend) v1x[i] = 0;
-                        if (v0x[i] >= 0x7c00u) nan[j] |= 1u << (2 * t + 8 * i), v0x[i] = 0;
-                        if (v1x[i] >= 0x7c00u) nan[j] |= 2u << (2 * t + 8 * i), v1x[i] = 0;
-                        if (kx[i] < 0x7c00u && pos + g + 8 * i < kend) kmost = max(kmost, kx[i]);
-                        vmost = max(vmost, max(v0x[i], v1x[i]));
-                    }
-                    raw[j].vs0 = make_uint2(v0x[0] | v0x[1] << 16, v0x[2] | v0x[3] << 16);
-                    raw[j].vs1 = make_uint2(v1x[0] | v1x[1] << 16, v1x[2] | v1x[3] << 16);
-                    nan[j] = __reduce_or_sync(0xffffffffu, nan[j]);
-                }
-                kmost = __reduce_max_sync(0xffffffffu, kmost);
-                vmost = __reduce_max_sync(0xffffffffu, vmost);
-                if (lane == 0) sm.most[buf][pw] = kmost << 16 | vmost;
-                asm volatile("bar.sync 2, 128;" ::: "memory");
-                kmost = vmost = 0;
-#pragma unroll
-                for (int i = 0; i < kUnpackWarps; i++) {
-                    const unsigned w = sm.most[buf][i];
-                    kmost = max(kmost, w >> 16), vmost = max(vmost, w & 0xffffu);
-                }
-                const int ek = scale_exponent(kmost), ev = scale_exponent(vmost);
-                const float upk = pow2(ek), upv = pow2(ev);
-                if (gi >= 2) wait_for(&sm.k_empty[buf], ((gi >> 1) - 1) & 1, &sm.abort, a.err);
-#pragma unroll
-                for (int j = 0; j < kJobs; j++) {
-                    const int combo = pw + kUnpackWarps * j, c = combo % C, u = combo / C;
-                    const uint32_t kw[4] = {raw[j].k.x, raw[j].k.y, raw[j].k.z, raw[j].k.w};
-                    // keys g + 8i: dimensions 32c + 8t .. + 7 are one operand row of 16 bytes
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        __half2 x[4];
-                        codes(kw[i], magic, x);
-                        const __half2 s = __float2half2_rn(half_of(raw[j].ks, i) * upk);
-                        uint32_t hi[4], lo[4];
-#pragma unroll
-                        for (int p = 0; p < 4; p++) {
-                            const __half2 w = __hmul2(s, x[p]);
-                            hi[p] = h2u(w);
-                            lo[p] = h2u(__hfma2(s, x[p], __hneg2(w)));
-                        }
-                        const int at = ((4 * u + i) * (D / 8) + 4 * c + t) * S::kKStep + g * 16;
-                        *reinterpret_cast<uint4 *>(sm.k[buf][0] + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                        *reinterpret_cast<uint4 *>(sm.k[buf][1] + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                    }
-                    if (lane == 0) sm.vnan[slot][u][c] = nan[j];
-                }
-                if (pw == 0 && lane == 0) {
-                    sm.unk[slot] = pow2(-ek);
-                    sm.unv[slot] = pow2(-ev);
-                }
-                tc::fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(&sm.info[slot]);
-                    mbar_arrive(&sm.k_full[buf]);
-                }
-                if (gi >= 2) wait_for(&sm.v_empty[buf], ((gi >> 1) - 1) & 1, &sm.abort, a.err);
-#pragma unroll
-                for (int j = 0; j < kJobs; j++) {
-                    const int combo = pw + kUnpackWarps * j, c = combo % C, u = combo / C;
-                    const uint32_t vw[4] = {raw[j].v.x, raw[j].v.y, raw[j].v.z, raw[j].v.w};
-                    // dimensions 32c + 4g + p: positions 2t + e + 8i are one operand row
-                    uint32_t hi[4][4], lo[4][4];
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        __half2 x[4];
-                        codes(vw[i], magic, x);
-                        // a word is two positions: the pair of nibble p has both
-                        const __half2 s = __floats2half2_rn(half_of(raw[j].vs0, i) * upv, half_of(raw[j].vs1, i) * upv);
-#pragma unroll
-                        for (int p = 0; p < 4; p++) {
-                            const __half2 w = __hmul2(s, x[p]);
-                            hi[p][i] = h2u(w);
-                            lo[p][i] = h2u(__hfma2(s, x[p], __hneg2(w)));
-                        }
-                    }
-#pragma unroll
-                    for (int p = 0; p < 4; p++) {
-                        const int at = ((4 * c + (g >> 1)) * (kKeys / 8) + 4 * u + t) * S::kVStep + (4 * (g & 1) + p) * 16;
-                        *reinterpret_cast<uint4 *>(sm.v[buf][0] + at) = make_uint4(hi[p][0], hi[p][1], hi[p][2], hi[p][3]);
-                        *reinterpret_cast<uint4 *>(sm.v[buf][1] + at) = make_uint4(lo[p][0], lo[p][1], lo[p][2], lo[p][3]);
-                    }
-                    raw[j] = next[j];
-                }
-                tc::fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sm.v_full[buf]);
-            }
-        } else {
+        });
+    } else if (warp < kSoftWarps + kUnpackWarps) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kUnpackRegs));
+        each_tile([&](const Tile &T) { unpack<D, false>(sm, a, b, h, T.ntiles, T.kend, T.done); });
+    } else if (warp < kSoftWarps + 2 * kUnpackWarps) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kUnpackRegs));
+        each_tile([&](const Tile &T) { unpack<D, true>(sm, a, b, h, T.ntiles, T.kend, T.done); });
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLastRegs));
+        each_tile([&](const Tile &T) {
+            const int ntiles = T.ntiles, done = T.done, turn = T.turn;
             // ================================================= products
-            if (lane == 0) {
+            if (warp == kSoftWarps + 2 * kUnpackWarps && elect_one()) {
                 constexpr uint32_t id_s = tc::idesc_f16_f32(kRows, kKeys), id_o = tc::idesc_f16_f32(kRows, D);
                 const uint32_t qt = tmem + kColQ;
-                bool go = wait_one(&sm.q_full, turn & 1, &sm.abort, a.err);
-                tc::fence_after_sync();
-                // S of tile ns and O of tile no, each as soon as its operands are there; S has
-                // two buffers, so it is at most two tiles ahead
-                int ns = 0, no = 0;
-                uint64_t t0 = global_ns();
-                while (go && no < ntiles) {
-                    bool did = false;
-                    const int gs = done + ns, go_ = done + no;
-                    if (ns < ntiles && ns <= no + 1 && ready(&sm.k_full[gs & 1], (gs >> 1) & 1)) {
-                        tc::fence_after_sync();
-                        const int buf = gs & 1;
-                        const uint32_t kh = smem_u32(sm.k[buf][0]), kl = smem_u32(sm.k[buf][1]);
-                        const uint32_t d = tmem + kColS + 64 * buf;
+                auto arrived = [&](uint64_t *bar, int phase) { return wait_one(bar, phase & 1, &sm.abort, a.err); };
+                // (the buffer is a constant in each product: addresses and descriptors are too)
+                auto scores_in = [&](auto buf_, int gi) {
+                    constexpr int buf = decltype(buf_)::value;
+                    if (!arrived(&sm.k_full[buf], gi >> 1)) return false;
+                    tc::fence_after_sync();
+                    const uint32_t kh = smem_u32(sm.k[buf][0]), kl = smem_u32(sm.k[buf][1]);
+                    const uint32_t d = tmem + kColS + 64 * buf;
 #pragma unroll
-                        for (int j = 0; j < D / 16; j++) {
-                            const uint64_t bh = tc::smem_desc(kh + 2 * S::kKStep * j, S::kKStep, (D / 8) * S::kKStep);
-                            const uint64_t bl = tc::smem_desc(kl + 2 * S::kKStep * j, S::kKStep, (D / 8) * S::kKStep);
-                            tc::mma_f16_ts(d, qt + 8 * j, bh, id_s, j != 0 ? 1u : 0u);
-                            tc::mma_f16_ts(d, qt + 8 * j, bl, id_s, 1u);
-                            tc::mma_f16_ts(d, qt + D / 2 + 8 * j, bh, id_s, 1u);
-                        }
-                        tc::commit(&sm.s_full[buf]);
-                        tc::commit(&sm.k_empty[buf]);
-                        ns++;
-                        did = true;
+                    for (int j = 0; j < D / 16; j++) {
+                        const uint64_t bh = tc::smem_desc(kh + 2 * S::kKStep * j, S::kKStep, (D / 8) * S::kKStep);
+                        const uint64_t bl = tc::smem_desc(kl + 2 * S::kKStep * j, S::kKStep, (D / 8) * S::kKStep);
+                        tc::mma_f16_ts(d, qt + 8 * j, bh, id_s, j != 0 ? 1u : 0u);
+                        tc::mma_f16_ts(d, qt + 8 * j, bl, id_s, 1u);
+                        tc::mma_f16_ts(d, qt + D / 2 + 8 * j, bh, id_s, 1u);
                     }
-                    if (no < ns && ready(&sm.p_full[go_ & 1], (go_ >> 1) & 1) && ready(&sm.v_full[go_ & 1], (go_ >> 1) & 1) &&
-                        (go_ == 0 || ready(&sm.o_free, (go_ - 1) & 1))) {
-                        tc::fence_after_sync();
-                        const int buf = go_ & 1;
-                        const uint32_t vh = smem_u32(sm.v[buf][0]), vl = smem_u32(sm.v[buf][1]);
-                        const uint32_t d = tmem + kColO, p = tmem + kColP + 64 * buf;
+                    tc::commit(&sm.s_full[buf]);
+                    return true;
+                };
+                auto values_in = [&](auto buf_, int gi) {
+                    constexpr int buf = decltype(buf_)::value;
+                    if (!arrived(&sm.v_full[buf], gi >> 1) || (gi > 0 && !arrived(&sm.o_free, gi - 1)) ||
+                        !arrived(&sm.p_full[buf], gi >> 1))
+                        return false;
+                    tc::fence_after_sync();
+                    const uint32_t vh = smem_u32(sm.v[buf][0]), vl = smem_u32(sm.v[buf][1]);
+                    const uint32_t d = tmem + kColO, p = tmem + kColP + 64 * buf;
 #pragma unroll
-                        for (int j = 0; j < kKeys / 16; j++) {
-                            const uint64_t bh = tc::smem_desc(vh + 2 * S::kVStep * j, S::kVStep, (kKeys / 8) * S::kVStep);
-                            const uint64_t bl = tc::smem_desc(vl + 2 * S::kVStep * j, S::kVStep, (kKeys / 8) * S::kVStep);
-                            tc::mma_f16_ts(d, p + 8 * j, bh, id_o, j != 0 ? 1u : 0u);
-                            tc::mma_f16_ts(d, p + 8 * j, bl, id_o, 1u);
-                            tc::mma_f16_ts(d, p + 32 + 8 * j, bh, id_o, 1u);
-                        }
-                        tc::commit(&sm.o_full);
-                        tc::commit(&sm.v_empty[buf]);
-                        no++;
-                        did = true;
+                    for (int j = 0; j < kKeys / 16; j++) {
+                        const uint64_t bh = tc::smem_desc(vh + 2 * S::kVStep * j, S::kVStep, (kKeys / 8) * S::kVStep);
+                        const uint64_t bl = tc::smem_desc(vl + 2 * S::kVStep * j, S::kVStep, (kKeys / 8) * S::kVStep);
+                        tc::mma_f16_ts(d, p + 8 * j, bh, id_o, j != 0 ? 1u : 0u);
+                        tc::mma_f16_ts(d, p + 8 * j, bl, id_o, 1u);
+                        tc::mma_f16_ts(d, p + 32 + 8 * j, bh, id_o, 1u);
                     }
-                    if (did) {
-                        t0 = global_ns();
-                    } else if (*(volatile int *)&sm.abort) {
-                        go = false;
-                    } else if (global_ns() - t0 > 1000000000ull) {
-                        raise_error(a.err, kDevTimeout);
-                        *(volatile int *)&sm.abort = 1;
-                        go = false;
-                    }
-                }
+                    tc::commit(&sm.o_full[buf]);
+                    return true;
+                };
+                using B0 = std::integral_constant<int, 0>;
+                using B1 = std::integral_constant<int, 1>;
+                auto scores = [&](int it) {  // S of a tile
+                    const int gi = done + it;
+                    return (gi & 1) ? scores_in(B1{}, gi) : scores_in(B0{}, gi);
+                };
+                auto values = [&](int it) {  // O of a tile
+                    const int gi = done + it;
+                    return (gi & 1) ? values_in(B1{}, gi) : values_in(B0{}, gi);
+                };
+                // S is two tiles ahead of O at most (two buffers): the softmax of a tile runs
+                // beside the products of the tiles around it
+                bool go = arrived(&sm.q_full, turn) && scores(0) && (ntiles < 2 || scores(1));
+                for (int it = 0; go && it < ntiles; it++) go = values(it) && (it + 2 >= ntiles || scores(it + 2));
             }
             __syncwarp();
-        }
-        done += ntiles;
-        tc::fence_before_sync();
-        __syncthreads();  // operands and tensor memory are free for the next row tile
-        tc::fence_after_sync();
-        if (sm.abort) break;
+        });
     }
     __syncthreads();
     if (warp == 0) tc::tmem_dealloc(tmem, kTmemCols);
