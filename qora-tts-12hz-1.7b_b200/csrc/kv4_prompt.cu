@@ -110,6 +110,28 @@ __device__ __forceinline__ bool wait_for(uint64_t *bar, uint32_t parity, int *ab
     return __all_sync(0xffffffffu, wait_one(bar, parity, abort, err));
 }
 
+// Two f32 at a time.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    uint64_t r;
+    asm("{\n .reg .b64 a, b, c;\n mov.b64 a, {%1, %2};\n mov.b64 b, {%3, %4};\n mov.b64 c, {%5, %6};\n"
+        " fma.rn.f32x2 %0, a, b, c;\n}"
+        : "=l"(r)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return *reinterpret_cast<float2 *>(&r);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    uint64_t r;
+    asm("{\n .reg .b64 a, b;\n mov.b64 a, {%1, %2};\n mov.b64 b, {%3, %4};\n add.rn.f32x2 %0, a, b;\n}"
+        : "=l"(r)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return *reinterpret_cast<float2 *>(&r);
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
 template <uint32_t Mask>
 __device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t magic) {
     uint32_t r;
@@ -426,21 +448,30 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const PromptArgs a) 
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sm.q_full);
             }
-            float m = -INFINITY, l = 0.0f, corr = 0.0f, unv = 0.0f;
+            float m = -INFINITY, corr = 0.0f, unv = 0.0f;
+            float2 l = make_float2(0.0f, 0.0f);
             float o[D / 2];
 #pragma unroll
             for (int i = 0; i < D / 2; i++) o[i] = 0.0f;
             // adds O of tile `it` (which the products have finished)
             auto fold = [&](int it) {
                 const int gi = done + it;
+                const bool grown = __any_sync(0xffffffffu, corr != 1.0f);
                 wait_for(&sm.o_full[gi & 1], (gi >> 1) & 1, &sm.abort, a.err);
                 tc::fence_after_sync();
 #pragma unroll
                 for (int p = 0; p < D / 64; p++) {
                     float u[32];
                     tc::ld_32x32b_x32(t_lane + kColO + (D / 2) * hs + 32 * p, u);
+                    if (grown)
 #pragma unroll
-                    for (int i = 0; i < 32; i++) o[32 * p + i] = fmaf(u[i], unv, o[32 * p + i] * corr);
+                        for (int i = 0; i < 32; i++) o[32 * p + i] *= corr;
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) {
+                        const float2 s = fma2(make_float2(u[i], u[i + 1]), make_float2(unv, unv),
+                                              make_float2(o[32 * p + i], o[32 * p + i + 1]));
+                        o[32 * p + i] = s.x, o[32 * p + i + 1] = s.y;
+                    }
                 }
                 tc::fence_before_sync();
                 __syncwarp();
@@ -468,21 +499,28 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const PromptArgs a) 
                     for (int i = 0; i < 32; i++)
                         if (32 * hs + i > left) x[i] = -INFINITY;
                 }
-                float top = -INFINITY;
+                float top = max3(x[0], x[1], x[2]), top1 = max3(x[3], x[4], x[5]);
 #pragma unroll
-                for (int i = 0; i < 32; i++) top = fmaxf(top, x[i]);
+                for (int i = 6; i < 30; i += 4) top = max3(top, x[i], x[i + 1]), top1 = max3(top1, x[i + 2], x[i + 3]);
+                top = max3(top, x[30], fmaxf(top1, x[31]));
                 sm.top[buf][hs][r] = top;
                 asm volatile("bar.sync %0, 64;" ::"r"(3 + (warp & 3)) : "memory");  // the row's two warps
+                // The reference of the exponentials follows the running maximum only where
+                // that has passed it by 2^7: O is hardly ever rescaled.  P is up to 2^8 too
+                // large, 2^15 with that, and so is its sum.
                 const float to = fmaxf(m, fmaxf(top, sm.top[buf][hs ^ 1][r]) * f);
-                // P is 2^8 too large, and so is its sum
-                const float ref = to == -INFINITY ? 0.0f : to - 8.0f;
-                const float corr_now = ex2(m - (to == -INFINITY ? 0.0f : to));
-                m = to;
-                l *= corr_now;
+                float corr_now = 1.0f;
+                if (to > m + 7.0f) {
+                    corr_now = ex2(m - to);
+                    m = to;
+                    l.x *= corr_now, l.y *= corr_now;
+                }
+                const float ref = m == -INFINITY ? 0.0f : m - 8.0f;
 #pragma unroll
-                for (int i = 0; i < 32; i++) {
-                    x[i] = ex2(fmaf(x[i], f, -ref));
-                    l += x[i];
+                for (int i = 0; i < 32; i += 2) {
+                    const float2 z = fma2(make_float2(x[i], x[i + 1]), make_float2(f, f), make_float2(-ref, -ref));
+                    x[i] = ex2(z.x), x[i + 1] = ex2(z.y);
+                    l = add2(l, make_float2(x[i], x[i + 1]));
                 }
                 uint32_t hi[16], lo[16];
 #pragma unroll
@@ -490,7 +528,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const PromptArgs a) 
                     const int at = 8 * (p & 3) + 2 * (p >> 2);
                     const __half2 w = __floats2half2_rn(x[at], x[at + 1]);
                     hi[p] = h2u(w);
-                    lo[p] = h2u(__floats2half2_rn(x[at] - __low2float(w), x[at + 1] - __high2float(w)));
+                    const float2 rest = fma2(__half22float2(w), make_float2(-1.0f, -1.0f), make_float2(x[at], x[at + 1]));
+                    lo[p] = h2u(__floats2half2_rn(rest.x, rest.y));
                 }
                 tc::st_32x32b_x16(t_lane + kColP + 64 * buf + 16 * hs, hi);
                 tc::st_32x32b_x16(t_lane + kColP + 64 * buf + 32 + 16 * hs, lo);
@@ -516,7 +555,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const PromptArgs a) 
                 }
             }
             fold(ntiles - 1);
-            sm.l[hs][r] = l;
+            sm.l[hs][r] = l.x + l.y;
             asm volatile("bar.sync 1, 256;" ::: "memory");
             if (r < rows) {
                 const float sum = sm.l[0][r] + sm.l[1][r];
