@@ -63,6 +63,9 @@ struct Sm {
     static constexpr int kV = (D / 8) * (kKeys / 8) * kVStep;
     alignas(128) uint8_t k[2][2][kK];      // [buffer][high, low]
     alignas(128) uint8_t v[2][2][kV];
+    // a softmax warp's halves of rows on their way in and out, 16 bytes at a time (place of
+    // piece c of row r: c ^ r, so that rows and columns of pieces both fall on distinct banks)
+    float4 stage[kSoftWarps][32][D / 8];
     float l[2][kRows], top[2][2][kRows];   // a row's sum, and largest score, by half
     // of a tile (four deep: unpacking is up to three tiles ahead of the softmax)
     float unk[4], unv[4];                  // its scales back
@@ -407,19 +410,34 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const PromptArgs a) 
             const int hs = warp >> 2, r = 32 * (warp & 3) + lane;
             const uint32_t t_lane = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
             const int limit = r < rows ? len + (row0 + r) / G : -1;
+            constexpr int kPieces = D / 8;
+            const int place = r < rows ? (row0 + r) / G * a.heads + (row0 + r) % G : -1;  // of the row, in heads
             // ---- the row's queries: a power of two, then high and low halves; a thread has
             // half of the dimensions, in the order in which a key's words give them
             float rs;
             {
                 constexpr int H = D / 2;
                 float x[H], most = 0.0f;
-                const float4 *src = reinterpret_cast<const float4 *>(
-                    q + ((int64_t)((row0 + r) / G) * a.heads + (row0 + r) % G) * D + H * hs);
+                // (a thread that reads its own row takes one line of 128 bytes for every 16 bytes)
 #pragma unroll
-                for (int i = 0; i < H / 4; i++) {
-                    const float4 u = r < rows ? __ldg(src + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int i = 0; i < kPieces; i++) {
+                    const int rr = (32 * i + lane) / kPieces, c = (32 * i + lane) % kPieces;
+                    const int at = __shfl_sync(0xffffffffu, place, rr);
+                    const float4 u = at >= 0 ? __ldg(reinterpret_cast<const float4 *>(q + (int64_t)at * D + H * hs) + c)
+                                             : make_float4(0.f, 0.f, 0.f, 0.f);
                     x[4 * i] = u.x, x[4 * i + 1] = u.y, x[4 * i + 2] = u.z, x[4 * i + 3] = u.w;
-                    most = fmaxf(fmaxf(most, fmaxf(fabsf(u.x), fabsf(u.y))), fmaxf(fabsf(u.z), fabsf(u.w)));
+                }
+#pragma unroll
+                for (int i = 0; i < kPieces; i++) {
+                    const int rr = (32 * i + lane) / kPieces, c = (32 * i + lane) % kPieces;
+                    sm.stage[warp][rr][c ^ (rr % kPieces)] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+                }
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < kPieces; i++) {
+                    const float4 u = sm.stage[warp][lane][i ^ (lane % kPieces)];
+                    x[4 * i] = u.x, x[4 * i + 1] = u.y, x[4 * i + 2] = u.z, x[4 * i + 3] = u.w;
+                    most = fmaxf(max3(most, fabsf(u.x), fabsf(u.y)), fmaxf(fabsf(u.z), fabsf(u.w)));
                 }
                 sm.top[0][hs][r] = most;
                 asm volatile("bar.sync 1, 256;" ::: "memory");
@@ -557,15 +575,20 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const PromptArgs a) 
             fold(ntiles - 1);
             sm.l[hs][r] = l.x + l.y;
             asm volatile("bar.sync 1, 256;" ::: "memory");
-            if (r < rows) {
-                const float sum = sm.l[0][r] + sm.l[1][r];
-                float *dst = a.out + ((int64_t)(off + (row0 + r) / G) * a.heads + h * G + (row0 + r) % G) * D + (D / 2) * hs;
+            const float inv = __fdiv_rn(1.0f, sm.l[0][r] + sm.l[1][r]);
 #pragma unroll
-                for (int i = 0; i < D / 2; i += 4)
-                    *reinterpret_cast<float4 *>(dst + i) =
-                        make_float4(__fdiv_rn(o[i], sum), __fdiv_rn(o[i + 1], sum), __fdiv_rn(o[i + 2], sum),
-                                    __fdiv_rn(o[i + 3], sum));
+            for (int i = 0; i < kPieces; i++)
+                sm.stage[warp][lane][i ^ (lane % kPieces)] =
+                    make_float4(o[4 * i] * inv, o[4 * i + 1] * inv, o[4 * i + 2] * inv, o[4 * i + 3] * inv);
+            __syncwarp();
+            float *dst = a.out + ((int64_t)off * a.heads + h * G) * D + (D / 2) * hs;
+#pragma unroll
+            for (int i = 0; i < kPieces; i++) {
+                const int rr = (32 * i + lane) / kPieces, c = (32 * i + lane) % kPieces;
+                const int at = __shfl_sync(0xffffffffu, place, rr);
+                if (at >= 0) reinterpret_cast<float4 *>(dst + (int64_t)at * D)[c] = sm.stage[warp][rr][c ^ (rr % kPieces)];
             }
+            __syncwarp();
         });
     } else if (warp < kSoftWarps + kUnpackWarps) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kUnpackRegs));
