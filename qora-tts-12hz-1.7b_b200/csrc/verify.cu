@@ -110,16 +110,15 @@ __device__ double block_scan_f64(double v, double *wsum, double &total) {
     return before + x - v;
 }
 
-// The bin (or digit) of a histogram of the whole row in which the count from
-// its start reaches `need`: hist bins are summed over the cluster's blocks.
+// The digit of a histogram of the whole row in which the count from the largest
+// down reaches `need`: hist bins are summed over the cluster's blocks.
 // Called by warp 0 of every block; writes sel_bin / sel_below / sel_in.
-template <bool DESC>
 __device__ __forceinline__ void select_bin(cg::cluster_group &cl, ProbsSmem *sm, int bins, unsigned need) {
     const int lane = threadIdx.x & 31;
     const unsigned nr = cl.num_blocks();
     unsigned below = 0;
     for (int b0 = 0; b0 < bins; b0 += 32) {
-        const int bin = DESC ? bins - 1 - (b0 + lane) : b0 + lane;
+        const int bin = bins - 1 - (b0 + lane);
         unsigned c = 0;
 #pragma unroll
         for (unsigned r = 0; r < kMaxCluster; r++)  // (reads in flight together)
@@ -141,6 +140,45 @@ __device__ __forceinline__ void select_bin(cg::cluster_group &cl, ProbsSmem *sm,
         }
         below += __shfl_sync(0xffffffffu, x, 31);
     }
+}
+
+// Sorts list[0 .. found), found <= E kVThreads <= kCand, by a bitonic network: a thread
+// has E neighbours, so partners up to 32 E apart are in the thread or the warp, and
+// 4 of the 9 (2: 10, 4: 11) distances go through shared memory.
+template <int E>
+__device__ __noinline__ void sort_descending(unsigned long long *list, unsigned found) {
+    const int tid = threadIdx.x;
+    unsigned long long v[E];
+#pragma unroll
+    for (int e = 0; e < E; e++) v[e] = tid * E + e < (int)found ? list[tid * E + e] : 0ull;
+    for (int span = 2; span <= E * kVThreads; span <<= 1)
+        for (int step = span >> 1; step > 0; step >>= 1) {
+            unsigned long long w[E];
+            if (step < E) {
+#pragma unroll
+                for (int e = 0; e < E; e++) w[e] = step == 1 ? v[e ^ (E > 1)] : v[e ^ (E > 2 ? 2 : 0)];
+            } else if (step < 32 * E) {
+#pragma unroll
+                for (int e = 0; e < E; e++) w[e] = __shfl_xor_sync(0xffffffffu, v[e], step / E);
+            } else {
+                __syncthreads();
+#pragma unroll
+                for (int e = 0; e < E; e++) list[tid * E + e] = v[e];
+                __syncthreads();
+#pragma unroll
+                for (int e = 0; e < E; e++) w[e] = list[(tid * E + e) ^ step];
+            }
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                const int i = tid * E + e;
+                const bool larger = ((i & step) == 0) == ((i & span) == 0);
+                if ((w[e] > v[e]) == larger) v[e] = w[e];
+            }
+        }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < E; e++) list[tid * E + e] = v[e];
+    __syncthreads();
 }
 
 // VEC: rows and slices are multiples of 16 bytes.
@@ -267,12 +305,27 @@ __global__ void __launch_bounds__(kVThreads) k_sample_probs(const ProbsArgs a) {
         return;
     }
     if (!topk) {
-        double s = 0.0;
+        // exp((x - max) / T) in 32 bits: the product with 1 / T keeps its rounding error
+        // (and 1 / T's), which enters as e^z (1 + error).  Sums of four go into a 64-bit
+        // sum.  (All in 64 bits took 49 us for 92 rows of 151936, against 46, most of it waiting.)
         const double per = 1.0 / temp;
-        for (int i = tid; i < n; i += kVThreads) {
-            const float e = expf((float)(((double)x[i] - (double)mx) * per));
-            x[i] = e;
-            s += e;
+        const float per_hi = (float)fmin(per, 3.4e38), per_lo = per < 3.4e38 ? (float)(per - (double)per_hi) : 0.0f;
+        auto weight = [&](float v) {
+            const float d = v - mx, z = d * per_hi;
+            const float e = expf(z);
+            return fmaf(e, fmaxf(fmaf(d, per_hi, -z) + d * per_lo, -1.0f), e);  // (d = -inf: NaN to -1, e = 0)
+        };
+        double s = 0.0;
+        if constexpr (VEC) {
+            float4 *x4 = reinterpret_cast<float4 *>(x);
+            for (int i = tid; i < n / 4; i += kVThreads) {
+                float4 v = x4[i];
+                v.x = weight(v.x), v.y = weight(v.y), v.z = weight(v.z), v.w = weight(v.w);
+                x4[i] = v;
+                s += (double)((v.x + v.y) + (v.z + v.w));
+            }
+        } else {
+            for (int i = tid; i < n; i += kVThreads) s += (double)(x[i] = weight(x[i]));
         }
         s = block_sum_f64(s, sm->wsum);
         if (tid == 0) sm->slice_sum = s;
@@ -283,8 +336,16 @@ __global__ void __launch_bounds__(kVThreads) k_sample_probs(const ProbsArgs a) {
             sm->sum = 1.0 / t;
         }
         __syncthreads();
-        const double inv = sm->sum;
-        for (int i = tid; i < n; i += kVThreads) out[i] = (float)(x[i] * inv);
+        const float inv = (float)sm->sum;
+        if constexpr (VEC) {
+            const float4 *x4 = reinterpret_cast<const float4 *>(x);
+            for (int i = tid; i < n / 4; i += kVThreads) {
+                const float4 v = x4[i];
+                __stcs(reinterpret_cast<float4 *>(out) + i, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+            }
+        } else {
+            for (int i = tid; i < n; i += kVThreads) out[i] = x[i] * inv;
+        }
         meet();
         return;
     }
@@ -324,10 +385,10 @@ __global__ void __launch_bounds__(kVThreads) k_sample_probs(const ProbsArgs a) {
         sel = sm->sel_bin;
     }
     ProbsSmem *lead = cl.map_shared_rank(sm, 0);
+    auto candidate = [&](int i) { return ((unsigned long long)order_key(x[i]) << 32) | (unsigned)~(unsigned)(v0 + i); };
     auto offer = [&](int i) {
         const unsigned at = atomicAdd(&lead->n_cand, 1u);
-        if (at < kCand)
-            lead->cand[at] = ((unsigned long long)order_key(x[i]) << 32) | (unsigned)~(unsigned)(v0 + i);
+        if (at < kCand) lead->cand[at] = candidate(i);
     };
     if (few) {
         each([&](int i, float v) {
@@ -336,7 +397,11 @@ __global__ void __launch_bounds__(kVThreads) k_sample_probs(const ProbsArgs a) {
         meet();
         few = lead->n_cand <= kCand;
     }
-    if (!few) {
+    if (!few && a.V <= kCand) {  // (one block) every logit is one
+        for (int i = tid; i < n; i += kVThreads) sm->cand[i] = candidate(i);
+        if (tid == 0) sm->n_cand = n;
+        __syncthreads();
+    } else if (!few) {
         meet();  // (every block has seen the count)
         if (tid == 0) sm->n_cand = 0;
         meet();
@@ -350,7 +415,7 @@ __global__ void __launch_bounds__(kVThreads) k_sample_probs(const ProbsArgs a) {
                 if ((key & mask) == prefix) atomicAdd(&sm->hist[(key >> shift) & 255u], 1u);
             }
             meet();
-            if (warp == 0) select_bin<true>(cl, sm, 256, need);
+            if (warp == 0) select_bin(cl, sm, 256, need);
             __syncthreads();
             prefix |= sm->sel_bin << shift;
             mask |= 255u << shift;
@@ -384,7 +449,6 @@ __global__ void __launch_bounds__(kVThreads) k_sample_probs(const ProbsArgs a) {
     if (nr > 1) cl.sync();  // (no block leaves before its count is read)
     if (rank != 0) return;  // the rest is the leader's; it reads no other block's memory
     const unsigned found = min(sm->n_cand, (unsigned)kCand);
-    const int size = found <= 256 ? 256 : kCand;
     if (found <= 256) {  // few: each counts those before it
         unsigned long long mine = 0;
         unsigned at = 0;
@@ -396,26 +460,19 @@ __global__ void __launch_bounds__(kVThreads) k_sample_probs(const ProbsArgs a) {
         __syncthreads();
         if (tid < (int)found) sm->cand[at] = mine;
         __syncthreads();
-    } else {  // descending bitonic sort
-        for (int i = found + tid; i < size; i += kVThreads) sm->cand[i] = 0ull;
-        __syncthreads();
-        for (int span = 2; span <= size; span <<= 1)
-            for (int step = span >> 1; step > 0; step >>= 1) {
-                for (int i = tid; i < size / 2; i += kVThreads) {
-                    const int lo = (i / step) * step * 2 + (i % step), hi = lo + step;
-                    const unsigned long long p = sm->cand[lo], q = sm->cand[hi];
-                    const bool down = (lo & span) == 0;
-                    if ((p < q) == down) sm->cand[lo] = q, sm->cand[hi] = p;
-                }
-                __syncthreads();
-            }
+    } else if (found <= kVThreads) {
+        sort_descending<1>(sm->cand, found);
+    } else if (found <= 2 * kVThreads) {
+        sort_descending<2>(sm->cand, found);
+    } else {
+        sort_descending<4>(sm->cand, found);
     }
     // k <= kMaxSurvivors = 2 kVThreads: thread i has ranks 2i and 2i + 1
     double e[2];
 #pragma unroll
     for (int j = 0; j < 2; j++) {
         const unsigned r = 2 * tid + j;
-        e[j] = r < k ? exp(((double)order_value((unsigned)(sm->cand[min(r, (unsigned)size - 1)] >> 32)) - (double)mx) / temp) : 0.0;
+        e[j] = r < k ? exp(((double)order_value((unsigned)(sm->cand[min(r, found - 1)] >> 32)) - (double)mx) / temp) : 0.0;
     }
     double total;
     const double before = block_scan_f64(e[0] + e[1], sm->wsum, total);
