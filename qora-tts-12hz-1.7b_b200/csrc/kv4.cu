@@ -27,7 +27,9 @@ namespace {
 // all warps, 256 entries at a time with eight loads in flight; each block then
 // joins its share of the bit maps through distributed shared memory and hands
 // out the free pages in it; tokens are spread over all threads, which look
-// their stream up in the scanned offsets.
+// their stream up in the scanned offsets.  What bounds it is latency: 512 streams
+// of up to 16000 positions in pages of 64 take 17 us, 5.5 of them for marking, and
+// 32 streams 5.7 us.  Walking each stream's pages from one block took 336 us.
 constexpr int kResThreads = 1024;
 constexpr int kResCluster = 16;  // (not a portable size; what bounds the large case is marking, a block's share of it)
 constexpr int kResChunk = 128;  // table entries of one stream that a warp marks at a time,
@@ -488,6 +490,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 6) k_kv4_append(const RowArgs 
 }
 
 // Rows of keys and values as they are (READ: back to f32), 256 / D heads a warp.
+// Bound by memory: reading 8191 rows of 8 heads of 128 takes 13.5 us, 5.7 TB/s.
 template <int D, bool READ>
 __global__ void __launch_bounds__(kRowWarps * 32) k_kv4_rows(const RowArgs a) {
     constexpr int HW = 256 / D;

@@ -26,6 +26,12 @@
 // through the middle of items.  Partial (max, sum, weighted sum) of an item that
 // several blocks share meet in distributed shared memory, in block order, so
 // there is no workspace and the result does not depend on timing.
+//
+// One token of 32 streams of 4096 positions, 16 / 8 heads of 128: 45 us, 3.4 TB/s
+// of cache read (of 16384: 5.4 TB/s).  A launch costs some 8 us besides the units:
+// lengths, tables, first copies and the join, one after the other.  The units are
+// bound by instructions: some 780 for 32 positions at a tile of 4 rows, issued in
+// 60 % of the cycles at 16 warps a multiprocessor, as many as registers allow.
 #include <cooperative_groups.h>
 
 #include "kv4.cuh"
