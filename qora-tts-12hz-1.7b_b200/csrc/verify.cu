@@ -145,6 +145,14 @@ __device__ __forceinline__ void select_bin(cg::cluster_group &cl, ProbsSmem *sm,
     }
 }
 
+// The two halves of a cluster barrier, by every thread.
+__device__ __forceinline__ void cluster_arrive() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 // Sorts list[0 .. found), found <= E kVThreads <= kCand, by a bitonic network: a thread
 // has E neighbours, so partners up to 32 E apart are in the thread or the warp, and
 // 4 of the 9 (2: 10, 4: 11) distances go through shared memory.
@@ -340,6 +348,7 @@ __global__ void __launch_bounds__(kVThreads) k_sample_probs(const ProbsArgs a) {
         }
         __syncthreads();
         const float inv = (float)sm->sum;
+        if (nr > 1) cluster_arrive();  // (the sums have been read; before the stores, which it would wait for)
         if constexpr (VEC) {
             const float4 *x4 = reinterpret_cast<const float4 *>(x);
             for (int i = tid; i < n / 4; i += kVThreads) {
@@ -349,15 +358,10 @@ __global__ void __launch_bounds__(kVThreads) k_sample_probs(const ProbsArgs a) {
         } else {
             for (int i = tid; i < n; i += kVThreads) out[i] = x[i] * inv;
         }
-        meet();
+        if (nr > 1) cluster_wait();
         return;
     }
     const unsigned k = a.params.top_k;
-    if constexpr (VEC) {
-        for (int i = tid; i < n / 4; i += kVThreads) reinterpret_cast<float4 *>(out)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    } else {
-        for (int i = tid; i < n; i += kVThreads) out[i] = 0.0f;
-    }
     const float per_bin = mx > mn ? (float)(kBins - 1) / (mx - mn) : 0.0f;
     auto bin_of = [&](float v) { return (int)fminf((mx - v) * per_bin, (float)(kBins - 1)); };
     bool few = a.by_maxima;
@@ -449,8 +453,22 @@ __global__ void __launch_bounds__(kVThreads) k_sample_probs(const ProbsArgs a) {
         }
         meet();
     }
-    if (nr > 1) cl.sync();  // (no block leaves before its count is read)
-    if (rank != 0) return;  // the rest is the leader's; it reads no other block's memory
+    // The zeros of the row go out here, beside the leader's sort: a cluster barrier
+    // waits for the stores before it.  The leader's own arrival does not wait for its
+    // sort, so the other blocks leave as soon as their zeros are written; it reads no
+    // other block's memory from here on.
+    if (nr > 1 && rank == 0) cluster_arrive();
+    if constexpr (VEC) {
+        for (int i = tid; i < n / 4; i += kVThreads) reinterpret_cast<float4 *>(out)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    } else {
+        for (int i = tid; i < n; i += kVThreads) out[i] = 0.0f;
+    }
+    if (nr > 1 && rank != 0) {
+        cluster_arrive();
+        cluster_wait();
+        return;
+    }
+    __syncthreads();
     const unsigned found = min(sm->n_cand, (unsigned)kCand);
     if (found <= 256) {  // few: each counts those before it
         unsigned long long mine = 0;
@@ -485,6 +503,7 @@ __global__ void __launch_bounds__(kVThreads) k_sample_probs(const ProbsArgs a) {
         stay[1] = (before + e[0]) / total < (double)a.params.top_p;
         total = block_sum_f64((stay[0] ? e[0] : 0.0) + (stay[1] ? e[1] : 0.0), sm->wsum);
     }
+    if (nr > 1) cluster_wait();  // the other blocks' zeros are written
 #pragma unroll
     for (int j = 0; j < 2; j++) {
         const unsigned r = 2 * tid + j;
