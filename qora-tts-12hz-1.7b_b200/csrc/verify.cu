@@ -398,8 +398,10 @@ __global__ void __launch_bounds__(kVThreads) k_sample_probs(const ProbsArgs a) {
         if (at < kCand) lead->cand[at] = candidate(i);
     };
     if (few) {
+        // bin_of(v) <= sel, without a conversion for every logit
+        const float below = (float)(sel + 1);
         each([&](int i, float v) {
-            if (bin_of(v) <= sel) offer(i);
+            if (sel == kBins - 1 || (mx - v) * per_bin < below) offer(i);
         });
         meet();
         few = lead->n_cand <= kCand;
