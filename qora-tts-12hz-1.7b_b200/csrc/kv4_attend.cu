@@ -317,6 +317,14 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_attend(const AttendArgs a) 
         Piece<R> p;
         p.locate(a, G, b, w - sm.start[b], w1 - w, warp);
         h = p.h, u0 = p.u0, mine = p.mine;
+        {  // the queries are on their way to the first level while the table is read
+            const int row = p.qt * R + lane / (32 / R);
+            if (row < p.s.n * G) {
+                const float *q = a.q + ((int64_t)(p.s.off + row / G) * a.heads + h * G + row % G) * D;
+                const int line = lane % (32 / R);
+                if (line < D / 32 && warp == 0) asm volatile("prefetch.global.L1 [%0];" ::"l"(q + line * 32));
+            }
+        }
         fetch_units(0);
         if (!dead)
             for (int k = 0; k < ST && k < mine; k++) issue(k);
@@ -594,21 +602,23 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_attend(const AttendArgs a) 
         const Shared e = sm.open;
         for (int i = tid; i < e.rows * D; i += kThreads) {
             const int r = i / D, d = i % D;
-            float pm[kMaxCluster], mx = sm.pm[1][r];
+            float pm[kMaxCluster], po[kMaxCluster], pl[kMaxCluster];  // (all reads in flight together)
+            pm[0] = sm.pm[1][r], po[0] = sm.po[1][r][d], pl[0] = sm.pl[1][r];
 #pragma unroll
             for (int x = 1; x < kMaxCluster; x++) {
-                pm[x] = rank + x <= e.last ? cl.map_shared_rank(&sm, rank + x)->pm[0][r] : -INFINITY;
-                mx = fmaxf(mx, pm[x]);
+                const Sm *q = cl.map_shared_rank(&sm, rank + x <= e.last ? rank + x : rank);
+                pm[x] = rank + x <= e.last ? q->pm[0][r] : -INFINITY;
+                po[x] = rank + x <= e.last ? q->po[0][r][d] : 0.0f;
+                pl[x] = rank + x <= e.last ? q->pl[0][r] : 0.0f;
             }
-            const float f0 = ex2(sm.pm[1][r] - mx);
-            float o = f0 * sm.po[1][r][d], sum = f0 * sm.pl[1][r];
+            float mx = pm[0], o = 0.0f, sum = 0.0f;
 #pragma unroll
-            for (int x = 1; x < kMaxCluster; x++) {
-                if (rank + x > e.last) break;
-                const Sm *q = cl.map_shared_rank(&sm, rank + x);
+            for (int x = 1; x < kMaxCluster; x++) mx = fmaxf(mx, pm[x]);
+#pragma unroll
+            for (int x = 0; x < kMaxCluster; x++) {
                 const float f = ex2(pm[x] - mx);
-                o = fmaf(f, q->po[0][r][d], o);
-                sum = fmaf(f, q->pl[0][r], sum);
+                o = fmaf(f, po[x], o);
+                sum = fmaf(f, pl[x], sum);
             }
             const int row = e.qt * R + r;
             a.out[((int64_t)(e.off + row / G) * a.heads + e.h * G + row % G) * D + d] = __fdiv_rn(o, sum);
