@@ -45,6 +45,7 @@ namespace {
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
 constexpr int kMaxCluster = 8;  // blocks of a cluster
+constexpr int kStages = 2;      // units of a warp in flight or in use
 
 struct AttendArgs {
     Kv4Layer L;
@@ -184,26 +185,26 @@ struct Piece {
     }
 };
 
-template <int D, int NT, int ST>
+template <int D, int NT>
 struct Smem {
     static constexpr int R = 4 * NT;
     static constexpr int kRow = D + 8;  // a quarter-warp's 16-byte stores fall on distinct banks
-    alignas(128) uint8_t ring[kWarps][ST][kv4_unit_bytes(D)];
-    float wo[kWarps][R][kRow];
-    float wm[kWarps][R], wl[kWarps][R];
+    alignas(128) uint8_t ring[kWarps][kStages][kv4_unit_bytes(D)];
+    float wo[kWarps][4][kRow];  // warps' sums, four rows at a time
+    float wm[kWarps][4], wl[kWarps][4];
     float po[2][R][D];       // partials: [0] of the item that a block before began, [1] of the one begun here
     float pm[2][R], pl[2][R];
     uint2 qf[NT][D / 16][NT > 1 ? 32 : 1];  // query fragments, by lane
     float rs[R];                                            // and their scales back
-    uint64_t full[kWarps][ST];
+    uint64_t full[kWarps][kStages];
     int64_t scan[kWarps];
     Shared open;
     int64_t start[1];  // [streams + 1] first unit of each stream in the work line
 };
 
-template <int D, int NT, int ST>
+template <int D, int NT>
 __global__ void __launch_bounds__(kThreads, 2) k_kv4_attend(const AttendArgs a) {
-    using Sm = Smem<D, NT, ST>;
+    using Sm = Smem<D, NT>;
     using U = Kv4Unit<D>;
     constexpr int R = Sm::R, C = D / 32;
     extern __shared__ uint4 dyn[];
@@ -213,7 +214,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_attend(const AttendArgs a) 
     const int G = a.heads / a.L.kvh;
     if (tid == 0) {
         for (int w = 0; w < kWarps; w++)
-            for (int s = 0; s < ST; s++) mbar_init(&sm.full[w][s], 1);
+            for (int s = 0; s < kStages; s++) mbar_init(&sm.full[w][s], 1);
         mbar_fence_init();
     }
     griddep_launch_dependents();
@@ -307,7 +308,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_attend(const AttendArgs a) 
         const uint8_t *from = reinterpret_cast<const uint8_t *>(
             __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), k & 31));
         if (lane == 0) {
-            const int st = (turn + k) % ST;
+            const int st = (turn + k) % kStages;
             mbar_arrive_expect_tx(&sm.full[warp][st], U::kBytes);
             bulk_g2s(&sm.ring[warp][st][0], from, U::kBytes, &sm.full[warp][st]);
         }
@@ -327,7 +328,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_attend(const AttendArgs a) 
         }
         fetch_units(0);
         if (!dead)
-            for (int k = 0; k < ST && k < mine; k++) issue(k);
+            for (int k = 0; k < kStages && k < mine; k++) issue(k);
     };
     if (w < w1) begin();
     while (w < w1) {
@@ -404,8 +405,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_attend(const AttendArgs a) 
 
         for (int k = 0; k < mine && !dead; k++) {
             const int u = u0 + warp + k * kWarps;
-            const int st = (turn + k) % ST;
-            const bool here = mbar_wait_bounded(&sm.full[warp][st], ((turn + k) / ST) & 1, a.err);
+            const int st = (turn + k) % kStages;
+            const bool here = mbar_wait_bounded(&sm.full[warp][st], ((turn + k) / kStages) & 1, a.err);
             if (__any_sync(0xffffffffu, !here)) {
                 dead = true;
                 break;
@@ -534,9 +535,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_attend(const AttendArgs a) 
                 }
             }
             __syncwarp();  // the stage is read
-            if (k + ST < mine) {
-                if (((k + ST) & 31) == 0) fetch_units(k + ST);
-                issue(k + ST);
+            if (k + kStages < mine) {
+                if (((k + kStages) & 31) == 0) fetch_units(k + kStages);
+                issue(k + kStages);
             }
         }
         turn += mine;
@@ -547,47 +548,51 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_attend(const AttendArgs a) 
         const bool more = w < w1;
         if (more) begin();
 
-        // ---- join the warps
+        // ---- join the warps, four rows at a time
         const float unlift = __int_as_float((127 - ke) << 23);
+        const bool whole = p.u0 == 0 && p.u1 == p.s.ub;
+        const int part = p.u0 == 0;
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) l[nt] += __shfl_xor_sync(0xffffffffu, l[nt], o);
+            if (nt > 0) {
+                if (nt * 4 >= p.rows) break;
+                __syncthreads();
+            }
             if (g == 0) {
-                sm.wm[warp][nt * 4 + t] = m[nt];
-                sm.wl[warp][nt * 4 + t] = l[nt];
+                sm.wm[warp][t] = m[nt];
+                sm.wl[warp][t] = l[nt];
             }
             if (nt * 4 + t < p.rows)
 #pragma unroll
                 for (int c = 0; c < C; c++)
-                    *reinterpret_cast<float4 *>(&sm.wo[warp][nt * 4 + t][32 * c + 4 * g]) =
+                    *reinterpret_cast<float4 *>(&sm.wo[warp][t][32 * c + 4 * g]) =
                         make_float4(acc[nt][c][0] * unlift, acc[nt][c][1] * unlift, acc[nt][c][2] * unlift,
                                     acc[nt][c][3] * unlift);
-        }
-        __syncthreads();
-        const bool whole = p.u0 == 0 && p.u1 == p.s.ub;
-        const int part = p.u0 == 0;
-        for (int i = tid; i < p.rows * D; i += kThreads) {
-            const int r = i / D, d = i % D;
-            float mx = -INFINITY;
+            __syncthreads();
+            for (int i = tid; i < min(4, p.rows - nt * 4) * D; i += kThreads) {
+                const int r4 = i / D, r = nt * 4 + r4, d = i % D;
+                float mx = -INFINITY;
 #pragma unroll
-            for (int x = 0; x < kWarps; x++) mx = fmaxf(mx, sm.wm[x][r]);
-            const float ref = mx == -INFINITY ? 0.0f : mx;
-            float o = 0.0f, sum = 0.0f;
+                for (int x = 0; x < kWarps; x++) mx = fmaxf(mx, sm.wm[x][r4]);
+                const float ref = mx == -INFINITY ? 0.0f : mx;
+                float o = 0.0f, sum = 0.0f;
 #pragma unroll
-            for (int x = 0; x < kWarps; x++) {
-                const float f = ex2(sm.wm[x][r] - ref);
-                o = fmaf(f, sm.wo[x][r][d], o);
-                sum = fmaf(f, sm.wl[x][r], sum);
-            }
-            if (whole) {
-                const int row = p.qt * R + r;
-                a.out[((int64_t)(p.s.off + row / G) * a.heads + p.h * G + row % G) * D + d] = __fdiv_rn(o, sum);
-            } else {
-                sm.po[part][r][d] = o;
-                if (d == 0) {
-                    sm.pm[part][r] = mx;
-                    sm.pl[part][r] = sum;
+                for (int x = 0; x < kWarps; x++) {
+                    const float f = ex2(sm.wm[x][r4] - ref);
+                    o = fmaf(f, sm.wo[x][r4][d], o);
+                    sum = fmaf(f, sm.wl[x][r4], sum);
+                }
+                if (whole) {
+                    const int row = p.qt * R + r;
+                    a.out[((int64_t)(p.s.off + row / G) * a.heads + p.h * G + row % G) * D + d] = __fdiv_rn(o, sum);
+                } else {
+                    sm.po[part][r][d] = o;
+                    if (d == 0) {
+                        sm.pm[part][r] = mx;
+                        sm.pl[part][r] = sum;
+                    }
                 }
             }
         }
@@ -643,16 +648,16 @@ void cluster_config(cudaLaunchConfig_t &cfg, cudaLaunchAttribute &at, int cluste
 
 constexpr int kSizes[3] = {8, 4, 2};  // blocks of a cluster
 
-template <int D, int NT, int ST>
-size_t smem_of(int streams) { return sizeof(Smem<D, NT, ST>) + (size_t)streams * 8; }
+template <int D, int NT>
+size_t smem_of(int streams) { return sizeof(Smem<D, NT>) + (size_t)streams * 8; }
 
 // How many clusters of each size run at once.
-template <int D, int NT, int ST>
+template <int D, int NT>
 int clusters_of(const qora_kv4 *kv, int (&n)[3]) {
-    auto kern = k_kv4_attend<D, NT, ST>;
-    const size_t smem = smem_of<D, NT, ST>(kv->streams);
+    auto kern = k_kv4_attend<D, NT>;
+    const size_t smem = smem_of<D, NT>(kv->streams);
     static std::atomic<uint64_t> done;  // (as much as the most streams need: caches share the kernel)
-    QORA_TRY(allow_smem(kern, smem_of<D, NT, ST>(kKv4MaxStreams), kv->ctx->device, done));
+    QORA_TRY(allow_smem(kern, smem_of<D, NT>(kKv4MaxStreams), kv->ctx->device, done));
     for (int i = 0; i < 3; i++) {
         cudaLaunchConfig_t cfg;
         cudaLaunchAttribute at;
@@ -669,10 +674,10 @@ int clusters_of(const qora_kv4 *kv, int (&n)[3]) {
 // run at once).  Measured at 16 / 8 heads of 128, one token: 1 stream of 16384
 // positions 23.4 us with clusters of 8, 34.2 with 4; 8 streams of 4096 23.1 us with
 // 8, 19.5 with 4, 25.9 with 2; 32 streams of 4096 46.8 us with 8, 43.1 with 2.
-template <int D, int NT, int ST>
+template <int D, int NT>
 int launch(const qora_kv4 *kv, const AttendArgs &a, const int (&n)[3], int64_t items, cudaStream_t st) {
-    auto kern = k_kv4_attend<D, NT, ST>;
-    const size_t smem = smem_of<D, NT, ST>(a.streams);
+    auto kern = k_kv4_attend<D, NT>;
+    const size_t smem = smem_of<D, NT>(a.streams);
     const int i = items <= n[0] ? 0 : items <= n[1] ? 1 : 2;
     return launch_ex(kern, dim3(n[i], kSizes[i]), dim3(kThreads), smem, st, (unsigned)kSizes[i], a);
 }
@@ -682,8 +687,8 @@ int launch(const qora_kv4 *kv, const AttendArgs &a, const int (&n)[3], int64_t i
 namespace {
 template <int D>
 int setup(qora_kv4 *kv) {
-    QORA_TRY((clusters_of<D, 1, 2>(kv, kv->clusters[0])));
-    return clusters_of<D, 2, 1>(kv, kv->clusters[1]);
+    QORA_TRY((clusters_of<D, 1>(kv, kv->clusters[0])));
+    return clusters_of<D, 2>(kv, kv->clusters[1]);
 }
 // Row tiles of 4 or 8.  (Tiles of 12 read the cache once where these read it twice,
 // but do not fit 128 registers: 6 drafts of 16 streams of 4096 took 58 us against 40.)
@@ -692,7 +697,7 @@ int launch_rows(const qora_kv4 *kv, const AttendArgs &a, int64_t rows, cudaStrea
     const int nt = rows <= 4 ? 1 : 2;
     const int64_t items = (int64_t)kv->streams * kv->kvh * ((rows + 4 * nt - 1) / (4 * nt));
     const auto &n = kv->clusters[nt - 1];
-    return nt == 1 ? launch<D, 1, 2>(kv, a, n, items, st) : launch<D, 2, 1>(kv, a, n, items, st);
+    return nt == 1 ? launch<D, 1>(kv, a, n, items, st) : launch<D, 2>(kv, a, n, items, st);
 }
 }  // namespace
 

@@ -510,6 +510,61 @@ def test_captured_step_replays_with_other_lengths(ctx, orc):
     assert _error(ctx) == 0 and list(kv.lengths()) == list(eager.lengths())
 
 
+def test_two_streams_and_a_replayed_graph(ctx):
+    """Prompts on one cache, drafts on another and a captured step of a third, each on
+    a stream of its own at the same time: the bits of one after the other."""
+    import torch
+    shapes = [([70, 0], [150, 200], 64), ([900, 33, 0, 5], [5, 0, 3, 6], 6), ([400] * 9, [1] * 9, 1)]
+    jobs = []
+    for i, (lens, counts, most) in enumerate(shapes):
+        kv, offsets, held, rng = _filled(ctx, lens, counts, 4, 2, 128, 64, 40 + i)
+        q = _dev(rng.standard_normal((sum(counts), 4 * 128)).astype(np.float32))
+        jobs.append((kv, q, offsets, most, kv.attend(1, q, offsets, most), torch.zeros_like(q), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    kv, q, offsets, most, _, out, s = jobs[2]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        for _ in range(3):
+            kv.attend(1, q, offsets, most, out=out)
+    for _ in range(20):
+        for kv, q, offsets, most, want, out, s in jobs[:2]:
+            with torch.cuda.stream(s):
+                kv.attend(1, q, offsets, most, out=out)
+        with torch.cuda.stream(jobs[2][6]):
+            graph.replay()
+    torch.cuda.synchronize()
+    for kv, q, offsets, most, want, out, s in jobs:
+        assert bool((out == want).all())
+    assert _error(ctx) == 0
+
+
+def test_captured_prompt_replays(ctx):
+    """A prompt's attention in a graph reads lengths, offsets and tables at each replay."""
+    import torch
+    lens, counts, heads, kvh, hd = [3, 0], [90, 40], 4, 2, 64
+    kv, offsets, held, rng = _filled(ctx, lens, counts, heads, kvh, hd, 32, 50)
+    q = rng.standard_normal((130, heads, hd)).astype(np.float32)
+    qd, out = _dev(q.reshape(130, -1)), torch.zeros(130, heads * hd, device="cuda")
+    s = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        kv.attend(1, qd, offsets, 90, out=out)
+    for counts in ([90, 40], [17, 40], [0, 1]):
+        held_now = [[x[:n + c] for x in h] for h, n, c in zip(held, lens, counts)]
+        offsets.copy_(_i32([0, counts[0], sum(counts)]))
+        out.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        got, at = out.cpu().numpy(), 0
+        for b, c in enumerate(counts):
+            if c:
+                ref, bound = R.attend(q[at:at + c], *held_now[b], lens[b], heads, kvh)
+                assert np.all(np.abs(got[at:at + c].reshape(c, heads, hd) - ref) <= bound)
+            at += c
+        assert (got[at:] == 7.0).all()
+    assert _error(ctx) == 0
+
+
 def test_long_cache_past_32_bit_offsets(ctx):
     """A pool of more than 2^31 bytes: the stream's pages lie at its end."""
     import torch
