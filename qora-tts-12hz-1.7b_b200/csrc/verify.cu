@@ -35,8 +35,8 @@ constexpr int kMaxCluster = 8;
 // radix selection over the slices decides exactly.  Exponentials and
 // sums of the kept are in 64 bits: the order and the top_p border are decided
 // by values next to each other.
-// 96 rows of 151936 with top_k 50: 58 us, 2.0 TB/s.  Memory is busy 13 % of that:
-// a block lives some 18 us, of which the read is 4 and the rest barriers of the
+// 96 rows of 151936 with top_k 50: 54.5 us, 2.1 TB/s.  Memory is busy 14 % of that:
+// a block lives some 17 us, of which the read is 4 and the rest barriers of the
 // block and the cluster, and shared memory lets 296 of the 768 blocks run at once.
 constexpr int kBins = 256;
 constexpr int kCand = 2048;          // candidates that one sort takes
@@ -362,6 +362,14 @@ __global__ void __launch_bounds__(kVThreads) k_sample_probs(const ProbsArgs a) {
         return;
     }
     const unsigned k = a.params.top_k;
+    auto zeros = [&]() {
+        if constexpr (VEC) {
+            for (int i = tid; i < n / 4; i += kVThreads) reinterpret_cast<float4 *>(out)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        } else {
+            for (int i = tid; i < n; i += kVThreads) out[i] = 0.0f;
+        }
+    };
+    if (nr == 1) zeros();
     const float per_bin = mx > mn ? (float)(kBins - 1) / (mx - mn) : 0.0f;
     auto bin_of = [&](float v) { return (int)fminf((mx - v) * per_bin, (float)(kBins - 1)); };
     bool few = a.by_maxima;
@@ -455,16 +463,12 @@ __global__ void __launch_bounds__(kVThreads) k_sample_probs(const ProbsArgs a) {
         }
         meet();
     }
-    // The zeros of the row go out here, beside the leader's sort: a cluster barrier
+    // A cluster's zeros go out here, beside the leader's sort: a cluster barrier
     // waits for the stores before it.  The leader's own arrival does not wait for its
     // sort, so the other blocks leave as soon as their zeros are written; it reads no
     // other block's memory from here on.
     if (nr > 1 && rank == 0) cluster_arrive();
-    if constexpr (VEC) {
-        for (int i = tid; i < n / 4; i += kVThreads) reinterpret_cast<float4 *>(out)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    } else {
-        for (int i = tid; i < n; i += kVThreads) out[i] = 0.0f;
-    }
+    if (nr > 1) zeros();
     if (nr > 1 && rank != 0) {
         cluster_arrive();
         cluster_wait();
@@ -525,7 +529,7 @@ __global__ void __launch_bounds__(kVThreads) k_sample_probs(const ProbsArgs a) {
 // left), from p_a when all passed.  The products and sums are in 64 bits, so
 // that neither comparison turns on rounding.  Weights that are not positive
 // (NaN among them) count as zero.
-// 64 streams of 5 drafts at 151936: 27 us (one row read where all pass, two where a
+// 64 streams of 5 drafts at 151936: 23.5 us (one row read where all pass, two where a
 // draft is rejected: 58 MB).  What bounds it is the length of the chain (verdicts,
 // sums, search), with one wave of blocks and eight loads of a thread in flight.
 constexpr int kVocabMax = 1 << 30, kDraftsMax = 1 << 20;  // (indexes of a row stay in 32 bits)
