@@ -28,10 +28,10 @@ constexpr int kMaxCluster = 8;
 //   top_p in (0, 1): in that order, a token stays while the probabilities
 //       before it sum to less than top_p; p is divided by the sum of what stays
 // The row's slice stays in shared memory after one read.  The top_k-th largest of
-// the threads' own maxima bounds the top_k-th logit from below: a histogram of
-// the maxima (256 bins between the least and the largest of them) gives a bin
-// that it lies in, and only logits down to that bin are sorted, hardly more than
-// top_k.  Where there are too few maxima, or too many candidates (equal logits), a
+// the maxima of groups (one or four a thread) bounds the top_k-th logit from below: a
+// histogram of the maxima (256 bins between the least and the largest of them)
+// gives a bin that it lies in, and only logits down to that bin are sorted, hardly
+// more than top_k.  Where there are too few maxima, or too many candidates (equal logits), a
 // radix selection over the slices decides exactly.  Exponentials and
 // sums of the kept are in 64 bits: the order and the top_p border are decided
 // by values next to each other.
@@ -39,6 +39,7 @@ constexpr int kMaxCluster = 8;
 // a block lives some 17 us, of which the read is 4 and the rest barriers of the
 // block and the cluster, and shared memory lets 296 of the 768 blocks run at once.
 constexpr int kBins = 256;
+constexpr float kBinRange = 64.0f;   // the bins reach no further down: masks of -1e9 would leave the rest one bin
 constexpr int kCand = 2048;          // candidates that one sort takes
 constexpr int kSliceMax = 40960;     // logits of a slice in shared memory (a multiple of 4)
 
@@ -270,14 +271,45 @@ __global__ void __launch_bounds__(kVThreads) k_sample_probs(const ProbsArgs a) {
         }
         __syncthreads();
     }
-    // the thread's maximum, the row's, and the least finite one of a thread
-    float top = -INFINITY;
+    // the maxima of the thread's four groups of logits, the row's, and the least finite group's
+    float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
     bool nan = false;
-    each([&](int, float v) {
-        top = fmaxf(top, v);
-        nan = nan || v != v;
-    });
-    float mx = warp_max(top), mn = -warp_max(top > -INFINITY ? -top : -INFINITY);
+    if constexpr (VEC) {
+        const float4 *x4 = reinterpret_cast<const float4 *>(x);
+        for (int i = tid; i < n / 4; i += kVThreads) {
+            const float4 v = x4[i];
+            tops[0] = fmaxf(tops[0], v.x), tops[1] = fmaxf(tops[1], v.y);
+            tops[2] = fmaxf(tops[2], v.z), tops[3] = fmaxf(tops[3], v.w);
+            nan = nan || v.x != v.x || v.y != v.y || v.z != v.z || v.w != v.w;
+        }
+    } else {
+        int i = tid;
+        for (; i + 3 * kVThreads < n; i += 4 * kVThreads)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float v = x[i + j * kVThreads];
+                tops[j] = fmaxf(tops[j], v);
+                nan = nan || v != v;
+            }
+#pragma unroll
+        for (int j = 0; j < 3; j++)
+            if (i + j * kVThreads < n) {
+                const float v = x[i + j * kVThreads];
+                tops[j] = fmaxf(tops[j], v);
+                nan = nan || v != v;
+            }
+    }
+    if (a.by_maxima == 1) {  // (one group)
+        tops[0] = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+        tops[1] = tops[2] = tops[3] = -INFINITY;
+    }
+    float mx = -INFINITY, mn = INFINITY;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        mx = fmaxf(mx, tops[j]);
+        if (tops[j] > -INFINITY) mn = fminf(mn, tops[j]);
+    }
+    mx = warp_max(mx), mn = -warp_max(-mn);
     if (lane == 0) sm->red[0][warp] = mx, sm->red[1][warp] = mn;
     for (int i = tid; i < kBins; i += kVThreads) sm->hist[i] = 0;
     nan = __syncthreads_or(nan);
@@ -305,7 +337,7 @@ __global__ void __launch_bounds__(kVThreads) k_sample_probs(const ProbsArgs a) {
         }
     }
     __syncthreads();
-    mx = sm->mx, mn = sm->mn;
+    mx = sm->mx, mn = fmaxf(sm->mn, sm->mx - kBinRange);
     const bool bad = sm->bad;
     const double temp = a.params.temperature > 0.0f ? (double)a.params.temperature : 1.0;
     const bool topk = a.params.top_k > 0 && a.params.top_k < a.V;
@@ -375,7 +407,9 @@ __global__ void __launch_bounds__(kVThreads) k_sample_probs(const ProbsArgs a) {
     bool few = a.by_maxima;
     int sel = 0;
     if (few) {
-        if (top > -INFINITY) atomicAdd(&sm->hist[bin_of(top)], 1u);
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (tops[j] > -INFINITY) atomicAdd(&sm->hist[bin_of(tops[j])], 1u);
         meet();
         // the bin of the k-th largest maximum; with fewer finite maxima than k, all bins
         unsigned c = 0;
@@ -809,10 +843,13 @@ int qora_sample_probs(qora_ctx *ctx, const float *logits, int32_t B, int32_t V, 
     a.n_prev = n_prev;
     a.slice = ((V + nr - 1) / nr + 3) / 4 * 4;
     a.params = *params;
-    // threads that hold a logit, at least: half of them have to be enough for top_k
-    const int64_t holders = (int64_t)(nr - 1) * (a.slice / 4 < kVThreads ? a.slice / 4 : kVThreads) +
-                            (nr == 1 ? (V / 4 < kVThreads ? V / 4 : kVThreads) : 0);
-    a.by_maxima = topk && params->top_k <= holders / 2;
+    // threads that hold a logit, at least: half of them, or of their groups of which
+    // there are four, have to be enough for top_k (fewer maxima are quicker: 160 rows
+    // of 2048 with 50 take 7.3 us by one a thread, 7.6 by four; with 1000 of 512 rows,
+    // where one is not enough, 44 us by four and 60 without)
+    const auto holders = [](int64_t logits) { return logits / 4 < kVThreads ? logits / 4 : kVThreads; };
+    const int64_t held = nr == 1 ? holders(V) : (nr - 1) * holders(a.slice);
+    a.by_maxima = !topk ? 0 : params->top_k <= held / 2 ? 1 : params->top_k <= 2 * held ? 4 : 0;
     const size_t smem = sizeof(ProbsSmem) + (size_t)a.slice * 4;
     auto kern = vec ? k_sample_probs<true> : k_sample_probs<false>;
     static std::atomic<uint64_t> done[2];
