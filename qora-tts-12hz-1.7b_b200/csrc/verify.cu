@@ -356,7 +356,8 @@ __global__ void __launch_bounds__(kVThreads) k_sample_probs(const ProbsArgs a) {
         auto weight = [&](float v) {
             const float d = v - mx, z = d * per_hi;
             const float e = expf(z);
-            return fmaf(e, fmaxf(fmaf(d, per_hi, -z) + d * per_lo, -1.0f), e);  // (d = -inf: NaN to -1, e = 0)
+            // (z past f32's range, -inf among it: the error is NaN or infinite, and e = 0)
+            return fmaf(e, fminf(fmaxf(fmaf(d, per_hi, -z) + d * per_lo, -1.0f), 1.0f), e);
         };
         double s = 0.0;
         if constexpr (VEC) {

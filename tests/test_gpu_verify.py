@@ -89,6 +89,29 @@ def test_probs_ties_go_to_the_lowest_index(E, ctx, V):
     assert list(np.nonzero(got[2])[0]) == list(range(V // 2, V // 2 + 50))
 
 
+@pytest.mark.parametrize("V", [257, 1500, 2049, 9001, 20000, 60000])
+@pytest.mark.parametrize("top_k", [50, 200, 1000])
+@pytest.mark.parametrize("mask", [-1e9, float(np.finfo(np.float32).min)])
+def test_probs_of_masked_rows(E, ctx, V, top_k, mask):
+    """Most tokens masked by a large negative number: fewer left than top_k, about as
+    many, and more, and all but one."""
+    rng = np.random.default_rng(V + top_k)
+    left = [1, min(V, top_k // 2), min(V, top_k + 1), V // 2]
+    x = np.full((len(left), V), mask, np.float32)
+    for r, n in enumerate(left):
+        at = rng.permutation(V)[:n]
+        x[r, at] = (3 * rng.standard_normal(n)).astype(np.float32)
+    got = E.sample_probs(ctx, _dev(x), None, E._lib.SampleParams(0.9, top_k, 0.95 if top_k < V else 1.0, 1.0)).cpu().numpy()
+    assert _error(ctx) == 0
+    for r in range(len(left)):
+        ref = R.probs(x[r], None, 0.9, top_k, 0.95 if top_k < V else 1.0, 1.0)
+        # as in _check_probs, with the range of the logits that are left (masked ones are 0
+        # exactly: e^-1e9); a cut is exact in 64 bits
+        tol = 2.0 ** -21 + 2.0 ** -23 * 2 * np.abs(x[r][x[r] > mask]).max() / 0.9
+        assert np.array_equal(got[r] > 0, ref > 0)
+        assert np.all(np.abs(got[r] - ref) <= tol * ref)
+
+
 def test_probs_agree_with_the_sampler(E, ctx):
     """qora_sample draws what the cumulative probabilities give for its random numbers."""
     import torch
