@@ -668,9 +668,9 @@ int qora_kv4_reserve(qora_kv4 *kv, const int32_t *counts, int32_t max_tokens, in
     const size_t smem = ((size_t)((kv->pool_pages + 31) / 32) + 3 * (size_t)kv->streams) * 4;
     static std::atomic<uint64_t> done;
     QORA_TRY(allow_smem(k_kv4_reserve, ((1 << 20) / 32 + 3 * kKv4MaxStreams) * 4, kv->ctx->device, done));
-    // a cluster pays when there are more table entries and tokens than one block
-    // takes in a few rounds
-    const bool wide = (int64_t)kv->streams * kv->pages_per_stream + max_tokens > 16384;
+    // a cluster pays where there are many table entries and tokens: 16448 of them take
+    // 8.8 us by one block and 10.5 by a cluster, 32896 9.9 and 9.3, 66048 16.3 and 11.5
+    const bool wide = (int64_t)kv->streams * kv->pages_per_stream + max_tokens > 24576;
     const unsigned nr = wide ? kResCluster : 1;
     if (wide) QORA_CUDA(cudaFuncSetAttribute(k_kv4_reserve, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     return launch_ex(k_kv4_reserve, dim3(1, nr), dim3(kResThreads), smem, as_stream(stream), nr, a);

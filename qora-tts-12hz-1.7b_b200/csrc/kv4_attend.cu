@@ -32,6 +32,8 @@
 // lengths, tables, first copies and the join, one after the other.  The units are
 // bound by instructions: some 780 for 32 positions at a tile of 4 rows, issued in
 // 60 % of the cycles at 16 warps a multiprocessor, as many as registers allow.
+#include <algorithm>
+
 #include <cooperative_groups.h>
 
 #include "kv4.cuh"
@@ -701,6 +703,27 @@ int launch_rows(const qora_kv4 *kv, const AttendArgs &a, int64_t rows, cudaStrea
 }
 }  // namespace
 
+namespace {
+// Whether the prompt kernel (tiles of 128 rows, one block a multiprocessor) is the
+// better one.  Both take time in proportion to the positions, so tiles decide: here
+// all tiles of 8 rows share the machine, there the waves of blocks count, one wave
+// as long as 400 tiles of 8 at head_dim 128, 600 at 64.  Measured at
+// 16 / 8 heads of 128, us here / there: 16 streams of 2000 positions 34 / 51 with 16
+// rows a kv head, 63 / 51 with 32, 113 / 51 with 64; 32 streams of 4096 118 / 215 with
+// 16, 207 / 216 with 32, 317 / 216 with 48; 4 streams of 4000 60 / 88 with 64, 100 / 90
+// with 96; one stream of 1000 22 / 29 with 128.  At 64, 16 streams of 2000: 40 / 41
+// with 32 rows, 58 / 41 with 48.
+bool prompt_pays(const qora_kv4 *kv, int64_t tokens, int64_t max_count, int64_t rows) {
+    if (rows >= 128) return true;
+    if (rows <= 24) return false;
+    const int64_t G = kv->heads / kv->kvh, streams = std::min<int64_t>(kv->streams, tokens);
+    const int64_t all = G * std::min(tokens, streams * max_count);
+    const int64_t here = kv->kvh * std::max(streams, (all + 7) / 8), there = kv->kvh * std::max(streams, (all + 127) / 128);
+    const int64_t waves = (there + kv->ctx->num_sms - 1) / kv->ctx->num_sms;
+    return here > (kv->hd == 64 ? 600 : 400) * waves;
+}
+}  // namespace
+
 int kv4_attend_setup(qora_kv4 *kv) { return kv->hd == 64 ? setup<64>(kv) : setup<128>(kv); }
 
 }  // namespace qora
@@ -731,6 +754,8 @@ extern "C" int qora_kv4_attend(qora_kv4 *kv, int32_t layer, const float *q, cons
     a.tokens = tokens;
     a.scale_log2 = 1.4426950408889634f / sqrtf((float)kv->hd);
     const int64_t rows = kv->heads / kv->kvh * (int64_t)max_count;  // of a stream's kv head
-    if (rows > 64) return kv4_launch_prompt(kv, layer, q, offsets, tokens, rows, out, as_stream(stream));
+    if (prompt_pays(kv, tokens, max_count, rows)) 
+        return kv4_launch_prompt(kv, layer, q, offsets, tokens, std::min(rows, (int64_t)tokens * (kv->heads / kv->kvh)), out,
+                                 as_stream(stream));
     return kv->hd == 64 ? launch_rows<64>(kv, a, rows, as_stream(stream)) : launch_rows<128>(kv, a, rows, as_stream(stream));
 }

@@ -335,6 +335,8 @@ CASES = [
     (16, 8, 64, 64, [5] * 40, [1] * 40),
     (2, 1, 128, 32, [0, 0, 0], [0, 1, 0]),
     (16, 8, 128, 64, [2500, 40, 0], [1, 1, 1]),
+    (32, 8, 128, 32, [40, 0, 7, 65] * 4, [8, 7, 8, 8] * 4),  # few rows of many streams: the prompt kernel
+    (32, 8, 64, 64, [40, 0, 7, 65] * 9, [7, 8, 0, 8] * 9),
 ]
 
 
