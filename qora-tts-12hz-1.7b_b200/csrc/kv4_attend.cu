@@ -692,12 +692,15 @@ int setup(qora_kv4 *kv) {
     QORA_TRY((clusters_of<D, 1>(kv, kv->clusters[0])));
     return clusters_of<D, 2>(kv, kv->clusters[1]);
 }
-// Row tiles of 4 or 8.  (Tiles of 12 read the cache once where these read it twice,
+// Row tiles of 4 or 8: 4 also where each of them has a cluster of 8 blocks of its own
+// (one stream of 1000 positions, 16 / 8 heads: 10.3 us against 12.6 with 8 rows a kv
+// head, 10.9 against 13.6 with 16; 4 streams of 4000, past that: 22.3 against 17.9).  (Tiles of 12 read the cache once where these read it twice,
 // but do not fit 128 registers: 6 drafts of 16 streams of 4096 took 58 us against 40.)
 template <int D>
 int launch_rows(const qora_kv4 *kv, const AttendArgs &a, int64_t rows, cudaStream_t st) {
-    const int nt = rows <= 4 ? 1 : 2;
-    const int64_t items = (int64_t)kv->streams * kv->kvh * ((rows + 4 * nt - 1) / (4 * nt));
+    const int64_t items4 = (int64_t)kv->streams * kv->kvh * ((rows + 3) / 4);
+    const int nt = rows <= 4 || items4 <= kv->clusters[0][0] ? 1 : 2;
+    const int64_t items = nt == 1 ? items4 : (int64_t)kv->streams * kv->kvh * ((rows + 7) / 8);
     const auto &n = kv->clusters[nt - 1];
     return nt == 1 ? launch<D, 1>(kv, a, n, items, st) : launch<D, 2>(kv, a, n, items, st);
 }
