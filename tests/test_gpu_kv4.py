@@ -423,6 +423,92 @@ def test_what_a_page_held_before_does_not_matter(ctx, hd, lens, counts):
     assert _error(ctx) == 0
 
 
+# Shapes with rows enough for the prompt kernel: 400 (head_dim 64: 600) tiles of 8 rows.
+MANY = [(32, 8, 128, 32, [37, 0, 90, 161], [50, 31, 1, 47]), (32, 16, 64, 64, [100, 5, 0], [90, 77, 0]),
+        (30, 10, 128, 64, [64, 0], [33, 100]), (16, 16, 128, 32, [3, 200], [129, 100])]
+
+
+@pytest.mark.parametrize("heads,kvh,hd,page,lens,counts", MANY)
+@pytest.mark.parametrize("q_size,k_size,v_size", [(1.5, 1.0, 1.0), (1e-30, 1.0, 1.0), (3e4, 1e-3, 1e-4), (1e6, 1e-5, 3e5)])
+def test_many_rows_any_range(ctx, heads, kvh, hd, page, lens, counts, q_size, k_size, v_size):
+    import torch
+    kv, offsets, held, rng = _filled(ctx, lens, counts, heads, kvh, hd, page, 60 + hd, k_size, v_size)
+    n = sum(counts)
+    q = (q_size * rng.standard_normal((n + 3, heads, hd))).astype(np.float32)
+    out = torch.full((n + 3, heads * hd), 9.0, device="cuda")
+    got = _check(kv, q, offsets, held, lens, counts, heads, kvh, hd, max(counts), out)
+    assert (got[n:] == 9.0).all()
+    assert np.array_equal(_check(kv, q, offsets, held, lens, counts, heads, kvh, hd, max(counts))[:n], got[:n])
+    _check(kv, q, offsets, held, lens, counts, heads, kvh, hd, 1)    # (the other kernel)
+    assert _error(ctx) == 0
+
+
+@pytest.mark.parametrize("heads,kvh,hd,page,lens,counts", MANY)
+def test_many_rows_see_nothing_behind_and_nan_where_it_is(ctx, heads, kvh, hd, page, lens, counts):
+    """Behind the streams' ends: zeros, the largest scales and NaN give the same bits.  A
+    NaN inside reaches the rows that see it, in its scale group for values."""
+    import torch
+    kv, offsets, held, rng = _filled(ctx, lens, counts, heads, kvh, hd, page, 70, 1e-3, 1e-4)
+    table, S, n, most = kv.state()["table"].cpu().numpy(), len(lens), sum(counts), max(counts)
+    slot = lambda b, p: int(table[b, p // page]) * page + p % page
+    behind = _i32([slot(b, p) for b in range(S) for p in range(lens[b] + counts[b], -(-(lens[b] + counts[b]) // page) * page)])
+    q = (50.0 * rng.standard_normal((n, heads, hd))).astype(np.float32)
+    got = []
+    for size in (0.0, 1e30, float("nan")):
+        rows = torch.full((behind.numel(), kvh * hd), size, device="cuda")
+        kv.write(1, behind, rows, rows)
+        got.append(_check(kv, q, offsets, held, lens, counts, heads, kvh, hd, most))
+    assert all(np.array_equal(g, got[0]) for g in got)
+    first = lens[0] + 20                                     # tokens 20 on of stream 0 see it
+    at = _i32([slot(0, first)])
+    k, v = kv.read(1, at)
+    half = v.clone()
+    half[:, hd - 32:hd] = float("nan")                       # the first kv head's last group
+    for keys, values in ((k * float("nan"), v), (k, v * float("nan")), (k, half)):
+        kv.write(1, at, keys, values)
+        nan = torch.isnan(kv.attend(1, _dev(q.reshape(n, -1)), offsets, most)).view(n, heads, hd).cpu().numpy()
+        want = np.zeros_like(nan)
+        want[20:counts[0], :heads // kvh if values is half else heads, hd - 32 if values is half else 0:] = True
+        assert np.array_equal(nan, want)
+    kv.write(1, at, k, v)
+    q[2, 1, 3] = np.inf
+    nan = torch.isnan(kv.attend(1, _dev(q.reshape(n, -1)), offsets, most)).view(n, heads, hd)
+    assert bool(nan[2, 1].all()) and int(nan.sum()) == hd
+    assert _error(ctx) == 0
+
+
+def test_captured_many_rows_replay_with_other_lengths(ctx):
+    import torch
+    heads, kvh, hd, page, lens, counts = 32, 8, 128, 32, [37, 0, 90], [50, 64, 20]
+    kv, offsets, held, rng = _filled(ctx, lens, counts, heads, kvh, hd, page, 80)
+    n = sum(counts)
+    q = rng.standard_normal((n, heads, hd)).astype(np.float32)
+    qd, out, side = _dev(q.reshape(n, -1)), torch.zeros(n, heads * hd, device="cuda"), torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        kv.attend(1, qd, offsets, 64, out=out)
+    other = _filled(ctx, lens, counts, heads, kvh, hd, page, 81)
+    want = other[0].attend(1, qd, other[1], 64)
+    torch.cuda.synchronize()
+    for now in (counts, [3, 64, 0], [0, 0, 1], [0, 0, 0]):
+        offsets.copy_(_i32(np.concatenate([[0], np.cumsum(now)])))
+        out.fill_(7.0)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            graph.replay()                                   # and another cache's prompt beside it
+        beside = other[0].attend(1, qd, other[1], 64)
+        torch.cuda.synchronize()
+        assert bool((beside == want).all())
+        got, at = out.cpu().numpy(), 0
+        for b, c in enumerate(now):
+            if c:
+                ref, bound = R.attend(q[at:at + c], held[b][0][:lens[b] + c], held[b][1][:lens[b] + c], lens[b], heads, kvh)
+                assert np.all(np.abs(got[at:at + c].reshape(c, heads, hd) - ref) <= bound)
+            at += c
+        assert (got[at:] == 7.0).all()
+    assert _error(ctx) == 0
+
+
 def test_unaligned_pointers_are_refused(ctx, orc):
     import torch
     from qora_b200 import _lib
