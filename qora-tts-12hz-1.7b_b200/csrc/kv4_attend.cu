@@ -714,8 +714,8 @@ namespace {
 // 16 / 8 heads of 128, us here / there: 16 streams of 2000 positions 34 / 51 with 16
 // rows a kv head, 63 / 51 with 32, 113 / 51 with 64; 32 streams of 4096 118 / 215 with
 // 16, 207 / 216 with 32, 317 / 216 with 48; 4 streams of 4000 60 / 88 with 64, 100 / 90
-// with 96; one stream of 1000 22 / 29 with 128, of 8000 61 / 165.  At 64, 16 streams of 2000: 40 / 41
-// with 32 rows, 58 / 41 with 48.
+// with 96; one stream of 1000 22 / 29 with 128, of 8000 61 / 165.  At head_dim 64, 16
+// streams of 2000 positions: 40 / 41 with 32 rows, 58 / 41 with 48.
 bool prompt_pays(const qora_kv4 *kv, int64_t tokens, int64_t max_count, int64_t rows) {
     if (rows <= 24) return false;
     const int64_t G = kv->heads / kv->kvh, streams = std::min<int64_t>(kv->streams, tokens);
@@ -756,7 +756,7 @@ extern "C" int qora_kv4_attend(qora_kv4 *kv, int32_t layer, const float *q, cons
     a.tokens = tokens;
     a.scale_log2 = 1.4426950408889634f / sqrtf((float)kv->hd);
     const int64_t rows = kv->heads / kv->kvh * (int64_t)max_count;  // of a stream's kv head
-    if (prompt_pays(kv, tokens, max_count, rows)) 
+    if (prompt_pays(kv, tokens, max_count, rows))
         return kv4_launch_prompt(kv, layer, q, offsets, tokens, std::min(rows, (int64_t)tokens * (kv->heads / kv->kvh)), out,
                                  as_stream(stream));
     return kv->hd == 64 ? launch_rows<64>(kv, a, rows, as_stream(stream)) : launch_rows<128>(kv, a, rows, as_stream(stream));

@@ -22,7 +22,7 @@
 // P's columns follow).  O of each tile is added in f32 registers, because the
 // tensor core's own additions do not round to nearest.
 //
-// 2 prompts of 2048 and some 1700 tokens, 16 / 8 heads of 128: 123 us, 188 TFLOP/s of
+// 2 prompts of 2048 and some 1700 tokens, 16 / 8 heads of 128: 121 us, 191 TFLOP/s of
 // the two products (three times that on the tensor cores).  What bounds it is the
 // softmax warps' chain of a tile, some 2400 cycles of wait, maximum, exponentials,
 // P and sum of O, against 1540 of products; and 6 us a block outside its tiles.
