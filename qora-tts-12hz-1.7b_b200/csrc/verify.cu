@@ -67,9 +67,10 @@ struct alignas(16) ProbsSmem {  // (the slice behind it is read in 16-byte piece
 
 static_assert(sizeof(ProbsSmem) % 16 == 0 && kSliceMax % 4 == 0, "the slice is 16-byte aligned");
 
-// Order of f32 values as unsigned integers.
+// Order of f32 values as unsigned integers; the two zeros are equal logits, so -0
+// becomes +0 (whose addition changes no other value).
 __device__ __forceinline__ unsigned order_key(float x) {
-    const unsigned u = __float_as_uint(x);
+    const unsigned u = __float_as_uint(__fadd_rn(x, 0.0f));
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 __device__ __forceinline__ float order_value(unsigned k) {

@@ -112,6 +112,28 @@ def test_probs_of_masked_rows(E, ctx, V, top_k, mask):
         assert np.all(np.abs(got[r] - ref) <= tol * ref)
 
 
+@pytest.mark.parametrize("V", [300, 2048, 5000, 100000])
+@pytest.mark.parametrize("top_k", [50, 600])
+def test_probs_zeros_of_both_signs_are_equal(E, ctx, V, top_k):
+    """Logits of +0 and -0, as masking by a product leaves them, tie: the lower index
+    comes first, with all of the row zeros (radix selection) and with few (sorting)."""
+    if top_k >= V:
+        top_k = V // 2
+    rng = np.random.default_rng(V + top_k)
+    x = np.zeros((4, V), np.float32)
+    x[0, ::2] = -0.0                                        # -0 first of each pair
+    x[1, rng.permutation(V)[:V // 2]] = -0.0
+    x[2:] = -5.0 - rng.random((2, V)).astype(np.float32)
+    zeros = np.sort(rng.permutation(V)[:min(V, top_k + 40)])
+    x[2, zeros] = np.where(np.arange(len(zeros)) % 3 == 0, 0.0, -0.0)
+    x[3] = x[2]
+    x[3, zeros[-10:]] = 1.5                                 # ten above the zeros
+    for top_p in (1.0, 0.9):
+        got = _check_probs(E, ctx, x, None, (0.9, top_k, top_p, 1.0))
+        for r in range(4):
+            assert np.array_equal(got[r] > 0, R.probs(x[r], None, 0.9, top_k, top_p, 1.0) > 0)
+
+
 def test_probs_agree_with_the_sampler(E, ctx):
     """qora_sample draws what the cumulative probabilities give for its random numbers."""
     import torch
