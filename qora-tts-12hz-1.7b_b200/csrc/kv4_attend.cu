@@ -495,14 +495,13 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_attend(const AttendArgs a) 
                 const float ref = mx == -INFINITY ? 0.0f : mx;
                 const float corr = ex2(m[nt] - ref);
                 m[nt] = mx;
-                l[nt] *= corr;
                 keep[nt] = corr * shrink;
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    sc[nt][i] = ex2(sc[nt][i] - ref);
-                    l[nt] += sc[nt][i];
-                    sc[nt][i] *= lift;
-                }
+                for (int i = 0; i < 4; i++) sc[nt][i] = ex2(sc[nt][i] - ref);
+                // (one addition a unit to the running sum, as the weighted sums have)
+                l[nt] = fmaf(l[nt], corr, (sc[nt][0] + sc[nt][1]) + (sc[nt][2] + sc[nt][3]));
+#pragma unroll
+                for (int i = 0; i < 4; i++) sc[nt][i] *= lift;
             }
 #pragma unroll
             for (int c = 0; c < C; c++) {

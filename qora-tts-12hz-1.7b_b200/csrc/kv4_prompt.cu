@@ -475,7 +475,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const PromptArgs a) 
                 if (lane == 0) mbar_arrive(&sm.q_full);
             }
             float m = -INFINITY, corr = 0.0f, unv = 0.0f;
-            float2 l = make_float2(0.0f, 0.0f);
+            // The sum, and what its additions have rounded away: a tile's 32 values are added
+            // on their own, then once to the sum.  (One by one, values that hardly differ all
+            // round in one direction: 1.3e-4 of the sum at 33000 positions.)
+            float l = 0.0f, l_rest = 0.0f;
             float o[D / 2];
 #pragma unroll
             for (int i = 0; i < D / 2; i++) o[i] = 0.0f;
@@ -539,15 +542,20 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const PromptArgs a) 
                 if (to > m + 7.0f) {
                     corr_now = ex2(m - to);
                     m = to;
-                    l.x *= corr_now, l.y *= corr_now;
+                    l *= corr_now, l_rest *= corr_now;
                 }
                 const float ref = m == -INFINITY ? 0.0f : m - 8.0f;
+                float2 s[4] = {};
 #pragma unroll
                 for (int i = 0; i < 32; i += 2) {
                     const float2 z = fma2(make_float2(x[i], x[i + 1]), make_float2(f, f), make_float2(-ref, -ref));
                     x[i] = ex2(z.x), x[i + 1] = ex2(z.y);
-                    l = add2(l, make_float2(x[i], x[i + 1]));
+                    s[(i >> 1) & 3] = add2(s[(i >> 1) & 3], make_float2(x[i], x[i + 1]));
                 }
+                s[0] = add2(add2(s[0], s[1]), add2(s[2], s[3]));
+                const float part = s[0].x + s[0].y, sum = __fadd_rn(l, part), back = __fsub_rn(sum, l);
+                l_rest += __fsub_rn(l, __fsub_rn(sum, back)) + __fsub_rn(part, back);
+                l = sum;
                 uint32_t hi[16], lo[16];
 #pragma unroll
                 for (int p = 0; p < 16; p++) {  // slot pair p: positions 8h + 2t, + 1 with t = p / 4, h = p % 4
@@ -581,7 +589,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const PromptArgs a) 
                 }
             }
             fold(ntiles - 1);
-            sm.l[hs][r] = l.x + l.y;
+            sm.l[hs][r] = l + l_rest;
             asm volatile("bar.sync 1, 256;" ::: "memory");
             const float inv = __fdiv_rn(1.0f, sm.l[0][r] + sm.l[1][r]);
 #pragma unroll
