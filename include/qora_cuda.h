@@ -426,9 +426,11 @@ int qora_sample_probs(qora_ctx *ctx, const float *logits, int32_t B, int32_t V,
  * when nothing is left), and when all counts[b] = a pass, from target row a: the
  * first index whose cumulative sum passes uniforms[K] times the sum.  Sums are in
  * 64 bits.  tokens [B][K + 1] = the a accepted drafts, the drawn token, then
- * -1; n_out [B] = a + 1.  K <= 2^20, V <= 2^30.  A draft outside [0, V) is rejected, a count outside
- * [0, K] clamped, and both are QORA_ERR_RANGE at the next
- * qora_ctx_check_device_error. */
+ * -1; n_out [B] = a + 1.  A row without any positive weight gives token 0.
+ * counts[b] = -1: the stream is idle; none of its rows is read, its tokens are
+ * all -1 and its n_out is 0.  K <= 2^20, V <= 2^30.  A draft outside [0, V) is
+ * rejected, any other count outside [0, K] clamped, and both are
+ * QORA_ERR_RANGE at the next qora_ctx_check_device_error. */
 int qora_verify_drafts(qora_ctx *ctx, const int32_t *drafts, const float *draft_probs,
                        const float *target_probs, const int32_t *counts, const float *uniforms,
                        int32_t B, int32_t K, int32_t V, int32_t *tokens, int32_t *n_out,

@@ -400,9 +400,10 @@ def verify_drafts(ctx: Context, drafts: torch.Tensor, draft_probs: torch.Tensor 
                   out=None, stream=None):
     """Speculative verification (qora_verify_drafts): drafts int32 [B][K] drawn
     from draft_probs [B][K][V] (None: deterministic), the target's probabilities
-    [B][K + 1][V], uniforms [B][K + 1] in [0, 1), counts int32 [B] (None: K
-    drafts each).  Returns tokens int32 [B][K + 1] (the accepted drafts, one
-    drawn token, then -1) and n_out int32 [B] (tokens of each stream)."""
+    [B][K + 1][V], uniforms [B][K + 1] in [0, 1), counts int32 [B] of drafts
+    (None: K each; -1: the stream is idle and gets no token).  Returns tokens
+    int32 [B][K + 1] (the accepted drafts, one drawn token, then -1) and n_out
+    int32 [B] (tokens of each stream)."""
     B, K = drafts.shape
     V = target_probs.shape[-1]
     dev, i32, f32 = ctx.device, torch.int32, torch.float32
