@@ -243,7 +243,7 @@ int qora_kv_attend_noalloc(qora_kv *kv, int32_t layer, const float *qkv, int32_t
  * `stream` and may be captured into a CUDA graph, so a step whose lengths
  * depend on the step before (drafted tokens that were accepted) needs no
  * return to the host:
- *     _reserve -> per layer: _append, _attend -> qora_verify_drafts -> _advance.
+ *     _reserve -> per layer: _append, _attend -> qora_verify_drafts -> _accept.
  * Nothing is kept between calls but pages, table and lengths, so calls on
  * different caches may overlap; calls on one cache that write what another
  * reads are ordered by the caller (one stream, or events).
@@ -278,6 +278,12 @@ int qora_kv4_reserve(qora_kv4 *kv, const int32_t *counts, int32_t max_tokens, in
  * length that would leave [0, max_pos] stops there and is QORA_ERR_RANGE at the
  * next qora_ctx_check_device_error. */
 int qora_kv4_advance(qora_kv4 *kv, const int32_t *counts, void *stream);
+/* The same after a step: a stream moves by counts[b], but by no more than the
+ * offsets[b + 1] - offsets[b] tokens that _reserve listed for it.  That is none
+ * for a stream without tokens, and none for any after a _reserve that was
+ * refused, so a step that ran on regardless (its rows are skipped) leaves all
+ * lengths as they were. */
+int qora_kv4_accept(qora_kv4 *kv, const int32_t *counts, const int32_t *offsets, void *stream);
 /* qk-norm, RoPE and the cache append of one layer (talker.rs:285-303) for
  * `tokens` rows: qkv [tokens][(num_heads + 2 kv_heads) head_dim] raw
  * projections, as qora_kv_attend takes them; positions and slots per row

@@ -159,6 +159,8 @@ extern "C" {
                             slots: *mut i32, positions: *mut i32, offsets: *mut i32,
                             stream: *mut c_void) -> c_int;
     pub fn qora_kv4_advance(kv: *mut qora_kv4, counts: *const i32, stream: *mut c_void) -> c_int;
+    pub fn qora_kv4_accept(kv: *mut qora_kv4, counts: *const i32, offsets: *const i32,
+                           stream: *mut c_void) -> c_int;
     pub fn qora_kv4_append(kv: *mut qora_kv4, layer: i32, qkv: *const f32, q_norm: *const u16,
                            k_norm: *const u16, rope_cos: *const f32, rope_sin: *const f32,
                            rope_max_pos: i32, positions: *const i32, slots: *const i32,

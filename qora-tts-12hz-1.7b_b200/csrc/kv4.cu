@@ -236,13 +236,16 @@ __global__ void __launch_bounds__(kResThreads) k_kv4_reserve(const ReserveArgs a
     }
 }
 
-// lengths += counts (negative counts roll back)
-__global__ void k_kv4_advance(int *len, const int *counts, int streams, int max_pos, int *err) {
+// lengths += counts (negative counts roll back); with offsets, by at most the tokens
+// that they list for the stream
+__global__ void k_kv4_advance(int *len, const int *counts, const int *offsets, int streams, int max_pos, int *err) {
     griddep_launch_dependents();
     griddep_wait();
     const int b = blockIdx.x * blockDim.x + threadIdx.x;
     if (b >= streams) return;
-    const int64_t to = (int64_t)len[b] + counts[b];
+    int64_t by = counts[b];
+    if (offsets) by = min(by, (int64_t)offsets[b + 1] - offsets[b]);
+    const int64_t to = (int64_t)len[b] + by;
     if (to < 0 || to > max_pos) raise_error(err, kDevRange);
     len[b] = (int)(to < 0 ? 0 : to > max_pos ? max_pos : to);
 }
@@ -547,6 +550,13 @@ int rows_args(const char *who, qora_kv4 *kv, int32_t layer, const int32_t *slots
     return QORA_OK;
 }
 
+int advance(qora_kv4 *kv, const int32_t *counts, const int32_t *offsets, void *stream) {
+    DeviceGuard dg;
+    QORA_TRY(dg.set(kv->ctx->device));
+    return launch_ex(k_kv4_advance, dim3((kv->streams + 255) / 256), dim3(256), 0, as_stream(stream), 1u,
+                     kv->len.as<int>(), counts, offsets, kv->streams, kv->max_pos, kv->ctx->err.as<int>());
+}
+
 }  // namespace
 
 }  // namespace qora
@@ -678,10 +688,12 @@ int qora_kv4_reserve(qora_kv4 *kv, const int32_t *counts, int32_t max_tokens, in
 
 int qora_kv4_advance(qora_kv4 *kv, const int32_t *counts, void *stream) {
     if (!kv || !counts) return set_error(QORA_ERR_INVALID, "qora_kv4_advance: null argument");
-    DeviceGuard dg;
-    QORA_TRY(dg.set(kv->ctx->device));
-    return launch_ex(k_kv4_advance, dim3((kv->streams + 255) / 256), dim3(256), 0, as_stream(stream), 1u,
-                     kv->len.as<int>(), counts, kv->streams, kv->max_pos, kv->ctx->err.as<int>());
+    return advance(kv, counts, nullptr, stream);
+}
+
+int qora_kv4_accept(qora_kv4 *kv, const int32_t *counts, const int32_t *offsets, void *stream) {
+    if (!kv || !counts || !offsets) return set_error(QORA_ERR_INVALID, "qora_kv4_accept: null argument");
+    return advance(kv, counts, offsets, stream);
 }
 
 int qora_kv4_append(qora_kv4 *kv, int32_t layer, const float *qkv, const uint16_t *q_norm, const uint16_t *k_norm,

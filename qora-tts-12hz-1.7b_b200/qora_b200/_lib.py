@@ -114,6 +114,7 @@ SIGNATURES = {
     "qora_kv4_state": (C.c_int, [_vp, _PP, C.POINTER(C.c_int32), _PP]),
     "qora_kv4_reserve": (C.c_int, [_vp, _vp, _i32, _vp, _vp, _vp, _vp]),
     "qora_kv4_advance": (C.c_int, [_vp, _vp, _vp]),
+    "qora_kv4_accept": (C.c_int, [_vp, _vp, _vp, _vp]),
     "qora_kv4_append": (C.c_int, [_vp, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _i32, _vp, _vp]),
     "qora_kv4_write": (C.c_int, [_vp, _i32, _vp, _i32, _vp, _vp, _vp]),
     "qora_kv4_read": (C.c_int, [_vp, _i32, _vp, _i32, _vp, _vp, _vp]),

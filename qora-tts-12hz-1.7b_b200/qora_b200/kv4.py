@@ -8,7 +8,7 @@ A speculative decode step of every stream, without a return to the host:
         q = kv.append(layer, qkv, q_norm, k_norm, cos, sin, positions, slots)
         o = kv.attend(layer, q, offsets, max_count)
     tokens, n_out = engine.verify_drafts(ctx, drafts, draft_probs, target_probs, uniforms)
-    kv.advance(n_out)
+    kv.advance(n_out, offsets=offsets)
 
 Tensors are on the context's device and contiguous; calls are asynchronous on
 the current stream (or `stream`).  One cache serves one stream at a time.
@@ -38,6 +38,7 @@ class Kv4Cache:
         self._L = L = _lib.load()
         # a decode step makes a call per layer: the entry points are looked up once
         self._reserve, self._advance, self._append = L.qora_kv4_reserve, L.qora_kv4_advance, L.qora_kv4_append
+        self._accept = L.qora_kv4_accept
         self._write, self._read, self._attend = L.qora_kv4_write, L.qora_kv4_read, L.qora_kv4_attend
         h = C.c_void_p()
         _lib.call("qora_kv4_create", ctx.h, layers, num_heads, kv_heads, head_dim, max_pos, streams,
@@ -101,9 +102,15 @@ class Kv4Cache:
             _lib.check(rc, "qora_kv4_reserve")
         return out
 
-    def advance(self, counts: torch.Tensor, stream=None):
-        """Adds counts[b] (int32 [streams]; negative: rolls back) to the lengths."""
-        rc = self._advance(self.h, self._typed("counts", counts, _I32, self.streams), self._stream(stream))
+    def advance(self, counts: torch.Tensor, stream=None, offsets: torch.Tensor | None = None):
+        """Adds counts[b] (int32 [streams]; negative: rolls back) to the lengths.
+        With `offsets` from `reserve`, a stream moves by at most the tokens that
+        were reserved for it: none without tokens, none after a refusal."""
+        n = self._typed("counts", counts, _I32, self.streams)
+        if offsets is None:
+            rc = self._advance(self.h, n, self._stream(stream))
+        else:
+            rc = self._accept(self.h, n, self._typed("offsets", offsets, _I32, self.streams + 1), self._stream(stream))
         if rc:
             _lib.check(rc, "qora_kv4_advance")
 

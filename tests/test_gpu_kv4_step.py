@@ -8,6 +8,8 @@ from test_gpu_kv4 import E, _cache, _dev, _error, _i32, ctx  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
+OOM, RANGE = 4, 5
+
 
 # ------------------------------------------------------------ streams without work
 def test_verify_count_of_an_idle_stream(E, ctx):  # noqa: F811
@@ -31,3 +33,19 @@ def test_verify_count_of_an_idle_stream(E, ctx):  # noqa: F811
                 if b != 1:
                     want = R.verify(drafts[b], None if q is None else q[b], p[b], u[b], K)
                     assert tokens[b].tolist() == want + [-1] * (K + 1 - len(want)) and n_out[b] == len(want)
+
+
+def test_advance_within_what_was_reserved(ctx):  # noqa: F811
+    """With reserve's offsets, a stream moves by at most the tokens that it was given:
+    none for one without tokens, none for all after a refusal, whatever n_out says."""
+    kv = _cache(ctx, 1, 2, 1, 64, 256, 4, 32, 8)
+    _, _, offsets = kv.reserve(_i32([5, 0, 31, 40]), 100)
+    kv.advance(_i32([3, 1, 31, 50]), offsets=offsets)
+    assert list(kv.lengths()) == [3, 0, 31, 40] and _error(ctx) == 0
+    _, _, offsets = kv.reserve(_i32([1, 0, 200, 1]), 300)   # the pool has 4 pages left
+    assert _error(ctx) == OOM
+    kv.advance(_i32([1, 1, 5, 1]), offsets=offsets)
+    assert list(kv.lengths()) == [3, 0, 31, 40] and _error(ctx) == 0
+    _, _, offsets = kv.reserve(_i32([1, 0, 1, 1]), 3)       # and the cache goes on
+    kv.advance(_i32([1, 1, -4, 0]), offsets=offsets)                # rolling back stays possible
+    assert list(kv.lengths()) == [4, 0, 27, 40] and _error(ctx) == 0

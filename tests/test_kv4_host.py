@@ -105,3 +105,10 @@ int main() { show<64>(); show<128>(); return 0; }
             else:
                 hit[int(a)] += 1
         assert (hit == 1).all()
+
+
+def test_accept_refuses_null_arguments(lib):
+    one = C.c_void_p(16)
+    assert lib.qora_kv4_accept(None, one, one, None) == INVALID
+    assert lib.qora_kv4_accept(one, None, one, None) == INVALID
+    assert lib.qora_kv4_accept(one, one, None, None) == INVALID
