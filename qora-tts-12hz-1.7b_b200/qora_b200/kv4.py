@@ -1,13 +1,17 @@
 """The 4-bit paged KV cache (qora_kv4): block tables built on the GPU, the
 append with qk-norm and rotation, and attention over the cache.
 
-A speculative decode step of every stream, without a return to the host:
+A speculative decode step of every stream, without a return to the host
+(drafted: int32 [streams], drafts of each; -1: idle):
 
-    slots, positions, offsets = kv.reserve(counts, max_tokens)
+    slots, positions, offsets = kv.reserve(drafted + 1, max_tokens)
     for each layer:
         q = kv.append(layer, qkv, q_norm, k_norm, cos, sin, positions, slots)
-        o = kv.attend(layer, q, offsets, max_count)
-    tokens, n_out = engine.verify_drafts(ctx, drafts, draft_probs, target_probs, uniforms)
+        o = kv.attend(layer, q, offsets, K + 1)
+    # logits are packed by offsets; verification takes K + 1 rows of every stream
+    row = torch.minimum(offsets[:-1, None] + torch.arange(K + 1, device=dev), offsets[1:, None] - 1)
+    p = engine.sample_probs(ctx, logits[row.clamp(min=0).view(-1)], prev, params)
+    tokens, n_out = engine.verify_drafts(ctx, drafts, draft_probs, p.view(streams, K + 1, -1), uniforms, drafted)
     kv.advance(n_out, offsets=offsets)
 
 Tensors are on the context's device and contiguous; calls are asynchronous on

@@ -1,10 +1,11 @@
 """A speculative step over the 4-bit cache as a whole, and what its calls do at
-its edges: streams without work, refused reservations, calls on other streams."""
+its edges: streams without work, refused reservations, calls on other streams, one
+captured graph from block tables to lengths."""
 import numpy as np
 import pytest
 
 import kv4_ref as R
-from test_gpu_kv4 import E, _cache, _dev, _error, _i32, ctx  # noqa: F401
+from test_gpu_kv4 import E, _cache, _dev, _error, _i32, _weights, ctx  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -49,3 +50,93 @@ def test_advance_within_what_was_reserved(ctx):  # noqa: F811
     _, _, offsets = kv.reserve(_i32([1, 0, 1, 1]), 3)       # and the cache goes on
     kv.advance(_i32([1, 1, -4, 0]), offsets=offsets)                # rolling back stays possible
     assert list(kv.lengths()) == [4, 0, 27, 40] and _error(ctx) == 0
+
+
+# ------------------------------------------------------------ a step in one graph
+def test_captured_step_from_tables_to_lengths(E, ctx, orc):  # noqa: F811
+    """reserve, append, attend, the logits' rows by stream, the distribution, verification
+    and advance in one graph without a return to the host: ragged drafts, streams that
+    come and go, a step that the pool refuses.  Replays equal eager calls with the
+    counts known on the host, and verification's definition."""
+    import torch
+    heads, kvh, hd, S, K, V, rows, pool = 4, 2, 64, 4, 3, 200, 18, 10
+    qn, kn, cos, sin = (_dev(t) for t in _weights(orc, hd, 4))
+    g = torch.Generator(device="cuda").manual_seed(9)
+    params = E._lib.SampleParams(0.9, 40, 0.95, 1.1)
+    rng = np.random.default_rng(12)
+
+    def inputs(drafted):
+        return (_i32(drafted), torch.randn(rows, (heads + 2 * kvh) * hd, generator=g, device="cuda"),
+                _i32(rng.integers(0, V, (S, K))), torch.rand(S, K + 1, generator=g, device="cuda"),
+                _i32(rng.integers(0, V, (S, K + 1, 8))))
+
+    def program(kv, drafted, qkv, drafts, u, prev, keep):
+        counts = drafted + 1                                # tokens: the last one said, and the drafts; -1: idle
+        slots, positions, offsets = kv.reserve(counts, rows)
+        q = kv.append(0, qkv, qn, kn, cos, sin, positions, slots, out=keep["q"])
+        o = kv.attend(0, q, offsets, K + 1, out=keep["o"])
+        logits = 30.0 * o[:, :V]
+        # row (b, j) is token j of stream b, its last one where it has fewer
+        at = torch.minimum(offsets[:-1, None] + torch.arange(K + 1, device="cuda"), offsets[1:, None] - 1)
+        dense = logits[at.clamp(min=0).reshape(-1)]
+        p = E.sample_probs(ctx, dense, prev.view(S * (K + 1), -1), params).view(S, K + 1, V)
+        tokens, n_out = E.verify_drafts(ctx, drafts, None, p, u, drafted)
+        kv.advance(n_out, offsets=offsets)
+        keep["p"].copy_(p), keep["tokens"].copy_(tokens), keep["n_out"].copy_(n_out)
+
+    def buffers():
+        return dict(q=torch.zeros(rows, heads * hd, device="cuda"), o=torch.zeros(rows, heads * hd, device="cuda"),
+                    p=torch.zeros(S, K + 1, V, device="cuda"), tokens=_i32(np.zeros((S, K + 1))), n_out=_i32(np.zeros(S)))
+
+    # idle streams, all drafts, none; and a step of all drafts that the pool refuses
+    steps = [inputs(d) for d in ([3, -1, 0, 2], [0, 3, -1, 3], [-1, -1, -1, -1], [2, 2, 2, 2], [-1, 0, 3, 1])]
+    full = inputs([3, 3, 3, 3])
+    kv, eager = (_cache(ctx, 1, heads, kvh, hd, 256, S, 32, pool) for _ in range(2))
+    for c in (kv, eager):
+        c.reserve(_i32([30, 0, 31, 60]), 121)               # (positions that hold zeros)
+        c.advance(_i32([30, 0, 31, 60]))
+    bufs, static = buffers(), [t.clone() for t in full]
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        program(kv, *static, bufs)
+    lens = [30, 0, 31, 60]
+    assert list(kv.lengths()) == lens
+    for step in steps:
+        ref = buffers()
+        program(eager, *step, ref)
+        for a, b in zip(static, step):
+            a.copy_(b)
+        for t in bufs.values():
+            t.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert _error(ctx) == 0
+        drafted, _, drafts, u, _ = (t.cpu().numpy() for t in step)
+        for name in ("tokens", "n_out", "q", "o", "p"):
+            assert torch.equal(bufs[name], ref[name]), name
+        tokens, n_out, p = (bufs[n].cpu().numpy() for n in ("tokens", "n_out", "p"))
+        for b in range(S):
+            want = [] if drafted[b] < 0 else R.verify(drafts[b], None, p[b], u[b], drafted[b])
+            assert tokens[b].tolist() == want + [-1] * (K + 1 - len(want)) and n_out[b] == len(want)
+            lens[b] += len(want)
+        assert list(kv.lengths()) == list(eager.lengths()) == lens
+    # a step that the pool refuses: stream 3 has all the other pages, in full
+    held = kv.state()["table"]
+    used = {int(held[b, j]) for b in range(3) for j in range(-(-lens[b] // 32))}
+    rest = [p for p in range(pool) if p not in used]
+    kv.advance(_i32([0, 0, 0, 32 * len(rest) - lens[3]]))
+    held[3, :len(rest)] = _i32(rest)
+    lens[3] = 32 * len(rest)
+    for a, b in zip(static, full):
+        a.copy_(b)
+    torch.cuda.synchronize()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert _error(ctx) == OOM and list(kv.lengths()) == lens
+    kv.advance(_i32([0, 0, 0, -100]))
+    graph.replay()                                          # with pages again it goes on
+    torch.cuda.synchronize()
+    assert _error(ctx) == 0 and all(a > b for a, b in zip(kv.lengths(), lens[:3]))
