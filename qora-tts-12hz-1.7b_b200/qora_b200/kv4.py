@@ -54,11 +54,22 @@ class Kv4Cache:
             self._L.qora_kv4_destroy(self.h)
             self.h = None
 
-    def _typed(self, name: str, t: torch.Tensor, dtype, n: int) -> int:
-        """Pointer of a contiguous tensor of the cache's device that holds at least n values of dtype."""
-        if t.dtype is not dtype or t.numel() < n or t.get_device() != self._dev or not t.is_contiguous():
+    def _typed(self, name: str, t: torch.Tensor, dtype, n: int, exact: bool = False) -> int:
+        """Pointer of a contiguous tensor of the cache's device that holds at least (exact: just) n values of dtype."""
+        if (t.dtype is not dtype or t.numel() < n or (exact and t.numel() != n) or t.get_device() != self._dev
+                or not t.is_contiguous()):
             raise ValueError(f"{name}: expected {n} contiguous values of {dtype} on {self.device}, got {tuple(t.shape)} "
                              f"of {t.dtype} on {t.device}")
+        return t.data_ptr()
+
+    def _rows(self, name: str, t: torch.Tensor, n: int, width: int) -> int:
+        """Pointer of n or more contiguous f32 rows of just `width` values (a wider row would be misread), or of the
+        n * width values in one."""
+        have = t.numel()
+        if (t.dtype is not _F32 or not (have == n * width or (t.dim() and t.shape[0] > n and have == t.shape[0] * width))
+                or t.get_device() != self._dev or not t.is_contiguous()):
+            raise ValueError(f"{name}: expected {n} contiguous rows of {width} {_F32} on {self.device}, got "
+                             f"{tuple(t.shape)} of {t.dtype} on {t.device}")
         return t.data_ptr()
 
     def _norm(self, name: str, t: torch.Tensor) -> int:
@@ -98,10 +109,10 @@ class Kv4Cache:
             out = (torch.empty(max_tokens, **i32), torch.empty(max_tokens, **i32),
                    torch.empty(self.streams + 1, **i32))
         slots, positions, offsets = out
-        rc = self._reserve(self.h, self._typed("counts", counts, _I32, self.streams), max_tokens,
+        rc = self._reserve(self.h, self._typed("counts", counts, _I32, self.streams, True), max_tokens,
                            self._typed("slots", slots, _I32, max_tokens),
                            self._typed("positions", positions, _I32, max_tokens),
-                           self._typed("offsets", offsets, _I32, self.streams + 1), self._stream(stream))
+                           self._typed("offsets", offsets, _I32, self.streams + 1, True), self._stream(stream))
         if rc:
             _lib.check(rc, "qora_kv4_reserve")
         return out
@@ -110,11 +121,11 @@ class Kv4Cache:
         """Adds counts[b] (int32 [streams]; negative: rolls back) to the lengths.
         With `offsets` from `reserve`, a stream moves by at most the tokens that
         were reserved for it: none without tokens, none after a refusal."""
-        n = self._typed("counts", counts, _I32, self.streams)
+        n = self._typed("counts", counts, _I32, self.streams, True)
         if offsets is None:
             rc = self._advance(self.h, n, self._stream(stream))
         else:
-            rc = self._accept(self.h, n, self._typed("offsets", offsets, _I32, self.streams + 1), self._stream(stream))
+            rc = self._accept(self.h, n, self._typed("offsets", offsets, _I32, self.streams + 1, True), self._stream(stream))
         if rc:
             _lib.check(rc, "qora_kv4_advance")
 
@@ -127,13 +138,15 @@ class Kv4Cache:
         n, hd = qkv.shape[0], self.head_dim
         if out is None:
             out = torch.empty(n, self.num_heads * hd, device=qkv.device)
-        table = rope_cos.numel()
-        rc = self._append(self.h, layer, self._typed("qkv", qkv, _F32, n * (self.num_heads + 2 * self.kv_heads) * hd),
+        table, half = rope_cos.numel(), hd // 2
+        if table % half or (rope_cos.dim() > 1 and rope_cos.shape[-1] != half):
+            raise ValueError(f"rope_cos: expected rows of {half} angles, got {tuple(rope_cos.shape)}")
+        rc = self._append(self.h, layer, self._rows("qkv", qkv, n, (self.num_heads + 2 * self.kv_heads) * hd),
                           self._norm("q_norm", q_norm), self._norm("k_norm", k_norm),
-                          self._typed("rope_cos", rope_cos, _F32, 0), self._typed("rope_sin", rope_sin, _F32, table),
-                          table // (hd // 2), self._typed("positions", positions, _I32, n),
+                          self._typed("rope_cos", rope_cos, _F32, 0), self._typed("rope_sin", rope_sin, _F32, table, True),
+                          table // half, self._typed("positions", positions, _I32, n),
                           self._typed("slots", slots, _I32, n), n,
-                          self._typed("out", out, _F32, n * self.num_heads * hd), self._stream(stream))
+                          self._rows("out", out, n, self.num_heads * hd), self._stream(stream))
         if rc:
             _lib.check(rc, "qora_kv4_append")
         return out
@@ -141,9 +154,9 @@ class Kv4Cache:
     def write(self, layer: int, slots: torch.Tensor, k: torch.Tensor, v: torch.Tensor, stream=None):
         """Stores rows of keys (normed, rotated) and values [n][kv_heads * head_dim]."""
         n = slots.numel()
-        want = n * self.kv_heads * self.head_dim
-        rc = self._write(self.h, layer, self._typed("slots", slots, _I32, n), n, self._typed("k", k, _F32, want),
-                         self._typed("v", v, _F32, want), self._stream(stream))
+        width = self.kv_heads * self.head_dim
+        rc = self._write(self.h, layer, self._typed("slots", slots, _I32, n), n, self._rows("k", k, n, width),
+                         self._rows("v", v, n, width), self._stream(stream))
         if rc:
             _lib.check(rc, "qora_kv4_write")
 
@@ -151,12 +164,12 @@ class Kv4Cache:
         """The keys and values that the slots hold, f32 [n][kv_heads * head_dim]
         (rows of slot -1 are left as they were)."""
         n = slots.numel()
-        want = n * self.kv_heads * self.head_dim
+        width = self.kv_heads * self.head_dim
         if out is None:
-            out = tuple(torch.zeros(n, self.kv_heads * self.head_dim, device=slots.device) for _ in range(2))
+            out = tuple(torch.zeros(n, width, device=slots.device) for _ in range(2))
         k, v = out
-        rc = self._read(self.h, layer, self._typed("slots", slots, _I32, n), n, self._typed("k", k, _F32, want),
-                        self._typed("v", v, _F32, want), self._stream(stream))
+        rc = self._read(self.h, layer, self._typed("slots", slots, _I32, n), n, self._rows("k", k, n, width),
+                        self._rows("v", v, n, width), self._stream(stream))
         if rc:
             _lib.check(rc, "qora_kv4_read")
         return out
@@ -169,9 +182,9 @@ class Kv4Cache:
         n, width = q.shape[0], self.num_heads * self.head_dim
         if out is None:
             out = torch.empty(n, width, device=q.device)
-        rc = self._attend(self.h, layer, self._typed("q", q, _F32, n * width),
-                          self._typed("offsets", offsets, _I32, self.streams + 1), n, max_count,
-                          self._typed("out", out, _F32, n * width), self._stream(stream))
+        rc = self._attend(self.h, layer, self._rows("q", q, n, width),
+                          self._typed("offsets", offsets, _I32, self.streams + 1, True), n, max_count,
+                          self._rows("out", out, n, width), self._stream(stream))
         if rc:
             _lib.check(rc, "qora_kv4_attend")
         return out
