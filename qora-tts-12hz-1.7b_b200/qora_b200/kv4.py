@@ -28,6 +28,7 @@ from . import _lib
 from .engine import Context, _device_view, _raw_stream
 
 _F32, _I32 = torch.float32, torch.int32
+_F16_BITS = (torch.float16, torch.int16, torch.uint16)
 
 
 class Kv4Cache:
@@ -73,8 +74,10 @@ class Kv4Cache:
         return t.data_ptr()
 
     def _norm(self, name: str, t: torch.Tensor) -> int:
-        if t.element_size() != 2 or t.numel() < self.head_dim or t.get_device() != self._dev or not t.is_contiguous():
-            raise ValueError(f"{name}: expected {self.head_dim} f16 values on {self.device}")
+        if (t.dtype not in _F16_BITS or t.numel() != self.head_dim or t.get_device() != self._dev
+                or not t.is_contiguous()):
+            raise ValueError(f"{name}: expected {self.head_dim} f16 values (or their bits as int16) on {self.device}, "
+                             f"got {tuple(t.shape)} of {t.dtype} on {t.device}")
         return t.data_ptr()
 
     def _stream(self, stream) -> int:

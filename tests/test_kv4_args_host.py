@@ -1,7 +1,6 @@
 """Kv4Cache's checks of its arguments, without a GPU: a cache that is not there
 (CPU tensors stand for the device's) and entry points that only record that they
 were reached."""
-import numpy as np
 import pytest
 import torch
 
@@ -77,4 +76,14 @@ def test_right_shapes_pass(kv):
 def test_wrong_shapes_are_refused(kv, call):
     with pytest.raises(ValueError):
         call(kv)
+    assert kv.calls == []
+
+
+@pytest.mark.parametrize("norm", [torch.zeros(D, dtype=torch.bfloat16), torch.zeros(D), torch.zeros(2, D, dtype=torch.float16),
+                                  torch.zeros(2 * D, dtype=torch.float16)[::2], torch.zeros(D // 2, dtype=torch.float16)])
+@pytest.mark.parametrize("name", ["q_norm", "k_norm"])
+def test_norms_are_f16(kv, name, norm):
+    """bf16 has as many bytes, and would be read as other numbers."""
+    with pytest.raises(ValueError):
+        append(kv, **{name: norm})
     assert kv.calls == []
