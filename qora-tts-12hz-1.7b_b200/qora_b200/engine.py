@@ -6,6 +6,7 @@ compute goes through libqora_b200.so.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 
 import numpy as np
@@ -25,6 +26,11 @@ def _stream(stream=None) -> int:
 def _raw_stream(device: int) -> int:
     """The device's current stream (without a Stream object: these calls are short)."""
     return torch._C._cuda_getCurrentRawStream(device)
+
+
+def _results_on(stream):
+    """Where a call on `stream` allocates its results: memory of another stream's pool may still be written there."""
+    return contextlib.nullcontext() if stream is None else torch.cuda.stream(stream)
 
 
 def _dp(t: torch.Tensor | None):
@@ -384,7 +390,9 @@ def sample_probs(ctx: Context, logits: torch.Tensor, prev: torch.Tensor | None, 
     token out.  prev int32 [B][n] (repetition penalty) or None."""
     B, V = shape = logits.shape
     dev, f32 = ctx.device, torch.float32
-    out = out if out is not None else torch.empty_like(logits)
+    if out is None:
+        with _results_on(stream):
+            out = torch.empty_like(logits)
     n_prev = 0 if prev is None else prev.shape[-1]
     rc = ctx._L.qora_sample_probs(ctx.h, _rows_of("logits", logits, f32, shape, dev), B, V,
                                   _rows_of("prev", prev, torch.int32, (B, n_prev), dev) if n_prev else None, n_prev,
@@ -408,7 +416,8 @@ def verify_drafts(ctx: Context, drafts: torch.Tensor, draft_probs: torch.Tensor 
     V = target_probs.shape[-1]
     dev, i32, f32 = ctx.device, torch.int32, torch.float32
     if out is None:
-        out = (torch.empty(B, K + 1, dtype=i32, device=drafts.device), torch.empty(B, dtype=i32, device=drafts.device))
+        with _results_on(stream):
+            out = (torch.empty(B, K + 1, dtype=i32, device=drafts.device), torch.empty(B, dtype=i32, device=drafts.device))
     tokens, n_out = out
     rc = ctx._L.qora_verify_drafts(
         ctx.h, _rows_of("drafts", drafts, i32, (B, K), dev),

@@ -15,7 +15,9 @@ A speculative decode step of every stream, without a return to the host
     kv.advance(n_out, offsets=offsets)
 
 Tensors are on the context's device and contiguous; calls are asynchronous on
-the current stream (or `stream`).  One cache serves one stream at a time.
+the current stream, or on `stream`: what they are given has to be ready there
+and to live until it is done (Tensor.record_stream), and results that they
+allocate belong to it.  One cache serves one stream at a time.
 """
 from __future__ import annotations
 
@@ -25,7 +27,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from .engine import Context, _device_view, _raw_stream
+from .engine import Context, _device_view, _raw_stream, _results_on
 
 _F32, _I32 = torch.float32, torch.int32
 _F16_BITS = (torch.float16, torch.int16, torch.uint16)
@@ -109,8 +111,9 @@ class Kv4Cache:
         returns (slots [max_tokens], positions [max_tokens], offsets [streams + 1])."""
         if out is None:
             i32 = dict(dtype=torch.int32, device=self.device)
-            out = (torch.empty(max_tokens, **i32), torch.empty(max_tokens, **i32),
-                   torch.empty(self.streams + 1, **i32))
+            with _results_on(stream):
+                out = (torch.empty(max_tokens, **i32), torch.empty(max_tokens, **i32),
+                       torch.empty(self.streams + 1, **i32))
         slots, positions, offsets = out
         rc = self._reserve(self.h, self._typed("counts", counts, _I32, self.streams, True), max_tokens,
                            self._typed("slots", slots, _I32, max_tokens),
@@ -140,7 +143,8 @@ class Kv4Cache:
         normed and rotated queries [n][num_heads * head_dim]."""
         n, hd = qkv.shape[0], self.head_dim
         if out is None:
-            out = torch.empty(n, self.num_heads * hd, device=qkv.device)
+            with _results_on(stream):
+                out = torch.empty(n, self.num_heads * hd, device=qkv.device)
         table, half = rope_cos.numel(), hd // 2
         if table % half or (rope_cos.dim() > 1 and rope_cos.shape[-1] != half):
             raise ValueError(f"rope_cos: expected rows of {half} angles, got {tuple(rope_cos.shape)}")
@@ -169,7 +173,8 @@ class Kv4Cache:
         n = slots.numel()
         width = self.kv_heads * self.head_dim
         if out is None:
-            out = tuple(torch.zeros(n, width, device=slots.device) for _ in range(2))
+            with _results_on(stream):
+                out = tuple(torch.zeros(n, width, device=slots.device) for _ in range(2))
         k, v = out
         rc = self._read(self.h, layer, self._typed("slots", slots, _I32, n), n, self._rows("k", k, n, width),
                         self._rows("v", v, n, width), self._stream(stream))
@@ -184,7 +189,8 @@ class Kv4Cache:
         one stream (1 in a decode step).  Returns [n][num_heads * head_dim]."""
         n, width = q.shape[0], self.num_heads * self.head_dim
         if out is None:
-            out = torch.empty(n, width, device=q.device)
+            with _results_on(stream):
+                out = torch.empty(n, width, device=q.device)
         rc = self._attend(self.h, layer, self._rows("q", q, n, width),
                           self._typed("offsets", offsets, _I32, self.streams + 1, True), n, max_count,
                           self._rows("out", out, n, width), self._stream(stream))

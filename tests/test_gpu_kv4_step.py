@@ -52,6 +52,55 @@ def test_advance_within_what_was_reserved(ctx):  # noqa: F811
     assert list(kv.lengths()) == [4, 0, 27, 40] and _error(ctx) == 0
 
 
+# ------------------------------------------------------------ results on other streams
+def _late(stream, n, dtype):
+    """Work on `stream` that is still to come, which writes blocks of n values that the
+    allocator has back already."""
+    import torch
+    with torch.cuda.stream(stream):
+        blocks = [torch.empty(n, dtype=dtype, device="cuda") for _ in range(64)]
+        torch.cuda._sleep(100_000_000)                      # some 0.05 s
+        for t in blocks:
+            t.fill_(77)
+
+
+@pytest.mark.parametrize("what", ["reserve", "append", "read", "attend", "probs", "verify"])
+def test_results_of_a_call_on_another_stream(E, ctx, orc, what):  # noqa: F811
+    """`stream=` without `out`: what the current stream still has to do (writes to memory
+    that was freed there, or a fill of the result) does not reach the result."""
+    import torch
+    heads, kvh, hd, n = 4, 2, 64, 32
+    kv = _cache(ctx, 1, heads, kvh, hd, 256, 1, 32, 8)
+    qn, kn, cos, sin = (_dev(t) for t in _weights(orc, hd, 3))
+    g = torch.Generator(device="cuda").manual_seed(5)
+    qkv = torch.randn(n, (heads + 2 * kvh) * hd, generator=g, device="cuda")
+    counts = _i32([n])
+    slots, positions, offsets = kv.reserve(counts, n)
+    q = kv.append(0, qkv, qn, kn, cos, sin, positions, slots)
+    logits, u = torch.randn(n, 500, generator=g, device="cuda"), torch.rand(n, 3, generator=g, device="cuda")
+    target = torch.softmax(torch.randn(n, 3, 500, generator=g, device="cuda"), -1)
+    drafts = _i32(np.arange(2 * n).reshape(n, 2))
+    calls = {"reserve": (lambda **kw: kv.reserve(counts, n, **kw), [(n, torch.int32), (n, torch.int32), (2, torch.int32)]),
+             "append": (lambda **kw: kv.append(0, qkv, qn, kn, cos, sin, positions, slots, **kw), [(n * heads * hd, torch.float32)]),
+             "read": (lambda **kw: kv.read(0, slots, **kw), [(n * kvh * hd, torch.float32)] * 2),
+             "attend": (lambda **kw: kv.attend(0, q, offsets, n, **kw), [(n * heads * hd, torch.float32)]),
+             "probs": (lambda **kw: E.sample_probs(ctx, logits, None, E.default_params(), **kw), [(n * 500, torch.float32)]),
+             "verify": (lambda **kw: E.verify_drafts(ctx, drafts, None, target, u, **kw), [(n * 3, torch.int32), (n, torch.int32)])}
+    call, blocks = calls[what]
+    want = call()
+    want = [t.clone() for t in (want if isinstance(want, tuple) else (want,))]
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for size, dtype in blocks:
+        _late(torch.cuda.current_stream(), size, dtype)
+    got = call(stream=side)
+    got = got if isinstance(got, tuple) else (got,)
+    torch.cuda.synchronize()
+    assert _error(ctx) == 0
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
 # ------------------------------------------------------------ a step in one graph
 def test_captured_step_from_tables_to_lengths(E, ctx, orc):  # noqa: F811
     """reserve, append, attend, the logits' rows by stream, the distribution, verification
