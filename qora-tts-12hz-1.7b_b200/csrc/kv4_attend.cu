@@ -517,7 +517,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_attend(const AttendArgs a) 
                     if (edge) {  // whatever lies behind a row's last position counts as zero
 #pragma unroll
                         for (int i = 0; i < 4; i++)
-                            bp[i] = split_hi_lo(sc[nt][i] == 0.0f ? 0.0f : sc[nt][i] * scale_of(vs[c], i));
+                            bp[i] = split_hi_lo(u * kKv4Unit + g + 8 * i > limit[nt] ? 0.0f : sc[nt][i] * scale_of(vs[c], i));
                     } else {
 #pragma unroll
                         for (int i = 0; i < 4; i++) bp[i] = split_hi_lo(sc[nt][i] * scale_of(vs[c], i));

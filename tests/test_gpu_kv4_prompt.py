@@ -1,10 +1,10 @@
-"""The prompt kernel of attention over the 4-bit cache (k_kv4_prompt): every test
-here asserts first that its call reaches that kernel, by the rule that
-qora_kv4_attend chooses by."""
+"""The prompt kernel of attention over the 4-bit cache (k_kv4_prompt), and the
+other beside it: every test here asserts first which kernel its call reaches, by
+the rule that qora_kv4_attend chooses by."""
 import numpy as np
 import pytest
 
-from test_gpu_kv4 import E, _cache, _dev, _error, _i32, ctx  # noqa: F401
+from test_gpu_kv4 import E, _cache, _dev, _error, _filled, _i32, ctx  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -48,3 +48,33 @@ def test_sums_over_a_long_cache(ctx, heads, kvh, hd, n):  # noqa: F811
     assert _error(ctx) == 0
     worst = float(np.abs(out / np.float32(7 * 0.21875) - 1).max())
     assert worst <= total / 64 * 2.0 ** -24 + 2.0 ** -19, worst
+
+
+@pytest.mark.parametrize("heads,kvh,hd,lens,counts,most", [
+    (4, 2, 64, [37, 0, 90], [2, 3, 1], 3), (16, 8, 128, [37, 0, 90], [2, 3, 1], 3),
+    (32, 8, 128, [37, 0, 90], [50, 64, 20], 64), (32, 8, 64, [37, 0, 90], [70, 64, 40], 70)])
+def test_nan_values_reach_rows_that_hardly_weigh_them(ctx, heads, kvh, hd, lens, counts, most):  # noqa: F811
+    """A NaN value is in the sum whatever its weight, 0 by underflow included, in a
+    stream's last unit of positions as in any other."""
+    import torch
+    page, S = 64, len(lens)
+    prompt_case = most > 3
+    assert prompt_runs(heads, kvh, hd, S, sum(counts), most) == prompt_case
+    kv, offsets, held, rng = _filled(ctx, lens, counts, heads, kvh, hd, page, 97)
+    table, n = kv.state()["table"].cpu().numpy(), sum(counts)
+    slot = lambda b, p: int(table[b, p // page]) * page + p % page  # noqa: E731
+    # the stream's first key is far above that of the position with the NaN
+    top, low = _i32([slot(2, 0)]), 88                        # 88: the last unit holds positions 64 on
+    k, v = kv.read(1, top)
+    kv.write(1, top, torch.full_like(k, 40.0), v)
+    at = _i32([slot(2, low)])
+    k, v = kv.read(1, at)
+    half = v.clone()
+    half[:, :32] = float("nan")
+    kv.write(1, at, torch.full_like(k, -40.0), half)
+    q = np.abs(rng.standard_normal((n, heads, hd))).astype(np.float32) + 0.5
+    got = kv.attend(1, _dev(q.reshape(n, -1)), offsets, most)
+    nan = torch.isnan(got).view(n, heads, hd).cpu().numpy()
+    want = np.zeros_like(nan)
+    want[n - counts[2]:, :heads // kvh, :32] = True
+    assert np.array_equal(nan, want) and _error(ctx) == 0
