@@ -670,7 +670,8 @@ int clusters_of(const qora_kv4 *kv, int (&n)[3]) {
 }
 
 // The cluster size goes by the items (stream, kv head, row tile) that the call may
-// have: with few, a wide cluster puts more blocks on each; with many, narrow ones
+// have, at most one stream a token (a cache of 64 streams with one of 16384 positions
+// at work: 53 us by the cache's streams, 23.5 by the call's): with few, a wide cluster puts more blocks on each; with many, narrow ones
 // leave no multiprocessor without a block (33 clusters of 8, 71 of 4 or 148 of 2
 // run at once).  Measured at 16 / 8 heads of 128, one token: 1 stream of 16384
 // positions 23.4 us with clusters of 8, 34.2 with 4; 8 streams of 4096 23.1 us with
@@ -697,9 +698,12 @@ int setup(qora_kv4 *kv) {
 // but do not fit 128 registers: 6 drafts of 16 streams of 4096 took 58 us against 40.)
 template <int D>
 int launch_rows(const qora_kv4 *kv, const AttendArgs &a, int64_t rows, cudaStream_t st) {
-    const int64_t items4 = (int64_t)kv->streams * kv->kvh * ((rows + 3) / 4);
-    const int nt = rows <= 4 || items4 <= kv->clusters[0][0] ? 1 : 2;
-    const int64_t items = nt == 1 ? items4 : (int64_t)kv->streams * kv->kvh * ((rows + 7) / 8);
+    // the most items of R rows that the call's tokens make: every stream that has one ends
+    // in a tile of its own
+    const int64_t S = std::min(kv->streams, a.tokens), all = (int64_t)a.tokens * (a.heads / kv->kvh);
+    const auto most = [&](int R) { return kv->kvh * std::min(S * ((rows + R - 1) / R), S + all / R); };
+    const int nt = rows <= 4 || most(4) <= kv->clusters[0][0] ? 1 : 2;
+    const int64_t items = most(4 * nt);
     const auto &n = kv->clusters[nt - 1];
     return nt == 1 ? launch<D, 1>(kv, a, n, items, st) : launch<D, 2>(kv, a, n, items, st);
 }

@@ -189,3 +189,29 @@ def test_captured_step_from_tables_to_lengths(E, ctx, orc):  # noqa: F811
     graph.replay()                                          # with pages again it goes on
     torch.cuda.synchronize()
     assert _error(ctx) == 0 and all(a > b for a, b in zip(kv.lengths(), lens[:3]))
+
+
+# ------------------------------------------------------------ a large cache with little work
+@pytest.mark.parametrize("streams,count", [(64, 1), (64, 2), (300, 2)])
+def test_attend_goes_by_the_streams_with_tokens(ctx, streams, count):  # noqa: F811
+    """One stream's call of a token or two in a cache of many: the work is split as in a cache of one, so
+    the bits are the same."""
+    import torch
+    heads, kvh, hd, length, page = 16, 8, 128, 5000, 64
+    pool = -(-(length + count) // page)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    k, v = (torch.randn(length + count, kvh * hd, generator=g, device="cuda") for _ in range(2))
+    q = torch.randn(count, heads * hd, generator=g, device="cuda")
+    got = []
+    for S, b in ((1, 0), (streams, streams - 3)):
+        kv = _cache(ctx, 1, heads, kvh, hd, pool * page, S, page, pool)
+        n = np.zeros(S, np.int32)
+        n[b] = length
+        slots, _, _ = kv.reserve(_i32(n), length)
+        kv.write(0, slots, k[:length], v[:length])
+        kv.advance(_i32(n))
+        n[b] = count
+        slots, _, offsets = kv.reserve(_i32(n), count)
+        kv.write(0, slots, k[length:], v[length:])
+        got.append(kv.attend(0, q, offsets, count))
+    assert _error(ctx) == 0 and torch.equal(*got)
