@@ -300,7 +300,8 @@ int qora_kv4_append(qora_kv4 *kv, int32_t layer, const float *qkv, const uint16_
 /* Stores rows of keys (normed and rotated) and values [rows][kv_heads head_dim]
  * f32 in 4 bits at their slots, e.g. those of an f32 cache; _read gives the
  * values that slots hold.  Slots as in _append.  Writing what was read stores
- * the same codes and scales. */
+ * the same codes and scales wherever the scale is 2^-21 or more; below, f16's
+ * steps are too wide for that (values under 3.4e-6 may change once more). */
 int qora_kv4_write(qora_kv4 *kv, int32_t layer, const int32_t *slots, int32_t rows, const float *k,
                    const float *v, void *stream);
 int qora_kv4_read(qora_kv4 *kv, int32_t layer, const int32_t *slots, int32_t rows, float *k,

@@ -215,3 +215,27 @@ def test_attend_goes_by_the_streams_with_tokens(ctx, streams, count):  # noqa: F
         kv.write(0, slots, k[length:], v[length:])
         got.append(kv.attend(0, q, offsets, count))
     assert _error(ctx) == 0 and torch.equal(*got)
+
+
+# ------------------------------------------------------------ small values
+@pytest.mark.parametrize("hd", [64, 128])
+def test_writing_what_was_read_at_the_smallest_scales(ctx, hd):  # noqa: F811
+    """From 2^-21 on the same codes and scales; below, what the definition gives for the
+    values that were read."""
+    rng = np.random.default_rng(hd)
+    kvh, n = 2, 64
+    kv = _cache(ctx, 2, 2, kvh, hd, 64, 1, 32, 2)
+    size = 2.0 ** rng.integers(-26, -12, (n, kvh, hd // 32, 1)) * 7
+    x = [(size * rng.uniform(-1, 1, (n, kvh, hd // 32, 32))).astype(np.float32).reshape(n, -1) for _ in range(2)]
+    slots = _i32(rng.permutation(64))
+    kv.write(0, slots, *map(_dev, x))
+    once = kv.read(0, slots)
+    kv.write(1, slots, *once)
+    twice = kv.read(1, slots)
+    for src, a, b in zip(x, once, twice):
+        a, b = a.cpu().numpy(), b.cpu().numpy()
+        rows = lambda t: t.reshape(n, kvh, hd)  # noqa: E731
+        assert np.array_equal(rows(a), R.held(rows(src))) and np.array_equal(rows(b), R.held(rows(a)))
+        keep = R.quantise(rows(src))[1] >= 2.0 ** -21
+        assert np.array_equal(a.reshape(n, kvh, -1, 32)[keep], b.reshape(n, kvh, -1, 32)[keep]) and not np.array_equal(a, b)
+    assert _error(ctx) == 0

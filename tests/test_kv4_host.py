@@ -112,3 +112,19 @@ def test_accept_refuses_null_arguments(lib):
     assert lib.qora_kv4_accept(None, one, one, None) == INVALID
     assert lib.qora_kv4_accept(one, None, one, None) == INVALID
     assert lib.qora_kv4_accept(one, one, None, None) == INVALID
+
+
+def test_writing_what_was_read_keeps_scales_from_2_to_the_minus_21():
+    """By the definition: code 7 is used, so amax / 7 of what is held is the scale again.
+    Below 2^-21 f16 has fewer than 3 bits for a scale, and that no longer holds."""
+    import kv4_ref as R
+    rng = np.random.default_rng(0)
+    changed = 0
+    for e in range(-26, 20):
+        x = (2.0 ** e * 7 * np.exp2(rng.random((3000, 1))) * rng.uniform(-1, 1, (3000, 32))).astype(np.float32)
+        codes, scales = R.quantise(x)
+        again, scales2 = R.quantise(R.held(x))
+        moved = (codes != again).any(-1) | (scales != scales2)
+        assert not moved[scales >= 2.0 ** -21].any()
+        changed += int(moved.sum())
+    assert changed > 0
