@@ -4,7 +4,8 @@ the rule that qora_kv4_attend chooses by."""
 import numpy as np
 import pytest
 
-from test_gpu_kv4 import E, _cache, _dev, _error, _filled, _i32, ctx  # noqa: F401
+import kv4_ref as R
+from test_gpu_kv4 import E, _cache, _check, _dev, _error, _filled, _i32, ctx  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -78,3 +79,87 @@ def test_nan_values_reach_rows_that_hardly_weigh_them(ctx, heads, kvh, hd, lens,
     want = np.zeros_like(nan)
     want[n - counts[2]:, :heads // kvh, :32] = True
     assert np.array_equal(nan, want) and _error(ctx) == 0
+
+
+# heads, kv heads, head_dim, page, lengths, new tokens, max_count: streams of one, several
+# and no row tiles of 128, of 1, 2, 3, 4 and more key tiles of 64
+UNDERSTATED = [
+    (32, 8, 128, 32, [70, 0, 161, 5], [200, 40, 40, 40], 32),
+    (32, 8, 128, 64, [0, 30, 0, 400], [90, 200, 0, 180], 33),
+    (32, 8, 64, 64, [70, 0, 161, 5], [200, 40, 40, 40], 40),
+    (24, 8, 64, 32, [3, 64, 129], [260, 130, 2], 90),
+]
+
+
+@pytest.mark.parametrize("heads,kvh,hd,page,lens,counts,most", UNDERSTATED)
+def test_a_block_takes_further_row_tiles(ctx, heads, kvh, hd, page, lens, counts, most):  # noqa: F811
+    """max_count below the tokens of some streams: the grid has fewer row tiles than
+    they have, so blocks take several in turn."""
+    assert prompt_runs(heads, kvh, hd, len(lens), sum(counts), most) and heads // kvh * max(counts) > 128
+    kv, offsets, held, rng = _filled(ctx, lens, counts, heads, kvh, hd, page, 90 + hd)
+    q = (1.5 * rng.standard_normal((sum(counts), heads, hd))).astype(np.float32)
+    got = _check(kv, q, offsets, held, lens, counts, heads, kvh, hd, most)
+    # a row's result does not depend on which block takes its tile, nor on the time
+    assert prompt_runs(heads, kvh, hd, len(lens), sum(counts), max(counts))
+    for mc in (most, max(counts)):
+        again = _check(kv, q, offsets, held, lens, counts, heads, kvh, hd, mc)
+        assert np.array_equal(again.view(np.uint32), got.view(np.uint32))
+    assert _error(ctx) == 0
+
+
+@pytest.mark.parametrize("heads,kvh,hd,page,lens,counts", [(32, 8, 64, 32, [3, 0, 70], [90, 70, 11]),
+                                                          (16, 16, 128, 64, [200, 7], [129, 90])])
+def test_captured_prompt_of_many_rows_replays(ctx, heads, kvh, hd, page, lens, counts):  # noqa: F811
+    """Lengths, offsets and tables are read at each replay; on a stream of its own beside
+    a prompt of another cache."""
+    import torch
+    n, most = sum(counts), max(counts)
+    assert prompt_runs(heads, kvh, hd, len(lens), n, most)
+    kv, offsets, held, rng = _filled(ctx, lens, counts, heads, kvh, hd, page, 95)
+    other, offsets2, _, _ = _filled(ctx, lens, counts, heads, kvh, hd, page, 96)
+    q = rng.standard_normal((n, heads, hd)).astype(np.float32)
+    qd, out, side = _dev(q.reshape(n, -1)), torch.zeros(n, heads * hd, device="cuda"), torch.cuda.Stream()
+    want = other.attend(1, qd, offsets2, most)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        kv.attend(1, qd, offsets, most, out=out)
+    for now in (counts, [c // 3 for c in counts], [0] * (len(counts) - 1) + [1]):
+        offsets.copy_(_i32(np.concatenate([[0], np.cumsum(now)])))
+        out.fill_(7.0)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            graph.replay()
+        beside = other.attend(1, qd, offsets2, most)
+        torch.cuda.synchronize()
+        assert bool((beside == want).all())
+        got, at = out.cpu().numpy(), 0
+        for b, c in enumerate(now):
+            if c:
+                ref, bound = R.attend(q[at:at + c], held[b][0][:lens[b] + c], held[b][1][:lens[b] + c], lens[b], heads, kvh)
+                assert np.all(np.abs(got[at:at + c].reshape(c, heads, hd) - ref) <= bound)
+            at += c
+        assert (got[at:] == 7.0).all()
+    assert _error(ctx) == 0
+
+
+def test_prompts_on_two_streams_beside_drafts(ctx):  # noqa: F811
+    """Two caches' prompts, of head_dim 64 and 128, and a third's drafts at the same time."""
+    import torch
+    shapes = [((32, 8, 64, 64), [70, 0], [90, 80], 90), ((32, 8, 128, 32), [5, 33, 90], [60, 50, 40], 60),
+              ((32, 8, 128, 64), [900, 33, 0, 5], [5, 0, 3, 6], 6)]
+    jobs = []
+    for i, (shape, lens, counts, most) in enumerate(shapes):
+        assert prompt_runs(*shape[:3], len(lens), sum(counts), most) == (i < 2)
+        kv, offsets, held, rng = _filled(ctx, lens, counts, *shape, 100 + i)
+        q = _dev(rng.standard_normal((sum(counts), shape[0] * shape[2])).astype(np.float32))
+        jobs.append((kv, q, offsets, most, kv.attend(1, q, offsets, most), torch.zeros_like(q), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for kv, q, offsets, most, want, out, s in jobs:
+            with torch.cuda.stream(s):
+                kv.attend(1, q, offsets, most, out=out)
+    torch.cuda.synchronize()
+    for kv, q, offsets, most, want, out, s in jobs:
+        assert bool((out == want).all())
+    assert _error(ctx) == 0

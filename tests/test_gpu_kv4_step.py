@@ -1,6 +1,8 @@
 """A speculative step over the 4-bit cache as a whole, and what its calls do at
 its edges: streams without work, refused reservations, calls on other streams, one
-captured graph from block tables to lengths."""
+captured graph from block tables to lengths, and attention against the f32 cache's."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
@@ -239,3 +241,77 @@ def test_writing_what_was_read_at_the_smallest_scales(ctx, hd):  # noqa: F811
         keep = R.quantise(rows(src))[1] >= 2.0 ** -21
         assert np.array_equal(a.reshape(n, kvh, -1, 32)[keep], b.reshape(n, kvh, -1, 32)[keep]) and not np.array_equal(a, b)
     assert _error(ctx) == 0
+
+
+# ------------------------------------------------------------ the largest cache
+def test_reserve_over_the_largest_pool(ctx):  # noqa: F811
+    """2^20 pages and 4096 streams: the widest cluster with as much shared memory as a call takes."""
+    S, page, pool, max_pos = 4096, 32, 1 << 20, 1 << 14
+    rng = np.random.default_rng(1)
+    lens = rng.integers(0, 8000, S)
+    counts = rng.integers(0, 70, S)
+    kv = _cache(ctx, 1, 1, 1, 64, max_pos, S, page, pool)
+    keep = -(-lens // page)
+    table = np.full((S, max_pos // page), -1, np.int32)
+    order = rng.permutation(pool)[:int(keep.sum())]
+    table[np.arange(table.shape[1]) < keep[:, None]] = order
+    st = kv.state()
+    st["table"].copy_(_i32(table))
+    st["lengths"].copy_(_i32(lens))
+    tokens = int(counts.sum()) + 9
+    got = kv.reserve(_i32(counts), tokens)
+    assert _error(ctx) == 0
+    want = R.reserve(table, lens, counts, page, pool, max_pos, tokens)
+    for x, y in zip((st["table"],) + tuple(got), want):
+        assert np.array_equal(x.cpu().numpy(), y)
+
+
+# ------------------------------------------------------------ against the f32 cache
+@pytest.mark.parametrize("heads,kvh,hd,length", [(4, 2, 128, 0), (16, 8, 128, 333), (4, 4, 64, 70), (8, 2, 64, 31)])
+def test_attend_agrees_with_the_f32_cache(E, ctx, orc, heads, kvh, hd, length):  # noqa: F811
+    """qora_kv_attend and qora_kv4_attend over the same keys and values: the f32 slab
+    holds what the 4-bit rows stand for, and the new token's own row is one that 4 bits
+    hold exactly (a key norm of zeros, values of whole codes)."""
+    import torch
+    from qora_b200 import _lib
+    from qora_b200.engine import _device_view
+    rng = np.random.default_rng(hd + length)
+    S, max_pos = 2, 512
+    qn, _, cos, sin = (_dev(t) for t in _weights(orc, hd, 6))
+    kn = torch.zeros(hd, dtype=torch.float16, device="cuda")
+    kv4 = _cache(ctx, 1, heads, kvh, hd, max_pos, S, 32, 2 * max_pos // 32)
+    slots, _, _ = kv4.reserve(_i32([length + 1] * S), S * (length + 1))
+    k, v = (_dev(rng.standard_normal((S * (length + 1), kvh * hd)).astype(np.float32)) for _ in range(2))
+    kv4.write(0, slots, k, v)
+    kv4.advance(_i32([length] * S))
+    k, v = (t.view(S, length + 1, kvh, hd).transpose(1, 2) for t in kv4.read(0, slots))
+    kv = E.KvCache(ctx, 1, kvh, hd, max_pos, S)
+    ptr = [C.c_void_p() for _ in range(3)]
+    _lib.call("qora_kv_layer_ptrs", kv.h, 0, *(C.byref(p) for p in ptr))
+    for p, rows in zip(ptr, (k, v)):
+        _device_view(p.value, (S, kvh, max_pos, hd), "<f4", "cuda:0", kv)[:, :, :length] = rows[:, :, :length]
+    _device_view(ptr[2].value, (S,), "<i4", "cuda:0", kv).fill_(length)
+    qkv = _dev(rng.standard_normal((S, (heads + 2 * kvh) * hd)).astype(np.float32))
+    codes = rng.integers(-7, 8, (S, kvh * hd // 32, 32))
+    codes[..., 5] = 7
+    qkv[:, -kvh * hd:] = _dev((codes * 0.25).astype(np.float32).reshape(S, -1))
+    positions = _i32([length] * S)
+    full = kv.attend(0, qkv, heads, qn.view(torch.int16), kn.view(torch.int16), cos, sin, positions)
+    slots, positions, offsets = kv4.reserve(_i32([1] * S), S)
+    q = kv4.append(0, qkv, qn, kn, cos, sin, positions, slots)
+    mine = kv4.attend(0, q, offsets, 1)
+    assert _error(ctx) == 0
+    # Each is within its own bound of the definition: kv4_ref.attend's for the 4-bit
+    # kernel; for f32 a score's head_dim products and sums, 2^-24 of its sum of
+    # magnitudes each, two roundings of q before, twice that for a probability, and 2^-19
+    # with 2^-24 a position for exponentials and sums.
+    kk, vv = kv4.read(0, slots)
+    for b in range(S):
+        ks = np.concatenate([k[b, :, :length].transpose(0, 1).cpu().numpy(), kk[b].view(1, kvh, hd).cpu().numpy()])
+        vs = np.concatenate([v[b, :, :length].transpose(0, 1).cpu().numpy(), vv[b].view(1, kvh, hd).cpu().numpy()])
+        qs = q[b].view(1, heads, hd).cpu().numpy()
+        ref, bound = R.attend(qs, ks, vs, length, heads, kvh)
+        size = max(np.abs(ks[:, h * kvh // heads]).dot(np.abs(qs[0, h])).max() for h in range(heads)) / np.sqrt(hd)
+        wide = (2 * (hd + 16) * 2.0 ** -24 * size + 2.0 ** -19 + (length + 1) * 2.0 ** -24) * np.abs(vs).max()
+        a, f = (t[b].view(1, heads, hd).cpu().numpy() for t in (mine, full))
+        assert np.all(np.abs(a - ref) <= bound) and np.all(np.abs(a - f) <= bound + wide)
