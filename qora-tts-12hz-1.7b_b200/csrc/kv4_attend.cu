@@ -411,6 +411,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_kv4_attend(const AttendArgs a) 
             const bool here = mbar_wait_bounded(&sm.full[warp][st], ((turn + k) / kStages) & 1, a.err);
             if (__any_sync(0xffffffffu, !here)) {
                 dead = true;
+                // no copy is left in flight behind the block (a limit again)
+                for (int j = k; j < min(mine, k + kStages); j++)
+                    mbar_wait_bounded(&sm.full[warp][(turn + j) % kStages], ((turn + j) / kStages) & 1, a.err);
                 break;
             }
             const uint8_t *unit = &sm.ring[warp][st][0];

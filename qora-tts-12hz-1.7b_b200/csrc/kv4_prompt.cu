@@ -80,7 +80,7 @@ struct Sm {
     unsigned vnan[4][2][D / 32];           // positions of a unit whose value scale is NaN, by group
     unsigned most[2][2][kUnpackWarps];     // largest scales: keys, values
     alignas(8) uint64_t info[4];           // these are written (k_full may be a phase too far by then)
-    uint64_t q_full, k_full[2], v_full[2], s_full[2], p_full[2], o_full[2], o_free;
+    uint64_t q_full, k_full[2], v_full[2], s_full[2], p_full[2], o_full[2], o_free, drained;
     uint32_t tmem;
     int abort;
 };
@@ -372,6 +372,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const PromptArgs a) 
         for (int i = 0; i < 4; i++) mbar_init(&sm.info[i], 2 * kUnpackWarps);
         mbar_init(&sm.q_full, kSoftWarps);
         mbar_init(&sm.o_free, kSoftWarps);
+        mbar_init(&sm.drained, 1);
         sm.abort = 0;
         mbar_fence_init();
     }
@@ -672,6 +673,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv4_prompt(const PromptArgs a) 
                 // beside the products of the tiles around it
                 bool go = arrived(&sm.q_full, turn) && scores(0) && (ntiles < 2 || scores(1));
                 for (int it = 0; go && it < ntiles; it++) go = values(it) && (it + 2 >= ntiles || scores(it + 2));
+                if (!go) {  // products are left behind by no block: their operands and tensor memory go with it
+                    tc::commit(&sm.drained);
+                    mbar_wait_bounded(&sm.drained, 0, a.err);
+                }
             }
             __syncwarp();
         });
