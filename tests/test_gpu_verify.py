@@ -134,6 +134,33 @@ def test_probs_zeros_of_both_signs_are_equal(E, ctx, V, top_k):
             assert np.array_equal(got[r] > 0, R.probs(x[r], None, 0.9, top_k, top_p, 1.0) > 0)
 
 
+@pytest.mark.parametrize("V,n_prev", [(300, 3000), (2048, 4096), (50000, 4096), (50001, 777)])
+def test_probs_of_a_long_history(E, ctx, V, n_prev):
+    """Thousands of mentions, most of a few tokens, some outside the vocabulary."""
+    rng = np.random.default_rng(V)
+    x = (3 * rng.standard_normal((3, V))).astype(np.float32)
+    prev = rng.integers(-5, V + 5, (3, n_prev)).astype(np.int32)
+    prev[1, ::2] = 7                                        # one token said n_prev / 2 times
+    prev[2, : n_prev // 2] = rng.integers(0, 9, n_prev // 2)
+    x[1, 7], x[2, :9] = 2.0, np.linspace(-1, 1, 9)
+    penalty = 1.0005                                        # 2000 times: a factor of e
+    params = E._lib.SampleParams(0.9, 200, 1.0, penalty)
+    got = E.sample_probs(ctx, _dev(x), _dev(prev), params).cpu().numpy()
+    assert _error(ctx) == 0
+    assert np.array_equal(got, E.sample_probs(ctx, _dev(x), _dev(prev), params).cpu().numpy())
+    for r in range(3):
+        ref = R.probs(x[r], prev[r], 0.9, 200, 1.0, penalty)
+        # an f32 logit after t mentions has t roundings, and the difference of two of them is
+        # divided by the temperature; its largest value is 15.  What the roundings may swap at
+        # the border of top_k is within that of each other too
+        t = np.bincount(prev[r][(prev[r] >= 0) & (prev[r] < V)], minlength=V).max()
+        tol = 2.0 ** -21 + 2 * (t + 2) * 2.0 ** -24 * 15 / 0.9
+        same = (got[r] > 0) == (ref > 0)
+        assert np.all(np.abs(got[r] - ref)[same] <= tol * ref[same] + 1e-38)
+        edge = ref[ref > 0].min()
+        assert np.all(np.abs(np.maximum(got[r], ref)[~same] - edge) <= 2 * tol * edge)
+
+
 def test_probs_agree_with_the_sampler(E, ctx):
     """qora_sample draws what the cumulative probabilities give for its random numbers."""
     import torch
