@@ -550,6 +550,35 @@ int rows_args(const char *who, qora_kv4 *kv, int32_t layer, const int32_t *slots
     return QORA_OK;
 }
 
+size_t reserve_smem(const qora_kv4 *kv) {
+    return ((size_t)((kv->pool_pages + 31) / 32) + 3 * (size_t)kv->streams) * 4;
+}
+
+// What k_kv4_reserve's launches need, once for the cache: its attributes, and how many
+// blocks of a cluster the device can place at once (16 is no size that it has to).
+int reserve_setup(qora_kv4 *kv) {
+    static std::atomic<uint64_t> done;
+    QORA_TRY(allow_smem(k_kv4_reserve, ((1 << 20) / 32 + 3 * kKv4MaxStreams) * 4, kv->ctx->device, done));
+    QORA_CUDA(cudaFuncSetAttribute(k_kv4_reserve, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    for (kv->wide = kResCluster; kv->wide > 1; kv->wide >>= 1) {
+        cudaLaunchConfig_t cfg = {};
+        cudaLaunchAttribute at;
+        cfg.gridDim = dim3(1, kv->wide);
+        cfg.blockDim = dim3(kResThreads);
+        cfg.dynamicSmemBytes = reserve_smem(kv);
+        at.id = cudaLaunchAttributeClusterDimension;
+        at.val.clusterDim.x = 1;
+        at.val.clusterDim.y = kv->wide;
+        at.val.clusterDim.z = 1;
+        cfg.attrs = &at;
+        cfg.numAttrs = 1;
+        int n = 0;
+        QORA_CUDA(cudaOccupancyMaxActiveClusters(&n, k_kv4_reserve, &cfg));
+        if (n > 0) break;
+    }
+    return QORA_OK;
+}
+
 int advance(qora_kv4 *kv, const int32_t *counts, const int32_t *offsets, void *stream) {
     DeviceGuard dg;
     QORA_TRY(dg.set(kv->ctx->device));
@@ -604,6 +633,7 @@ int qora_kv4_create(qora_ctx *ctx, int32_t num_layers, int32_t num_heads, int32_
     if (rc == QORA_OK) rc = kv->table.alloc((size_t)streams * kv->pages_per_stream * 4);
     if (rc == QORA_OK) rc = kv->len.alloc((size_t)streams * 4);
     if (rc == QORA_OK) rc = kv->len.zero();
+    if (rc == QORA_OK) rc = reserve_setup(kv);
     if (rc == QORA_OK) rc = kv4_attend_setup(kv);
     if (rc == QORA_OK && cudaMemsetAsync(kv->table.p, 0xff, kv->table.bytes, nullptr) != cudaSuccess)
         rc = set_error(QORA_ERR_CUDA, "qora_kv4_create: memset failed");
@@ -675,15 +705,11 @@ int qora_kv4_reserve(qora_kv4 *kv, const int32_t *counts, int32_t max_tokens, in
     a.pages_per_stream = kv->pages_per_stream;
     a.pool_pages = kv->pool_pages;
     a.max_tokens = max_tokens;
-    const size_t smem = ((size_t)((kv->pool_pages + 31) / 32) + 3 * (size_t)kv->streams) * 4;
-    static std::atomic<uint64_t> done;
-    QORA_TRY(allow_smem(k_kv4_reserve, ((1 << 20) / 32 + 3 * kKv4MaxStreams) * 4, kv->ctx->device, done));
     // a cluster pays where there are many table entries and tokens: 16448 of them take
     // 8.8 us by one block and 10.5 by a cluster, 32896 9.9 and 9.3, 66048 16.3 and 11.5
     const bool wide = (int64_t)kv->streams * kv->pages_per_stream + max_tokens > 24576;
-    const unsigned nr = wide ? kResCluster : 1;
-    if (wide) QORA_CUDA(cudaFuncSetAttribute(k_kv4_reserve, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    return launch_ex(k_kv4_reserve, dim3(1, nr), dim3(kResThreads), smem, as_stream(stream), nr, a);
+    const unsigned nr = wide ? kv->wide : 1;
+    return launch_ex(k_kv4_reserve, dim3(1, nr), dim3(kResThreads), reserve_smem(kv), as_stream(stream), nr, a);
 }
 
 int qora_kv4_advance(qora_kv4 *kv, const int32_t *counts, void *stream) {

@@ -34,6 +34,7 @@ struct qora_kv4 {
     int page_pos = 0, page_shift = 0, pages_per_stream = 0, pool_pages = 0;
     qora::DevBuf pages, table, len;
     int clusters[2][3] = {};  // attend: clusters that run at once, by kernel and cluster size
+    int wide = 0;             // reserve: blocks of its wide cluster
 };
 
 namespace qora {
