@@ -315,7 +315,9 @@ int qora_kv4_read(qora_kv4 *kv, int32_t layer, const int32_t *slots, int32_t row
  * as some other page; both are QORA_ERR_RANGE at the next
  * qora_ctx_check_device_error.  max_count: the most tokens that one stream
  * has in this call as the host knows it (1 in a decode step), by which the
- * kernel is chosen; any value >= 1 gives right results.  Deterministic. */
+ * kernel is chosen; any value >= 1 gives right results.  The same call gives the
+ * same bits; another max_count, or other streams in the call, by which the work
+ * is split, may change a stream's last bits. */
 int qora_kv4_attend(qora_kv4 *kv, int32_t layer, const float *q, const int32_t *offsets,
                     int32_t tokens, int32_t max_count, float *out, void *stream);
 

@@ -24,7 +24,7 @@ namespace {
 //
 // One cluster does it all (one launch, no workspace).  Every block scans the
 // streams' counts for itself (they are few); the table entries are marked by
-// all warps, 256 entries at a time with eight loads in flight; each block then
+// all warps, in pieces of 128 with 24 loads of a lane in flight; each block then
 // joins its share of the bit maps through distributed shared memory and hands
 // out the free pages in it; tokens are spread over all threads, which look
 // their stream up in the scanned offsets.  What bounds it is latency: 512 streams
@@ -450,7 +450,7 @@ __device__ __forceinline__ bool row_place(const RowArgs &a, int slot, int &page,
 // in 4 bits; v heads stored in 4 bits.  What bounds the large case is the way from
 // a multiprocessor to the L2 cache (69 % of its cycles): q rows in f32, and the
 // 2-byte pieces that 4-bit rows are written in, each a request of its own.  8191
-// rows of 16 / 8 heads of 128 take 54 us, against 56 to 66 with two rows or two
+// rows of 16 / 8 heads of 128 take 54 us in a loop of their own, against 56 to 66 with two rows or two
 // groups of heads a warp, and 83 with warps that fetch ahead and stay.
 template <int D>
 __global__ void __launch_bounds__(kRowWarps * 32, 6) k_kv4_append(const RowArgs a) {

@@ -27,7 +27,7 @@
 // several blocks share meet in distributed shared memory, in block order, so
 // there is no workspace and the result does not depend on timing.
 //
-// One token of 32 streams of 4096 positions, 16 / 8 heads of 128: 45 us, 3.4 TB/s
+// One token of 32 streams of 4096 positions, 16 / 8 heads of 128: 44 us, 3.4 TB/s
 // of cache read (of 16384: 5.4 TB/s).  A launch costs some 8 us besides the units:
 // lengths, tables, first copies and the join, one after the other.  The units are
 // bound by instructions: some 780 for 32 positions at a tile of 4 rows, issued in
@@ -721,7 +721,10 @@ namespace {
 // rows a kv head, 63 / 51 with 32, 113 / 51 with 64; 32 streams of 4096 118 / 215 with
 // 16, 207 / 216 with 32, 317 / 216 with 48; 4 streams of 4000 60 / 88 with 64, 100 / 90
 // with 96; one stream of 1000 22 / 29 with 128, of 8000 61 / 165.  At head_dim 64, 16
-// streams of 2000 positions: 40 / 41 with 32 rows, 58 / 41 with 48.
+// streams of 2000 positions: 40 / 41 with 32 rows, 58 / 41 with 48.  (Rows are all that
+// the host knows: lengths lie on the device, and one kernel takes all streams of a call.
+// 63 streams of 4096 with one token beside a prompt of 2048 take 529 us here, where calls
+// of their own take 83 and 168.)
 bool prompt_pays(const qora_kv4 *kv, int64_t tokens, int64_t max_count, int64_t rows) {
     if (rows <= 24) return false;
     const int64_t G = kv->heads / kv->kvh, streams = std::min<int64_t>(kv->streams, tokens);

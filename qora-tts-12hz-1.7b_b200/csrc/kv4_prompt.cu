@@ -22,8 +22,9 @@
 // P's columns follow).  O of each tile is added in f32 registers, because the
 // tensor core's own additions do not round to nearest.
 //
-// 2 prompts of 2048 and some 1700 tokens, 16 / 8 heads of 128: 121 us, 191 TFLOP/s of
-// the two products (three times that on the tensor cores).  What bounds it is the
+// 2 prompts of 2048 and some 1700 tokens, 16 / 8 heads of 128: 124 us in a captured loop,
+// 187 TFLOP/s of the two products (three times that on the tensor cores), and 131 to 136
+// as one call among others.  What bounds it is the
 // softmax warps' chain of a tile, some 2400 cycles of wait, maximum, exponentials,
 // P and sum of O, against 1540 of products; and 6 us a block outside its tiles.
 // Unpacking in the same warps as the issue of products took 360 us, one group of

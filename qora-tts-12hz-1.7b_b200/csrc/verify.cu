@@ -35,7 +35,7 @@ constexpr int kMaxCluster = 8;
 // radix selection over the slices decides exactly.  Exponentials and
 // sums of the kept are in 64 bits: the order and the top_p border are decided
 // by values next to each other.
-// 96 rows of 151936 with top_k 50: 54.5 us, 2.1 TB/s.  Memory is busy 14 % of that:
+// 96 rows of 151936 with top_k 50: 52.5 us in a captured loop, 2.2 TB/s.  Memory is busy 14 % of that:
 // a block lives some 17 us, of which the read is 4 and the rest barriers of the
 // block and the cluster, and shared memory lets 296 of the 768 blocks run at once.
 constexpr int kBins = 256;
@@ -566,7 +566,8 @@ __global__ void __launch_bounds__(kVThreads) k_sample_probs(const ProbsArgs a) {
 // that neither comparison turns on rounding.  Weights that are not positive
 // (NaN among them) count as zero.  A stream of count -1 is idle: nothing of it is
 // read, and it gets no token.
-// 64 streams of 5 drafts at 151936: 23.5 us (one row read where all pass, two where a
+// 64 streams of 5 drafts at 151936: 24.8 us in a captured loop, 28 as one call among
+// others (one row read where all pass, two where a
 // draft is rejected: 58 MB).  What bounds it is the length of the chain (verdicts,
 // sums, search), with one wave of blocks and eight loads of a thread in flight.
 constexpr int kVocabMax = 1 << 30, kDraftsMax = 1 << 20;  // (indexes of a row stay in 32 bits)
