@@ -573,8 +573,8 @@ int reserve_setup(qora_kv4 *kv) {
         cfg.attrs = &at;
         cfg.numAttrs = 1;
         int n = 0;
-        QORA_CUDA(cudaOccupancyMaxActiveClusters(&n, k_kv4_reserve, &cfg));
-        if (n > 0) break;
+        if (cudaOccupancyMaxActiveClusters(&n, k_kv4_reserve, &cfg) == cudaSuccess && n > 0) break;
+        (void)cudaGetLastError();  // (a size that it cannot place at all may be an error)
     }
     return QORA_OK;
 }
